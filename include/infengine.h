@@ -398,6 +398,87 @@ IE_API int ie_attn_prefill_core_paged(ie_context* ctx, int seq_len, int start_po
                                       const ie_bf16* d_q, const void* kv_pages, int n_pages,
                                       const int* block_table, int layer, ie_bf16* d_out);
 
+/* ---- serving many conversations over the page pool (no reference counterparts: the reference
+ * holds one sequence).  They take a ragged batch of up to IE_MAX_SEQS sequences: HOST arrays
+ * start_pos and n_new (n_new[b] >= 0 new rows of sequence b at positions start_pos[b] ..
+ * start_pos[b] + n_new[b] - 1; the batch's rows are the sequences' one after the other), read before the
+ * call returns, and block_tables as ie_decode_step_batched_paged, row b for sequence b, with
+ * start_pos[b] + n_new[b] <= 64 * table_stride.  Row-sized buffers hold the batch's rows and nothing
+ * behind them is touched.  n_q_heads: 16, 32 (this model) or 64, consecutive heads sharing a kv
+ * head.  Buffers are 16-byte aligned.  Everything runs on the context's stream, allocates nothing, and may be
+ * recorded into a graph (the lengths with it); calls that may overlap need workspaces of their own. */
+#define IE_MAX_SEQS 64
+/* Norms, rotation and append: d_qkv holds a row's projections [n_q_heads | 8 K | 8 V][128], rows
+ * qkv_stride elements apart (a multiple of 8).  Each q and k head x becomes
+ *   rope(x * rsqrt(mean(x^2) + 1e-5) * w)   (w = d_q_norm / d_k_norm [128]; NULL: rope(x))
+ * in fp32, rounded once, rope as ie_apply_rope with the tables' row of the position (rope_rows rows).
+ * q goes to d_q_out [rows][n_q_heads][128] (apart from d_qkv), k and v to the pages of layer `layer`.
+ * Page ids outside [0, n_pages) are not written; a page that several rows' tables share must not be
+ * appended to. */
+IE_API int ie_qk_norm_rope_paged(ie_context* ctx, int n_seqs, const int* start_pos,
+                                 const int* n_new, int n_q_heads, const ie_bf16* d_qkv,
+                                 long long qkv_stride, const ie_bf16* d_q_norm,
+                                 const ie_bf16* d_k_norm, const float* d_rope_cos,
+                                 const float* d_rope_sin, int rope_rows, ie_bf16* d_q_out,
+                                 void* kv_pages, int n_pages, const int* block_tables,
+                                 int table_stride, int layer);
+/* Attention of the batch's rows over the pages, with a sliding window and sinks: the row at position
+ * p sees the keys j <= p with j > p - window or j < n_sinks (window 1 .. IE_MAX_LONG_CONTEXT, the
+ * latter for none; n_sinks >= 0), scaled by 1/sqrt(128).  The new rows' own keys are read from the
+ * pages (ie_qk_norm_rope_paged has put them there).  Keys in pages outside [0, n_pages) are not seen
+ * (evicted pages; unlike ie_attn_prefill_core_paged, which reads them as zeros); a row that sees none
+ * gets zeros.  Values at keys that a row does not see never reach it, infinities and NaN included.
+ * d_q, d_out: [rows][n_q_heads][128] (bf16).  Softmax and sums in fp32; the weights are rounded to bf16
+ * for their product with V.  Few rows over many keys are split over the keys by a rule on all the
+ * lengths, on which the rounding depends.  workspace: ie_attn_window_workspace_size(rows,
+ * n_q_heads) bytes for at least the batch's rows, contents of no account. */
+IE_API size_t ie_attn_window_workspace_size(int rows, int n_q_heads);
+IE_API int ie_attn_window_paged(ie_context* ctx, int n_seqs, const int* start_pos,
+                                const int* n_new, int window, int n_sinks, int n_q_heads,
+                                const ie_bf16* d_q, const void* kv_pages, int n_pages,
+                                const int* block_tables, int table_stride, int layer,
+                                ie_bf16* d_out, void* workspace);
+/* Forks: fork i (of up to IE_MAX_SEQS) makes table row dst_rows[i] a continuation of the first n_pos[i]
+ * positions of row src_rows[i]: full pages are shared (their ids copied), the last page's
+ * n_pos[i] % 64 positions are copied, all layers, to page new_pages[i] (ignored where n_pos[i] is a multiple of
+ * 64), later entries become -1.  block_tables: device [n_rows][table_stride], updated; the four
+ * lists are HOST arrays.  A row may be forked several times, but not in the call that writes it; the
+ * new pages must be no table's, each taken once.  A source page outside [0, n_pages) is not copied. */
+IE_API int ie_kv_fork_paged(ie_context* ctx, int n_forks, const int* src_rows,
+                            const int* dst_rows, const int* n_pos, const int* new_pages,
+                            void* kv_pages, int n_pages, int* block_tables, int n_rows,
+                            int table_stride);
+/* Frees and compacts: of each table row b (device [n_rows][table_stride], n_rows up to
+ * IE_MAX_SEQS; HOST seq_lens[b] positions held) the entries stay that its next token needs: blocks
+ * of the first n_sinks positions, of positions > seq_lens[b] - window, and entries past the row's
+ * blocks (pages set aside).  seq_lens[b] = 0: the sequence is over, all its pages go.  Pages
+ * that no entry names any more are free.  The live ones come to lie at the pool's front with the
+ * fewest moves: live ids >= the live count go to the free ids below it, both in ascending order, all layers.
+ * Outputs (device): new_tables (may be block_tables), entries that went and ids outside
+ * [0, n_pages) as -1; d_remap [n_pages], a page's new id or -1; d_counts: live pages, moved pages.
+ * A page that several rows share is moved once.  n_pages up to 65536 (512 GiB).  workspace:
+ * ie_kv_compact_workspace_size(n_pages) bytes. */
+IE_API size_t ie_kv_compact_workspace_size(int n_pages);
+IE_API int ie_kv_compact_paged(ie_context* ctx, int n_rows, const int* seq_lens, int window,
+                               int n_sinks, void* kv_pages, int n_pages, const int* block_tables,
+                               int table_stride, int* new_tables, int* d_remap, int* d_counts,
+                               void* workspace);
+/* Sampling over [rows, vocab] fp32 logits (vocab up to 2^21) with the requests' own settings, DEVICE
+ * arrays [rows] each (NULL: off for all rows), from given uniforms d_uniform [rows] in [0, 1).
+ * Tokens in the order (logit descending, id ascending), weights exp((l - max) / temperature):
+ * top_k (<= 0: off) keeps the first top_k; top_p (>= 1: off) the shortest prefix of those with at least
+ * that share of their mass; min_p (<= 0: off) the tokens of at least min_p times the largest weight;
+ * the first token always stays.  The result is the first id, in id order, whose cumulative kept mass
+ * exceeds uniform x the kept mass.  temperature not > 0, or min_p > 1: the first of the largest logits.
+ * Weights and sums in 64 bits.  NaN logits count as -inf; a row without a logit above -inf gives -1.
+ * A NaN top_p or min_p is off; a uniform not > 0 counts as 0, one >= 1 draws the last kept token.
+ * workspace: ie_sample_filtered_workspace_size(rows, vocab) bytes. */
+IE_API size_t ie_sample_filtered_workspace_size(int rows, int vocab);
+IE_API int ie_sample_filtered(ie_context* ctx, int rows, int vocab, const float* d_logits,
+                              const float* d_temperature, const int* d_top_k,
+                              const float* d_top_p, const float* d_min_p, const float* d_uniform,
+                              int* d_output, void* workspace);
+
 #ifdef __cplusplus
 }
 #endif

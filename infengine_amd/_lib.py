@@ -13,6 +13,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "libinfengine_amd.so"
 # include/infengine.h constants (config.h:5-27)
 MAX_CONTEXT_LENGTH = 8192
 MAX_LONG_CONTEXT = 131072
+MAX_SEQS = 64
 VOCAB_SIZE = 128256
 NUM_LAYERS = 32
 HIDDEN_SIZE = 4096
@@ -117,6 +118,17 @@ SIGNATURES: dict[str, tuple] = {
     "ie_gemm_ex": (_i, [_p, _i, _i, _i, _i, _p, _p, _p, _p]),
     "ie_attn_prefill_core": (_i, [_p, _i, _i, _p, _p, _p, _p]),
     "ie_attn_prefill_core_paged": (_i, [_p, _i, _i, _p, _p, _i, _p, _i, _p]),
+    "ie_qk_norm_rope_paged": (_i, [_p, _i, C.POINTER(_i), C.POINTER(_i), _i, _p, C.c_longlong, _p,
+                                   _p, _p, _p, _i, _p, _p, _i, _p, _i, _i]),
+    "ie_attn_window_workspace_size": (_sz, [_i, _i]),
+    "ie_attn_window_paged": (_i, [_p, _i, C.POINTER(_i), C.POINTER(_i), _i, _i, _i, _p, _p, _i, _p,
+                                  _i, _i, _p, _p]),
+    "ie_kv_fork_paged": (_i, [_p, _i, C.POINTER(_i), C.POINTER(_i), C.POINTER(_i), C.POINTER(_i),
+                              _p, _i, _p, _i, _i]),
+    "ie_kv_compact_workspace_size": (_sz, [_i]),
+    "ie_kv_compact_paged": (_i, [_p, _i, C.POINTER(_i), _i, _i, _p, _i, _p, _i, _p, _p, _p, _p]),
+    "ie_sample_filtered_workspace_size": (_sz, [_i, _i]),
+    "ie_sample_filtered": (_i, [_p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p]),
     "ie_tune_gemv_waves": (_i, [_i]),
     "ie_tune_gemv_pairs_per_wave": (_i, [_i]),
     "ie_tune_gemm_schedule": (_i, [_i]),

@@ -249,6 +249,44 @@ int set_device(Context* c) {
   return IE_OK;
 }
 
+// ---- argument checks that the paged-serving entry points share
+template <typename... P>
+bool aligned16(P... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 15) == 0;
+}
+
+// A ragged batch: n_new[b] >= 0 new rows of sequence b from position start_pos[b] on, within its
+// table row.
+int check_batch(const char* what, int n_seqs, const int* start_pos, const int* n_new,
+                int table_stride) {
+  IE_REQUIRE(n_seqs >= 1 && n_seqs <= IE_MAX_SEQS, "%s: %d sequences out of [1, %d]", what, n_seqs,
+             IE_MAX_SEQS);
+  IE_REQUIRE(start_pos && n_new, "%s: null lengths", what);
+  IE_REQUIRE(table_stride >= 1 && table_stride <= kMaxLongCtx / kPagePos,
+             "%s: table_stride %d out of [1, %d]", what, table_stride, kMaxLongCtx / kPagePos);
+  const int cap = table_stride * kPagePos;
+  for (int b = 0; b < n_seqs; ++b)
+    IE_REQUIRE(start_pos[b] >= 0 && n_new[b] >= 0 && start_pos[b] <= cap && n_new[b] <= cap - start_pos[b],
+               "%s: sequence %d has %d rows from position %d, its table row holds %d", what, b,
+               n_new[b], start_pos[b], cap);
+  return IE_OK;
+}
+
+int check_paged(const char* what, int n_q_heads, int n_pages, int layer) {
+  IE_REQUIRE(n_q_heads == 16 || n_q_heads == 32 || n_q_heads == 64,
+             "%s: n_q_heads %d (16, 32 or 64)", what, n_q_heads);
+  IE_REQUIRE(n_pages >= 1 && layer >= 0 && layer < kLayers, "%s: n_pages %d, layer %d", what, n_pages,
+             layer);
+  return IE_OK;
+}
+
+int check_window(const char* what, int window, int n_sinks) {
+  IE_REQUIRE(window >= 1 && window <= kMaxLongCtx && n_sinks >= 0 && n_sinks <= kMaxLongCtx,
+             "%s: window %d out of [1, %d] or n_sinks %d out of [0, %d]", what, window, kMaxLongCtx,
+             n_sinks, kMaxLongCtx);
+  return IE_OK;
+}
+
 // ---- RoPE tables: rope.cu:68-96 (Llama-3 frequency scaling, theta 500000)
 void rope_tables_host(std::vector<float>& cos_t, std::vector<float>& sin_t) {
   const float theta = 500000.0f;
@@ -1633,6 +1671,160 @@ int ie_final_norm_lm_head(ie_context* c, int rows, const ie_bf16* d_x, const ie_
   IE_REQUIRE(rows >= 1 && rows <= 64, "final_norm_lm_head: rows %d out of [1, 64]", rows);
   return gemv_plain(kHidden, kEpiF32, d_x, d_norm_w, d_lm_head, nullptr, kVocab / 2, nullptr,
                     d_logits, rows, kVocab, c->stream);
+}
+
+// ---------------------------------------------------------------- paged serving
+int ie_qk_norm_rope_paged(ie_context* c, int n_seqs, const int* start_pos, const int* n_new,
+                          int n_q_heads, const ie_bf16* d_qkv, long long qkv_stride,
+                          const ie_bf16* d_q_norm, const ie_bf16* d_k_norm,
+                          const float* d_rope_cos, const float* d_rope_sin, int rope_rows,
+                          ie_bf16* d_q_out, void* kv_pages, int n_pages, const int* block_tables,
+                          int table_stride, int layer) {
+  IE_REQUIRE(c != nullptr, "qk_norm_rope_paged: null context");
+  IE_REQUIRE(d_qkv && d_rope_cos && d_rope_sin && d_q_out && kv_pages && block_tables,
+             "qk_norm_rope_paged: null pointer");
+  IE_TRY(check_batch("qk_norm_rope_paged", n_seqs, start_pos, n_new, table_stride));
+  IE_TRY(check_paged("qk_norm_rope_paged", n_q_heads, n_pages, layer));
+  IE_REQUIRE(qkv_stride >= (n_q_heads + 2 * kKVHeads) * kHeadDim && qkv_stride % 8 == 0,
+             "qk_norm_rope_paged: qkv_stride %lld (at least %d, a multiple of 8)", qkv_stride,
+             (n_q_heads + 2 * kKVHeads) * kHeadDim);
+  IE_REQUIRE(aligned16(d_qkv, d_q_norm, d_k_norm, d_rope_cos, d_rope_sin, d_q_out, kv_pages),
+             "qk_norm_rope_paged: a pointer is not 16-byte aligned");
+  for (int b = 0; b < n_seqs; ++b)
+    IE_REQUIRE(n_new[b] == 0 || start_pos[b] + n_new[b] <= rope_rows,
+               "qk_norm_rope_paged: sequence %d ends at position %d, past the %d RoPE table rows", b,
+               start_pos[b] + n_new[b], rope_rows);
+  IE_TRY(set_device(c));
+  QkNormRopeParams p{};
+  p.qkv = d_qkv;
+  p.qkv_stride = qkv_stride;
+  p.q_norm = d_q_norm;
+  p.k_norm = d_k_norm;
+  p.rope_cos = d_rope_cos;
+  p.rope_sin = d_rope_sin;
+  p.q_out = d_q_out;
+  p.k = static_cast<uint16_t*>(kv_pages) + (size_t)layer * kPageLayer;
+  p.v = p.k + (size_t)kKVHeads * kPageHead;
+  p.block_tables = block_tables;
+  p.table_stride = table_stride;
+  p.n_pages = n_pages;
+  p.heads = n_q_heads;
+  return launch_qk_norm_rope(p, SeqBatch{n_seqs, start_pos, n_new}, c->stream);
+}
+
+size_t ie_attn_window_workspace_size(int rows, int n_q_heads) {
+  return align256(std::max<size_t>(attn_window_workspace_bytes(std::max(rows, 1), std::max(n_q_heads, 1)), 1));
+}
+
+int ie_attn_window_paged(ie_context* c, int n_seqs, const int* start_pos, const int* n_new,
+                         int window, int n_sinks, int n_q_heads, const ie_bf16* d_q,
+                         const void* kv_pages, int n_pages, const int* block_tables,
+                         int table_stride, int layer, ie_bf16* d_out, void* workspace) {
+  IE_REQUIRE(c != nullptr, "attn_window_paged: null context");
+  IE_REQUIRE(d_q && kv_pages && block_tables && d_out && workspace,
+             "attn_window_paged: null pointer");
+  IE_TRY(check_batch("attn_window_paged", n_seqs, start_pos, n_new, table_stride));
+  IE_TRY(check_paged("attn_window_paged", n_q_heads, n_pages, layer));
+  IE_TRY(check_window("attn_window_paged", window, n_sinks));
+  IE_REQUIRE(aligned16(d_q, kv_pages, d_out, workspace),
+             "attn_window_paged: a pointer is not 16-byte aligned");
+  IE_TRY(set_device(c));
+  AttnWindowParams p{};
+  p.q = d_q;
+  p.k = static_cast<const uint16_t*>(kv_pages) + (size_t)layer * kPageLayer;
+  p.v = p.k + (size_t)kKVHeads * kPageHead;
+  p.out = d_out;
+  p.block_tables = block_tables;
+  p.table_stride = table_stride;
+  p.n_pages = n_pages;
+  p.window = window;
+  p.n_sinks = n_sinks;
+  p.group_shift = n_q_heads == 16 ? 1 : n_q_heads == 32 ? 2 : 3;
+  return launch_attn_window(p, SeqBatch{n_seqs, start_pos, n_new}, workspace, c->stream);
+}
+
+int ie_kv_fork_paged(ie_context* c, int n_forks, const int* src_rows, const int* dst_rows,
+                     const int* n_pos, const int* new_pages, void* kv_pages, int n_pages,
+                     int* block_tables, int n_rows, int table_stride) {
+  IE_REQUIRE(c != nullptr, "kv_fork_paged: null context");
+  IE_REQUIRE(src_rows && dst_rows && n_pos && new_pages && kv_pages && block_tables,
+             "kv_fork_paged: null pointer");
+  IE_REQUIRE(n_forks >= 0 && n_forks <= IE_MAX_SEQS, "kv_fork_paged: %d forks out of [0, %d]",
+             n_forks, IE_MAX_SEQS);
+  IE_REQUIRE(n_pages >= 1 && n_rows >= 1, "kv_fork_paged: n_pages %d, n_rows %d", n_pages, n_rows);
+  IE_REQUIRE(table_stride >= 1 && table_stride <= kMaxLongCtx / kPagePos,
+             "kv_fork_paged: table_stride %d out of [1, %d]", table_stride, kMaxLongCtx / kPagePos);
+  IE_REQUIRE(aligned16(kv_pages), "kv_fork_paged: kv_pages is not 16-byte aligned");
+  for (int i = 0; i < n_forks; ++i) {
+    IE_REQUIRE(src_rows[i] >= 0 && src_rows[i] < n_rows && dst_rows[i] >= 0 && dst_rows[i] < n_rows,
+               "kv_fork_paged: fork %d is of row %d to row %d of %d", i, src_rows[i], dst_rows[i], n_rows);
+    IE_REQUIRE(n_pos[i] >= 0 && n_pos[i] <= table_stride * kPagePos,
+               "kv_fork_paged: fork %d has %d positions, a row holds %d", i, n_pos[i],
+               table_stride * kPagePos);
+    const bool copies = n_pos[i] % kPagePos != 0;
+    IE_REQUIRE(!copies || (new_pages[i] >= 0 && new_pages[i] < n_pages),
+               "kv_fork_paged: fork %d takes page %d of %d", i, new_pages[i], n_pages);
+    for (int j = 0; j < n_forks; ++j) {
+      IE_REQUIRE(dst_rows[i] != src_rows[j], "kv_fork_paged: row %d is forked from and to", dst_rows[i]);
+      IE_REQUIRE(j == i || dst_rows[i] != dst_rows[j], "kv_fork_paged: row %d is forked to twice",
+                 dst_rows[i]);
+      IE_REQUIRE(j == i || !copies || n_pos[j] % kPagePos == 0 || new_pages[i] != new_pages[j],
+                 "kv_fork_paged: page %d is taken twice", new_pages[i]);
+    }
+  }
+  if (n_forks == 0) return IE_OK;
+  IE_TRY(set_device(c));
+  return launch_kv_fork(n_forks, src_rows, dst_rows, n_pos, new_pages,
+                        static_cast<uint16_t*>(kv_pages), n_pages, block_tables, table_stride,
+                        c->stream);
+}
+
+size_t ie_kv_compact_workspace_size(int n_pages) {
+  return align256(kv_compact_workspace_bytes(std::max(n_pages, 1)));
+}
+
+int ie_kv_compact_paged(ie_context* c, int n_rows, const int* seq_lens, int window, int n_sinks,
+                        void* kv_pages, int n_pages, const int* block_tables, int table_stride,
+                        int* new_tables, int* d_remap, int* d_counts, void* workspace) {
+  IE_REQUIRE(c != nullptr, "kv_compact_paged: null context");
+  IE_REQUIRE(seq_lens && kv_pages && block_tables && new_tables && d_remap && d_counts && workspace,
+             "kv_compact_paged: null pointer");
+  IE_REQUIRE(n_rows >= 1 && n_rows <= IE_MAX_SEQS, "kv_compact_paged: %d rows out of [1, %d]", n_rows,
+             IE_MAX_SEQS);
+  IE_REQUIRE(n_pages >= 1 && n_pages <= kCompactMaxPages, "kv_compact_paged: %d pages out of [1, %d]",
+             n_pages, kCompactMaxPages);
+  IE_REQUIRE(table_stride >= 1 && table_stride <= kMaxLongCtx / kPagePos,
+             "kv_compact_paged: table_stride %d out of [1, %d]", table_stride, kMaxLongCtx / kPagePos);
+  IE_TRY(check_window("kv_compact_paged", window, n_sinks));
+  IE_REQUIRE(aligned16(kv_pages, workspace), "kv_compact_paged: a pointer is not 16-byte aligned");
+  for (int r = 0; r < n_rows; ++r)
+    IE_REQUIRE(seq_lens[r] >= 0 && seq_lens[r] <= table_stride * kPagePos,
+               "kv_compact_paged: row %d has %d positions, a row holds %d", r, seq_lens[r],
+               table_stride * kPagePos);
+  IE_TRY(set_device(c));
+  return launch_kv_compact(n_rows, seq_lens, window, n_sinks, static_cast<uint16_t*>(kv_pages),
+                           n_pages, block_tables, table_stride, new_tables, d_remap, d_counts,
+                           workspace, c->stream);
+}
+
+size_t ie_sample_filtered_workspace_size(int rows, int vocab) {
+  return align256(sample_filtered_workspace_bytes(std::max(rows, 1), std::max(vocab, 1)));
+}
+
+int ie_sample_filtered(ie_context* c, int rows, int vocab, const float* d_logits,
+                       const float* d_temperature, const int* d_top_k, const float* d_top_p,
+                       const float* d_min_p, const float* d_uniform, int* d_output,
+                       void* workspace) {
+  IE_REQUIRE(c != nullptr, "sample_filtered: null context");
+  IE_REQUIRE(d_logits && d_uniform && d_output && workspace, "sample_filtered: null pointer");
+  IE_REQUIRE(rows >= 1 && rows <= 65535, "sample_filtered: rows=%d", rows);
+  IE_REQUIRE(vocab >= 1 && vocab <= kSampleMaxVocab, "sample_filtered: vocab %d out of [1, %d]",
+             vocab, kSampleMaxVocab);
+  IE_REQUIRE(aligned16(workspace), "sample_filtered: workspace is not 16-byte aligned");
+  IE_TRY(set_device(c));
+  const SampleParams p{d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_output,
+                       rows, vocab};
+  return launch_sample_filtered(p, workspace, c->stream);
 }
 
 int ie_model_weights_from_safetensors(ie_model_weights* out, const char* const* paths,

@@ -295,4 +295,74 @@ constexpr size_t kAttnPrefillPartRow = (size_t)kQHeads * (kHeadDim + 2);
 int attn_prefill_splits(int S, int nkeys, int part_rows);
 int launch_attn_prefill(const AttnPrefillParams& p, hipStream_t st);
 
+// ------------------------------------------------------------ paged serving (k_paged.hip,
+// k_attn_window.hip, k_sample_filtered.hip)
+constexpr int kMaxSeqs = IE_MAX_SEQS;
+// A ragged batch as its host arrays: rows of the sequences one after the other.
+struct SeqBatch {
+  int n;
+  const int* start;  // position of the sequence's first new row
+  const int* n_new;
+};
+
+struct QkNormRopeParams {
+  const uint16_t* qkv;   // [rows][heads + 16][128], rows qkv_stride elements apart
+  long long qkv_stride;
+  const uint16_t* q_norm;  // [128] or nullptr
+  const uint16_t* k_norm;
+  const float* rope_cos;   // [][64]
+  const float* rope_sin;
+  uint16_t* q_out;         // [rows][heads][128]
+  uint16_t* k;             // the layer's head-0 K / V planes of page 0 (pages kPageElems apart)
+  uint16_t* v;
+  const int* block_tables;
+  int table_stride, n_pages, heads, n_seqs, rows;
+  int start[kMaxSeqs], row_end[kMaxSeqs];  // (set by the launcher, as n_seqs and rows)
+};
+int launch_qk_norm_rope(QkNormRopeParams p, const SeqBatch& s, hipStream_t st);
+
+struct AttnWindowParams {
+  const uint16_t* q;   // [rows][heads][128], rotated
+  const uint16_t* k;   // the layer's head-0 K / V planes of page 0
+  const uint16_t* v;
+  uint16_t* out;       // [rows][heads][128]
+  const int* block_tables;
+  int table_stride, n_pages, window, n_sinks;
+  int group_shift;     // log2 of the q heads per kv head
+  // set by the launcher
+  float* part;         // splits' partials [slots][heads][128], then (m, l)
+  float* part_ml;
+  int n_seqs;
+  int start[kMaxSeqs], row_end[kMaxSeqs];  // first new position; rows up to and with the sequence's
+  int item_end[kMaxSeqs];                  // (row block, split) items up to and with the sequence's
+  int splits[kMaxSeqs], part0[kMaxSeqs];   // key splits; first partial row
+};
+constexpr int kMaxSplits = 64;
+constexpr int kAttnWindowPartRows = 4096;
+size_t attn_window_workspace_bytes(int rows, int heads);
+int launch_attn_window(AttnWindowParams p, const SeqBatch& s, void* workspace, hipStream_t st);
+
+int launch_kv_fork(int n_forks, const int* src_rows, const int* dst_rows, const int* n_pos,
+                   const int* new_pages, uint16_t* pages, int n_pages, int* tables, int stride,
+                   hipStream_t st);
+constexpr int kCompactMaxPages = 1 << 16;  // 512 GiB of pages
+size_t kv_compact_workspace_bytes(int n_pages);
+int launch_kv_compact(int n_rows, const int* seq_lens, int window, int n_sinks, uint16_t* pages,
+                      int n_pages, const int* tables, int stride, int* new_tables, int* remap,
+                      int* counts, void* workspace, hipStream_t st);
+
+constexpr int kSampleMaxVocab = 1 << 21;
+struct SampleParams {
+  const float* logits;        // [rows][vocab]
+  const float* temperature;   // [rows] each, or nullptr
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* uniform;
+  int* out;
+  int rows, vocab;
+};
+size_t sample_filtered_workspace_bytes(int rows, int vocab);
+int launch_sample_filtered(const SampleParams& p, void* workspace, hipStream_t st);
+
 }  // namespace ie

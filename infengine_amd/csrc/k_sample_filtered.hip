@@ -111,62 +111,88 @@ __device__ __forceinline__ double exp_neg(double x) {
   return ldexp(y, (int)n);
 }
 
-// Weight of a token in a bin below kBins (l above -inf, within 33 nats of the max).
+// Weight of a token: nothing past 33 nats below the max (it rounds to no unit), -inf, NaN.
 __device__ __forceinline__ double weight(float l, float mx, double inv_t) {
-  return l == mx ? 1.0 : exp_neg(((double)l - (double)mx) * inv_t);  // (infinite maxima too)
+  if (l == mx) return 1.0;  // (infinite maxima too)
+  const double x = ((double)l - (double)mx) * inv_t;
+  return x > -33.0 ? exp_neg(x) : 0.0;
 }
 __device__ __forceinline__ u64 fixed(double w) { return (u64)(w * kUnit + 0.5); }
 
 // The token's bin below that of `mx`, kBins for those that weigh nothing (further below, -inf, NaN).
-// Non-decreasing in falling l, and the same steps whatever mx: B(l) = floor(8 l / T).
+// Non-decreasing in falling l, and the same steps whatever mx: B(l) = floor(l x scale) in fp32, whose
+// rounding is monotone, and whose differences below kBins are exact at any size of l.  scale = 8 / T,
+// held finite: below that T bins are wider than 1/8 nat, and tokens past kBins only weigh less.
 struct Binner {
-  float mx;
-  double scale, top;
-  __device__ Binner(float m, double inv_t) : mx(m), scale(8.0 * inv_t), top(floor((double)m * scale)) {}
+  float mx, scale, top;
+  __device__ Binner(float m, double inv_t)
+      : mx(m), scale((float)fmin(8.0 * inv_t, 3.4e38)), top(floorf(m * scale)) {}
   __device__ __forceinline__ int operator()(float l) const {
-    const double d = top - floor((double)l * scale);
-    return l == mx ? 0 : l > -INFINITY && d < (double)kBins ? max((int)d, 0) : kBins;
+    const float d = top - floorf(l * scale);
+    return l == mx ? 0 : l > -INFINITY && d < (float)kBins ? max((int)d, 0) : kBins;
   }
 };
 
+// Lane moves within the VALU (the LDS-crossbar shuffles cost over ten times as much): CTRL a DPP control,
+// lanes without a source and rows outside ROWS get 0.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp_move(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(
+        T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
+  } else {
+    const u64 x = __builtin_bit_cast(u64, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(T, (u64)hi << 32 | lo);
+  }
+}
+// Inclusive scan of each row of 16 lanes (row_shr 1, 2, 4, 8), and of the wave (row_bcast 15, 31).
+template <typename T>
+__device__ __forceinline__ T row_scan_inc(T v) {
+  v += dpp_move<0x111, 0xF>(v);
+  v += dpp_move<0x112, 0xF>(v);
+  v += dpp_move<0x114, 0xF>(v);
+  v += dpp_move<0x118, 0xF>(v);
+  return v;
+}
 template <typename T>
 __device__ __forceinline__ T wave_scan_inc(T v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T w = __shfl_up(v, o, 64);
-    if (lane >= o) v += w;
-  }
+  v = row_scan_inc(v);
+  v += dpp_move<0x142, 0xA>(v);
+  v += dpp_move<0x143, 0xC>(v);
   return v;
+}
+// The value of one lane (the same lane for the whole wave).
+template <typename T>
+__device__ __forceinline__ T lane_value(T v, int lane) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    const u64 x = __builtin_bit_cast(u64, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane);
+    return __builtin_bit_cast(T, (u64)hi << 32 | lo);
+  }
 }
 
 // Inclusive scan over the workgroup and its total; `red` is a scratch of kWaves values.
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, T* red, T* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T inc = wave_scan_inc(v);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T inc = wave_scan_inc(v);
   __syncthreads();
   if (lane == 63) red[wave] = inc;
   __syncthreads();
-  T all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) inc += red[w];
-    all += red[w];
-  }
-  *total = all;
-  return inc;
+  static_assert(kWaves == 16, "a wave a lane of a row");
+  const T own = red[lane & 15], upto = row_scan_inc(own);
+  *total = lane_value(upto, 15);
+  return inc + lane_value(upto - own, wave);
 }
 
 __device__ __forceinline__ u64 block_sum(u64 v, u64* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  u64 all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) all += red[w];
+  u64 all;
+  block_scan(v, red, &all);
   return all;
 }
 
@@ -249,7 +275,8 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p,
   __shared__ double part_m[4][kBins];
   __shared__ CutBins s_cut;
   __shared__ int s_cnt[kRound * kWaves];
-  const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Row& R = row_state(ws, row, p.vocab);
   const float* L = p.logits + (size_t)row * p.vocab;
   const int cl = chunk_len(p.vocab), beg = min(p.vocab, c * cl), end = min(p.vocab, beg + cl);
@@ -296,11 +323,11 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p,
         int j = 0;
         while (j < 3 && a + h[j] < target) a += h[j++];
         const int bin4 = hit ? 4 * lane + j : kBins;
-        *above = __shfl(a, at, 64);
-        return __shfl(bin4, at, 64);
+        *above = lane_value(a, at);
+        return lane_value(bin4, at);
       };
       u64 k_above = 0;
-      double mass_k = __shfl(minc, 63, 64), mass_k_incl = mass_k, mass_p = 0.0, none;
+      double mass_k = lane_value(minc, 63), mass_k_incl = mass_k, mass_p = 0.0, none;
       if (s.top_k) {
         cut.k_bin = first_bin(ninc, nsum, n, (u64)s.top_k, &k_above);
         if (cut.k_bin == kBins) {
@@ -313,8 +340,8 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p,
             if (4 * lane + j < cut.k_bin) below += m[j];
             if (4 * lane + j == cut.k_bin) own = m[j];
           }
-          mass_k = __shfl(below, cut.k_bin >> 2, 64);
-          mass_k_incl = mass_k + __shfl(own, cut.k_bin >> 2, 64);
+          mass_k = lane_value(below, cut.k_bin >> 2);
+          mass_k_incl = mass_k + lane_value(own, cut.k_bin >> 2);
           cut.lo = cut.k_bin;
         }
       }
@@ -373,12 +400,12 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p,
 #pragma unroll
     for (int u = 0; u < kRound; ++u) {
       const int slot = u * kWaves + wave;
-      const int upto = __shfl(inc, slot >> 1, 64) - __shfl(slot & 1 ? b2 : a + b2, slot >> 1, 64);
+      const int upto = lane_value(inc, slot >> 1) - lane_value(slot & 1 ? b2 : a + b2, slot >> 1);
       const u64 vote = __ballot(hits >> u & 1);
       if (hits >> u & 1)
         list[listed + upto + __popcll(vote & ((1ull << lane) - 1))] = Listed{v[u], i + tid + u * kThreads};
     }
-    listed += __shfl(inc, 63, 64);
+    listed += lane_value(inc, 63);
   }
   low = block_sum(low, red);
   if (tid == 0) {
@@ -426,7 +453,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     return;
   }
   const Binner bin(mx, s.inv_t);
-  const int lo = R.cut_bins[0], p_lo = R.cut_bins[1], p_hi = R.cut_bins[2], k_bin = R.cut_bins[3];
+  const int p_lo = R.cut_bins[1], p_hi = R.cut_bins[2], k_bin = R.cut_bins[3];
   if (tid < 64) {
     const int n = tid < kChunks ? R.n_listed[tid] : 0;
     const int inc = wave_scan_inc(n);
@@ -541,27 +568,27 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
                  },
                  [&](Listed t) { return mass(t.l); }, want > 1.0 ? (u64)want : (u64)1);
   }
-  // (a listed token that weighs nothing has no place in either)
+  // (what is kept lies at or above the cut, the bins above it with it; a cut keeps all that weighs
+  // something where there is none)
   const auto kept_mass = [&](float l, int id) -> u64 {
-    const int b = bin(l);
-    if (b >= kBins || !(b < lo || cut.keeps(l, id))) return 0;
+    if (!cut.keeps(l, id)) return 0;
     const double w = weight(l, mx, s.inv_t);
     return !s.m || w >= (double)s.min_p ? fixed(w) : 0;
   };
   // the chunks' kept masses
   for (int j = tid; j < n; j += kThreads) {
     const Listed t = token(j);
-    if (!cut.keeps(t.l, t.id)) continue;
+    const u64 q = kept_mass(t.l, t.id);
+    if (!q) continue;
     int c = 0;
 #pragma unroll
     for (int k = 1; k < kChunks; ++k) c += j >= offset[k];
-    const u64 q = kept_mass(t.l, t.id);
-    if (q) atomicAdd(&kept_of[c], q);
+    atomicAdd(&kept_of[c], q);
   }
   __syncthreads();
   if (tid < 64) {
     const u64 own = tid < kChunks ? kept_of[tid] : 0, inc = wave_scan_inc(own);
-    const u64 z = __shfl(inc, 63, 64);
+    const u64 z = lane_value(inc, 63);
     const float u = p.uniform[row];
     const double x = (double)z * (u > 0.f ? (double)u : 0.0);
     const u64 at = x < (double)z ? min((u64)x, z - 1) : z - 1;

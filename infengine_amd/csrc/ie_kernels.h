@@ -361,8 +361,9 @@ struct SampleParams {
   const float* uniform;
   int* out;
   int rows, vocab;
+  int chunks = 0;             // set by the launcher
 };
 size_t sample_filtered_workspace_bytes(int rows, int vocab);
-int launch_sample_filtered(const SampleParams& p, void* workspace, hipStream_t st);
+int launch_sample_filtered(SampleParams p, void* workspace, hipStream_t st);
 
 }  // namespace ie

@@ -9,17 +9,18 @@
 //   kept = the first max(1, min(n_p, n_m)); the token: the first id, in id order, whose kept
 //          cumulative mass exceeds u x the kept mass.
 // Greedy rows (T not > 0, min_p > 1) are top_k = 1.  Weights are computed in fp64 and added in 64-bit
-// fixed point: sums are exact and free of order, and a draw next to a border of the distribution
-// falls as it does in 64 bits.  Kept masses are in 2^-42 units, so that the tokens below exp(-30)
-// of the largest weigh nothing.
+// fixed point within a chunk of the row (exact, free of order), the chunks' sums in fp64 in
+// order: a draw next to a border of the distribution falls as it does in 64 bits.  Tokens below
+// exp(-30) of the largest weigh nothing.
 //
-// A row is cut into kChunks chunks, a workgroup each, over three launches:
+// A row is cut into 8 or 16 chunks, a workgroup each, over three launches:
 //   hist    the chunk's max, and its tokens binned by B(l) = floor(8 l / T), which is the same scale
 //           in every chunk: counts and masses of the bins from the chunk max's down (relative to the chunk
-//           max: nothing of another chunk is needed).  Only what the row's settings need.
+//           max: nothing of another chunk is needed).  Only what the row's settings need; with top_k only
+//           the bins that can hold the chunk's first top_k
 //   gather  every workgroup adds up the chunks' histograms and finds the bins that hold the cuts (the
-//           same in all of them), then sums the mass of its tokens in the bins above (kept for
-//           certain) and lists those in the cuts' bins, in id order
+//           same in all of them), then the mass of its tokens in the bins above (kept for certain) and
+//           the list of those in the cuts' bins, in id order
 //   finish  a workgroup per row: the cuts by a radix select over the listed tokens, the chunks' kept
 //           masses, the chunk that holds the draw, its token by a scan in id order
 // The bins are 1/8 of a nat wide: of 128256 N(0, 2) logits at T = 1 at most 3200 are listed.  The list
@@ -33,18 +34,19 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kChunks = 16, kBins = 256;
+constexpr int kChunks = 16, kBins = 256;    // (at most 16 chunks)
 constexpr int kRound = 8;                   // logits a thread and round
-constexpr double kUnit = 4398046511104.0;   // 2^42: sums over kSampleMaxVocab = 2^21 tokens fit 63 bits
-constexpr double kBinUnit = 70368744177664.0;  // 2^46: a chunk's sums (2^17 tokens) fit 63 bits
-static_assert(kSampleMaxVocab / kChunks <= 1 << 17, "a bin's mass in 64 bits");
+constexpr double kUnit = 4398046511104.0;   // 2^42: masses of listed tokens (2^21 fit 63 bits)
+constexpr double kChunkUnit = 35184372088832.0;  // 2^45: of a chunk's tokens (2^18 fit 63 bits)
+static_assert(kSampleMaxVocab <= 1 << 21 && kSampleMaxVocab / (kChunks / 2) <= 1 << 18, "sums in 64 bits");
 
 // A row's state in the workspace; the listed tokens follow it, chunk by chunk.
 struct Row {
   float pmax[kChunks];
   int n_listed[kChunks];
-  u64 kept[kChunks];          // mass of the chunk's tokens in bins above the cuts'
-  int cut_bins[4];            // lo, p_lo, p_hi, k_bin
+  u64 total[kChunks];         // rows without cuts: the chunk's mass, relative to its max
+  double kept[kChunks];       // mass of the chunk's tokens in bins above the cuts'
+  int p_lo, p_hi, k_bin;
   u64 k_above;                // tokens in the bins above k_bin
   double mass_k, mass_p;      // masses of the bins above k_bin, above p_lo
   unsigned int count[kChunks][kBins];
@@ -55,17 +57,20 @@ struct Listed {
   int id;
 };
 
-__host__ __device__ __forceinline__ int chunk_len(int vocab) { return (vocab + kChunks - 1) / kChunks; }
+// Chunks a row: 16 for few rows, where a chunk's latency counts; 8 from 32 rows on, whose 1024-thread
+// workgroups then run in one turn of the chip.
+__host__ __device__ __forceinline__ int row_chunks(int rows) { return rows < 32 ? kChunks : kChunks / 2; }
+__host__ __device__ __forceinline__ int chunk_len(int vocab, int chunks) { return (vocab + chunks - 1) / chunks; }
 __host__ __device__ __forceinline__ size_t row_bytes(int vocab) {
   return ((sizeof(Row) + 255) & ~(size_t)255) +
-         (((size_t)chunk_len(vocab) * kChunks * sizeof(Listed) + 255) & ~(size_t)255);
+         ((((size_t)vocab + kChunks) * sizeof(Listed) + 255) & ~(size_t)255);
 }
 __device__ __forceinline__ Row& row_state(void* ws, int row, int vocab) {
   return *reinterpret_cast<Row*>(static_cast<char*>(ws) + row * row_bytes(vocab));
 }
-__device__ __forceinline__ Listed* row_list(Row& R, int chunk, int vocab) {
+__device__ __forceinline__ Listed* row_list(Row& R, int chunk, int len) {
   return reinterpret_cast<Listed*>(reinterpret_cast<char*>(&R) + ((sizeof(Row) + 255) & ~(size_t)255)) +
-         (size_t)chunk * chunk_len(vocab);
+         (size_t)chunk * len;
 }
 
 // A row's settings.
@@ -74,6 +79,7 @@ struct Setting {
   int top_k;       // 0: off
   float top_p;     // used when p
   float min_p;
+  int m_bins;      // no token of a bin past it reaches min_p (used when m)
   bool p, m;
 };
 __device__ __forceinline__ Setting setting(const SampleParams& p, int row) {
@@ -88,36 +94,56 @@ __device__ __forceinline__ Setting setting(const SampleParams& p, int row) {
   s.top_p = tp > 0.f ? tp : 0.f;
   s.m = !greedy && mp > 0.f;
   s.min_p = mp;
+  s.m_bins = s.m ? (int)fminf(-8.0f * __logf(mp), (float)kBins) + 2 : 0;
   return s;
 }
 
-// e^x for x <= 0, in 64 bits: 2^n e^r with |r| <= ln 2 / 2 and the exponential series to r^11 / 11!
-// (what is left out is below 7e-15 of it).
-__device__ __forceinline__ double exp_neg(double x) {
-  const double n = rint(x * 1.4426950408889634);
-  const double r = fma(n, -0.6931471805599453, x);
-  double y = 1.0 / 39916800.0;
-  y = fma(y, r, 1.0 / 3628800.0);
-  y = fma(y, r, 1.0 / 362880.0);
-  y = fma(y, r, 1.0 / 40320.0);
-  y = fma(y, r, 1.0 / 5040.0);
-  y = fma(y, r, 1.0 / 720.0);
-  y = fma(y, r, 1.0 / 120.0);
-  y = fma(y, r, 1.0 / 24.0);
-  y = fma(y, r, 1.0 / 6.0);
-  y = fma(y, r, 0.5);
-  y = fma(y, r, 1.0);
-  y = fma(y, r, 1.0);
-  return ldexp(y, (int)n);
+// 2^(j / 64), for the weights: held in LDS by each workgroup that computes many.
+constexpr double two_to(double x) {  // 0 <= x < 1, by the exponential series
+  const double r = x * 0.6931471805599453;
+  double y = 1.0;
+  for (int k = 24; k > 0; --k) y = 1.0 + y * r / k;
+  return y;
 }
+struct Powers {
+  double v[64];
+};
+constexpr Powers make_powers() {
+  Powers t{};
+  for (int j = 0; j < 64; ++j) t.v[j] = two_to(j / 64.0);
+  return t;
+}
+__device__ const Powers kPowers = make_powers();
 
-// Weight of a token: nothing past 33 nats below the max (it rounds to no unit), -inf, NaN.
-__device__ __forceinline__ double weight(float l, float mx, double inv_t) {
-  if (l == mx) return 1.0;  // (infinite maxima too)
-  const double x = ((double)l - (double)mx) * inv_t;
-  return x > -33.0 ? exp_neg(x) : 0.0;
+// Weights exp((l - mx) / T) of a row, nothing for tokens past 33 nats below mx (they round to no
+// unit), -inf and NaN.  (l - mx) / T = (64 e + j + f) ln 2 / 64 with |f| <= 1/2: 2^e 2^(j/64) times the
+// exponential series of f ln 2 / 64 to the fifth power (what is left out is below 4e-17 of it).  Two
+// additions of 1.5 x 2^52 round to whole numbers.
+struct Weigher {
+  const double* powers;  // the table in LDS
+  double mx, scale;      // 64 / (T ln 2)
+  float fmx;
+  __device__ Weigher(const double* t, float m, double inv_t)
+      : powers(t), mx(m), scale(inv_t * 92.33248261893583), fmx(m) {}
+  __device__ __forceinline__ double operator()(float l) const {
+    constexpr double c1 = 0.010830424696249145, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4,
+                     c5 = c4 * c1 / 5, whole = 6755399441055744.0;
+    const double z = ((double)l - mx) * scale;
+    const double t = z + whole, f = z - (t - whole);
+    double y = fma(f, c5, c4);
+    y = fma(y, f, c3);
+    y = fma(y, f, c2);
+    y = fma(y, f, c1);
+    y = fma(y, f, 1.0);
+    const int n = (int)__double_as_longlong(t);
+    const u64 w = (u64)__double_as_longlong(y * powers[n & 63]) + ((u64)(uint32_t)(n >> 6) << 52);
+    return l == fmx ? 1.0 : z > -33.0 * 92.33248261893583 ? __longlong_as_double((long long)w) : 0.0;
+  }
+};
+// w in whole units (2^42 or 2^45) for 0 <= w <= 1.
+__device__ __forceinline__ u64 in_units(double w, double unit) {
+  return (u64)__double_as_longlong(fma(w, unit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
 }
-__device__ __forceinline__ u64 fixed(double w) { return (u64)(w * kUnit + 0.5); }
 
 // The token's bin below that of `mx`, kBins for those that weigh nothing (further below, -inf, NaN).
 // Non-decreasing in falling l, and the same steps whatever mx: B(l) = floor(l x scale) in fp32, whose
@@ -190,59 +216,121 @@ __device__ __forceinline__ T block_scan(T v, T* red, T* total) {
   return inc + lane_value(upto - own, wave);
 }
 
-__device__ __forceinline__ u64 block_sum(u64 v, u64* red) {
-  u64 all;
+template <typename T>
+__device__ __forceinline__ T block_sum(T v, T* red) {
+  T all;
   block_scan(v, red, &all);
   return all;
 }
 
-// kRound logits of [i, end) a thread, kThreads apart (past the end: NaN, which weighs nothing).
+// Thread t's kRound logits of a round of the ids [i, end): a wave has 64 kRound ids in a row, 64 a load
+// (past the end: NaN, which weighs nothing).
+__device__ __forceinline__ int round_id(int i, int u) {
+  return i + (int)(threadIdx.x >> 6) * (64 * kRound) + u * 64 + (int)(threadIdx.x & 63);
+}
 __device__ __forceinline__ void load_round(const float* L, int i, int end, float (&v)[kRound]) {
 #pragma unroll
-  for (int u = 0; u < kRound; ++u) v[u] = L[min(i + u * kThreads, end - 1)];
+  for (int u = 0; u < kRound; ++u) v[u] = L[min(round_id(i, u), end - 1)];
 #pragma unroll
   for (int u = 0; u < kRound; ++u)
-    if (i + u * kThreads >= end) v[u] = NAN;
+    if (round_id(i, u) >= end) v[u] = NAN;
 }
 
-__global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p, void* ws) {
+// First of the wave's 256 bins (4 a lane: inc, own the inclusive scan and the lane's own sum of h) whose
+// cumulative value reaches the target, and what lies above it; kBins: none.
+template <typename T>
+__device__ __forceinline__ int first_bin(T inc, T own, const T (&h)[4], T target, T* above) {
+  const u64 hit = __ballot(inc >= target);
+  const int at = hit ? __ffsll((long long)hit) - 1 : 63;
+  T a = inc - own;
+  int j = 0;
+  while (j < 3 && a + h[j] < target) a += h[j++];
+  const int bin = hit ? 4 * (int)(threadIdx.x & 63) + j : kBins;
+  *above = lane_value(a, at);
+  return lane_value(bin, at);
+}
+
+// (64 VGPRs: two workgroups a CU)
+__global__ __launch_bounds__(kThreads, 8) void sample_hist_kernel(SampleParams p, void* ws) {
   // four histograms, by lane: lanes of a wave that meet in a bin wait for each other
   constexpr int kCopies = 4;
   __shared__ unsigned int count[kCopies * kBins];
   __shared__ u64 mass[kCopies * kBins];
-  __shared__ float red[kWaves];
+  __shared__ double powers[64];
+  __shared__ float redf[kWaves];
+  __shared__ u64 red[kWaves];
+  __shared__ int s_bin;
   const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   Row& R = row_state(ws, row, p.vocab);
   const float* L = p.logits + (size_t)row * p.vocab;
-  const int cl = chunk_len(p.vocab), beg = min(p.vocab, c * cl), end = min(p.vocab, beg + cl);
+  const int cl = chunk_len(p.vocab, p.chunks), beg = min(p.vocab, c * cl), end = min(p.vocab, beg + cl);
   const Setting s = setting(p, row);
   static_assert(kCopies * kBins == kThreads, "a bin a thread");
   count[tid] = 0;
   mass[tid] = 0;
-  float v[kRound], mx = -INFINITY;
+  if (tid < 64) powers[tid] = kPowers.v[tid];
+  float v[kRound], own_max = -INFINITY;
   for (int i = beg; i < end; i += kRound * kThreads) {
-    load_round(L, i + tid, end, v);
+    load_round(L, i, end, v);
 #pragma unroll
-    for (int u = 0; u < kRound; ++u) mx = fmaxf(mx, v[u]);  // (of a NaN and a number, the number)
+    for (int u = 0; u < kRound; ++u) own_max = fmaxf(own_max, v[u]);  // (of a NaN and a number, the number)
   }
-  mx = wave_max(mx);
-  if (lane == 0) red[tid >> 6] = mx;
+  float mx = wave_max(own_max);
+  if (lane == 0) redf[tid >> 6] = mx;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red[w]);
+  mx = wave_max(redf[lane & (kWaves - 1)]);
   if (tid == 0) R.pmax[c] = mx;
-  if (!s.top_k && !s.p) return;
+  const Weigher weight(powers, mx, s.inv_t);
+  const bool one_round = end - beg <= kRound * kThreads;
+  if (!s.top_k && !s.p) {
+    if (s.m) return;
+    u64 sum = 0;
+    if (mx > -INFINITY)
+      for (int i = beg; i < end; i += kRound * kThreads) {
+        if (!one_round) load_round(L, i, end, v);
+#pragma unroll
+        for (int u = 0; u < kRound; ++u) sum += in_units(weight(v[u]), kChunkUnit);
+      }
+    sum = block_sum(sum, red);
+    if (tid == 0) R.total[c] = sum;
+    return;
+  }
   if (mx > -INFINITY) {
     const Binner bin(mx, s.inv_t);
     const int copy = (lane & (kCopies - 1)) * kBins;
+    int last = kBins - 1;
+    if (s.top_k) {
+      // as many threads' largest tokens as top_k lie in the bins up to `last`: the chunk's first top_k do
+      // too, and the bins behind need no count (they keep those threads' part of it)
+      const int b = bin(own_max);
+      if (b < kBins) atomicAdd(&count[copy + b], 1u);
+      __syncthreads();
+      if (tid < 64) {
+        unsigned int h[4], own = 0, above;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          h[j] = 0;
+#pragma unroll
+          for (int k = 0; k < kCopies; ++k) h[j] += count[k * kBins + 4 * lane + j];
+          own += h[j];
+        }
+        const int at = first_bin(wave_scan_inc(own), own, h, (unsigned int)s.top_k, &above);
+        if (lane == 0) s_bin = min(at, kBins - 1);
+      }
+      __syncthreads();
+      last = s_bin;
+    }
+    bool counted = false;  // the thread's largest token, once
     for (int i = beg; i < end; i += kRound * kThreads) {
-      if (end - beg > kRound * kThreads) load_round(L, i + tid, end, v);
+      if (!one_round) load_round(L, i, end, v);
 #pragma unroll
       for (int u = 0; u < kRound; ++u) {
         const int b = bin(v[u]);
-        if (b == kBins) continue;
-        if (s.top_k) atomicAdd(&count[copy + b], 1u);
-        if (s.p) atomicAdd(&mass[copy + b], (u64)(weight(v[u], mx, s.inv_t) * kBinUnit + 0.5));
+        if (b > last) continue;
+        const bool again = !counted && v[u] == own_max;
+        counted |= again;
+        if (s.top_k && !again) atomicAdd(&count[copy + b], 1u);
+        if (s.p) atomicAdd(&mass[copy + b], in_units(weight(v[u]), kChunkUnit));
       }
     }
   }
@@ -256,11 +344,9 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p, v
   }
 }
 
-__device__ __forceinline__ float row_max(const Row& R) {
-  float mx = -INFINITY;
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) mx = fmaxf(mx, R.pmax[c]);
-  return mx;
+__device__ __forceinline__ float row_max(const Row& R, int chunks) {
+  const int lane = threadIdx.x & 63;
+  return wave_max(lane < chunks ? R.pmax[lane] : -INFINITY);
 }
 
 // The bins that hold the cuts: tokens of bins < lo are kept, those of k_bin and of p_lo .. p_hi are
@@ -269,37 +355,40 @@ struct CutBins {
   int lo, p_lo, p_hi, k_bin;
 };
 
-__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p, void* ws) {
+__global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams p, void* ws) {
   __shared__ u64 red[kWaves];
+  __shared__ double redd[kWaves];
   __shared__ u64 part_c[4][kBins];
   __shared__ double part_m[4][kBins];
+  __shared__ double powers[64];
   __shared__ CutBins s_cut;
-  __shared__ int s_cnt[kRound * kWaves];
+  __shared__ int s_cnt[kWaves];
   const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Row& R = row_state(ws, row, p.vocab);
   const float* L = p.logits + (size_t)row * p.vocab;
-  const int cl = chunk_len(p.vocab), beg = min(p.vocab, c * cl), end = min(p.vocab, beg + cl);
+  const int cl = chunk_len(p.vocab, p.chunks), beg = min(p.vocab, c * cl), end = min(p.vocab, beg + cl);
   const Setting s = setting(p, row);
-  float v[kRound];
-  if (beg < end) load_round(L, beg + tid, end, v);
-  const float mx = row_max(R);
+  if (tid < 64) powers[tid] = kPowers.v[tid];
+  const float mx = row_max(R, p.chunks);
   if (!(mx > -INFINITY)) return;  // nothing to choose from
   const Binner bin(mx, s.inv_t);
+  const Weigher weight(powers, mx, s.inv_t);
+  __syncthreads();
+  const bool cuts = s.top_k || s.p;
   CutBins cut{kBins, -1, -2, -1};
-  if (s.top_k || s.p) {
+  if (cuts) {
     // the row's histogram: thread (bin, quarter of the chunks), then the quarters in order
     const int b = tid & (kBins - 1), q = tid / kBins;
     u64 count = 0;
     double mass = 0.0;
-#pragma unroll
-    for (int j = 0; j < kChunks / 4; ++j) {
-      const int ch = q * (kChunks / 4) + j;
+    for (int j = 0; j < p.chunks / 4; ++j) {
+      const int ch = q * (p.chunks / 4) + j;
       const float cm = R.pmax[ch];
       const int from = b - bin(cm);  // (bin(-inf) = kBins: none)
       if (from < 0) continue;
       if (s.top_k) count += R.count[ch][from];
-      if (s.p) mass += (double)R.mass[ch][from] * weight(cm, mx, s.inv_t);
+      if (s.p) mass += (double)R.mass[ch][from] * weight(cm);
     }
     part_c[q][b] = count;
     part_m[q][b] = mass;
@@ -311,21 +400,10 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p,
       for (int j = 0; j < 4; ++j) {
         const int b4 = 4 * lane + j;
         nsum += n[j] = (part_c[0][b4] + part_c[1][b4]) + (part_c[2][b4] + part_c[3][b4]);
-        msum += m[j] = ((part_m[0][b4] + part_m[1][b4]) + (part_m[2][b4] + part_m[3][b4])) * (1.0 / kBinUnit);
+        msum += m[j] = ((part_m[0][b4] + part_m[1][b4]) + (part_m[2][b4] + part_m[3][b4])) * (1.0 / kChunkUnit);
       }
       const u64 ninc = wave_scan_inc(nsum);
       const double minc = wave_scan_inc(msum);
-      // first bin whose cumulative value reaches the target (kBins: none), and what lies above it
-      const auto first_bin = [&](auto inc, auto own, const auto (&h)[4], auto target, auto* above) {
-        const u64 hit = __ballot(inc >= target);
-        const int at = hit ? __ffsll((long long)hit) - 1 : 63;
-        auto a = inc - own;
-        int j = 0;
-        while (j < 3 && a + h[j] < target) a += h[j++];
-        const int bin4 = hit ? 4 * lane + j : kBins;
-        *above = lane_value(a, at);
-        return lane_value(bin4, at);
-      };
       u64 k_above = 0;
       double mass_k = lane_value(minc, 63), mass_k_incl = mass_k, mass_p = 0.0, none;
       if (s.top_k) {
@@ -358,8 +436,6 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p,
       if (lane == 0) {
         s_cut = cut;
         if (c == 0) {
-          R.cut_bins[0] = cut.lo, R.cut_bins[1] = cut.p_lo;
-          R.cut_bins[2] = cut.p_hi, R.cut_bins[3] = cut.k_bin;
           R.k_above = k_above;
           R.mass_k = mass_k;
           R.mass_p = mass_p;
@@ -368,46 +444,67 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p,
     }
     __syncthreads();
     cut = s_cut;
-  } else if (c == 0 && tid == 0) {
-    R.cut_bins[0] = cut.lo, R.cut_bins[1] = cut.p_lo;
-    R.cut_bins[2] = cut.p_hi, R.cut_bins[3] = cut.k_bin;
   }
-  Listed* list = row_list(R, c, p.vocab);
-  u64 low = 0;
+  if (c == 0 && tid == 0) R.p_lo = cut.p_lo, R.p_hi = cut.p_hi, R.k_bin = cut.k_bin;
+  // The chunk's certain mass: from the histogram (or the total) where there is one and no min-p, else
+  // token by token
+  const bool summed = !s.m && (s.p || !cuts);
+  double low = 0.0;
+  if (summed) {
+    const float cm = R.pmax[c];
+    const double scale = cm > -INFINITY ? weight(cm) * (1.0 / kChunkUnit) : 0.0;
+    if (scale > 0.0) {
+      if (!cuts) {
+        low = (double)R.total[c] * scale;
+      } else {
+        const int from = tid - bin(cm);
+        if (tid < cut.lo && from >= 0) low = (double)R.mass[c][from] * scale;  // (lo <= kBins)
+        low = block_sum(low, redd);
+      }
+    } else if (cuts) {
+      block_sum(low, redd);
+    }
+    if (!cuts) {
+      if (tid == 0) R.kept[c] = low, R.n_listed[c] = 0;
+      return;
+    }
+  }
+  Listed* list = row_list(R, c, cl);
+  const int sum_bins = summed ? 0 : s.m ? min(cut.lo, s.m_bins) : cut.lo;  // bins summed token by token
+  u64 sum = 0;
   int listed = 0;
   // (beg and end are the workgroup's: every thread runs every round and its barriers)
   for (int i = beg; i < end; i += kRound * kThreads) {
-    if (i > beg) load_round(L, i + tid, end, v);
+    float v[kRound];
+    load_round(L, i, end, v);
     unsigned int hits = 0;
+    int before = 0, place[kRound];
 #pragma unroll
     for (int u = 0; u < kRound; ++u) {
       const int b = bin(v[u]);
-      if (b < cut.lo && b < kBins) {
-        const double w = weight(v[u], mx, s.inv_t);
-        if (!s.m || w >= (double)s.min_p) low += fixed(w);
-      } else if (b < kBins && (b == cut.k_bin || (b >= cut.p_lo && b <= cut.p_hi))) {
-        hits |= 1u << u;
+      if (b < sum_bins && b < kBins) {
+        const double w = weight(v[u]);
+        if (!s.m || w >= (double)s.min_p) sum += in_units(w, kChunkUnit);
       }
-      const u64 vote = __ballot(hits >> u & 1);
-      if (lane == 0) s_cnt[u * kWaves + wave] = __popcll(vote);
+      const bool hit = b >= cut.lo && b < kBins && (b == cut.k_bin || (b >= cut.p_lo && b <= cut.p_hi));
+      const u64 vote = __ballot(hit);
+      place[u] = before + __popcll(vote & ((1ull << lane) - 1));
+      before += __popcll(vote);
+      hits |= (unsigned int)hit << u;
     }
+    if (!cuts) continue;
+    // places in id order: wave after wave
+    if (lane == 0) s_cnt[wave] = before;
     __syncthreads();
-    // places in id order: the slabs of kThreads ids one after the other, wave by wave
-    static_assert(kRound * kWaves == 128, "two counts a lane");
-    const int a = s_cnt[2 * lane], b2 = s_cnt[2 * lane + 1];
-    const int inc = wave_scan_inc(a + b2);
+    const int own = s_cnt[lane & (kWaves - 1)], upto = row_scan_inc(own);
+    const int at = listed + lane_value(upto - own, wave);
+    listed += lane_value(upto, kWaves - 1);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kRound; ++u) {
-      const int slot = u * kWaves + wave;
-      const int upto = lane_value(inc, slot >> 1) - lane_value(slot & 1 ? b2 : a + b2, slot >> 1);
-      const u64 vote = __ballot(hits >> u & 1);
-      if (hits >> u & 1)
-        list[listed + upto + __popcll(vote & ((1ull << lane) - 1))] = Listed{v[u], i + tid + u * kThreads};
-    }
-    listed += lane_value(inc, 63);
+    for (int u = 0; u < kRound; ++u)
+      if (hits >> u & 1) list[at + place[u]] = Listed{v[u], round_id(i, u)};
   }
-  low = block_sum(low, red);
+  if (!summed) low = (double)block_sum(sum, red) * (1.0 / kChunkUnit);
   if (tid == 0) {
     R.kept[c] = low;
     R.n_listed[c] = listed;
@@ -438,7 +535,8 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   __shared__ u64 hist[kDigits];
   __shared__ Listed held[kInLds];
   __shared__ u64 red[kWaves];
-  __shared__ u64 kept_of[kChunks];
+  __shared__ u64 listed_of[kChunks];
+  __shared__ double powers[64];
   __shared__ int offset[kChunks + 1];
   __shared__ uint32_t s_min, s_max;
   __shared__ int s_digit, s_id;
@@ -447,20 +545,23 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   Row& R = row_state(ws, row, p.vocab);
   const float* L = p.logits + (size_t)row * p.vocab;
   const Setting s = setting(p, row);
-  const float mx = row_max(R);
+  const float mx = row_max(R, p.chunks);
   if (!(mx > -INFINITY)) {
     if (tid == 0) p.out[row] = -1;
     return;
   }
   const Binner bin(mx, s.inv_t);
-  const int p_lo = R.cut_bins[1], p_hi = R.cut_bins[2], k_bin = R.cut_bins[3];
+  const Weigher weight(powers, mx, s.inv_t);
+  const int cl = chunk_len(p.vocab, p.chunks);
+  const int p_lo = R.p_lo, p_hi = R.p_hi, k_bin = R.k_bin;
   if (tid < 64) {
-    const int n = tid < kChunks ? R.n_listed[tid] : 0;
+    const int n = tid < p.chunks ? R.n_listed[tid] : 0;
     const int inc = wave_scan_inc(n);
     if (tid < kChunks) {
       offset[tid + 1] = inc;
-      kept_of[tid] = R.kept[tid];
+      listed_of[tid] = 0;
     }
+    powers[tid] = kPowers.v[tid];
     if (tid == 0) offset[0] = 0;
   }
   __syncthreads();
@@ -471,7 +572,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     int c = 0;
 #pragma unroll
     for (int k = 1; k < kChunks; ++k) c += j >= offset[k];
-    return row_list(R, c, p.vocab)[j - offset[c]];
+    return row_list(R, c, cl)[j - offset[c]];
   };
   if (in_lds)
     for (int j = tid; j < n; j += kThreads) held[j] = fetch(j);
@@ -543,7 +644,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     __syncthreads();
     return c;
   };
-  const auto mass = [&](float l) { return fixed(weight(l, mx, s.inv_t)); };
+  const auto mass = [&](float l) { return in_units(weight(l), kUnit); };
 
   Cut k_cut{-INFINITY, 0x7FFFFFFF}, cut = k_cut;
   if (k_bin >= 0) {
@@ -570,36 +671,39 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   }
   // (what is kept lies at or above the cut, the bins above it with it; a cut keeps all that weighs
   // something where there is none)
-  const auto kept_mass = [&](float l, int id) -> u64 {
+  const auto kept_mass = [&](float l, int id, double unit) -> u64 {
     if (!cut.keeps(l, id)) return 0;
-    const double w = weight(l, mx, s.inv_t);
-    return !s.m || w >= (double)s.min_p ? fixed(w) : 0;
+    const double w = weight(l);
+    return !s.m || w >= (double)s.min_p ? in_units(w, unit) : 0;
   };
   // the chunks' kept masses
   for (int j = tid; j < n; j += kThreads) {
     const Listed t = token(j);
-    const u64 q = kept_mass(t.l, t.id);
+    const u64 q = kept_mass(t.l, t.id, kUnit);
     if (!q) continue;
     int c = 0;
 #pragma unroll
     for (int k = 1; k < kChunks; ++k) c += j >= offset[k];
-    atomicAdd(&kept_of[c], q);
+    atomicAdd(&listed_of[c], q);
   }
   __syncthreads();
   if (tid < 64) {
-    const u64 own = tid < kChunks ? kept_of[tid] : 0, inc = wave_scan_inc(own);
-    const u64 z = lane_value(inc, 63);
-    const float u = p.uniform[row];
-    const double x = (double)z * (u > 0.f ? (double)u : 0.0);
-    const u64 at = x < (double)z ? min((u64)x, z - 1) : z - 1;
-    const int c = __ffsll((long long)__ballot(inc > at)) - 1;
-    if (lane == c) s_digit = c, s_at = at - (inc - own);
+    const double own =
+        tid < p.chunks ? R.kept[tid] + (double)listed_of[tid] * (1.0 / kUnit) : 0.0;
+    const double inc = wave_scan_inc(own), z = lane_value(inc, 63), u = p.uniform[row];
+    const double x = z * fmax(u, 0.0);  // (a NaN too: 0)
+    // (u >= 1, or a product rounded up: the last chunk that keeps anything)
+    const u64 more = __ballot(inc > x), some = __ballot(own > 0.0);
+    const int c = more ? __ffsll((long long)more) - 1 : some ? 63 - __clzll((long long)some) : 0;
+    if (lane == c) s_digit = c, s_at = (u64)fmin(fmax(x - (inc - own), 0.0) * kChunkUnit, 9e18), s_id = -1;
   }
   __syncthreads();
-  // the chunk's first id whose kept cumulative mass exceeds the draw
+  // the chunk's first id whose kept cumulative mass exceeds the draw (its last kept id where the sums'
+  // roundings, or a uniform past 1, leave none)
   const u64 at = s_at;
-  const int cl = chunk_len(p.vocab), beg = s_digit * cl, end = min(p.vocab, beg + cl);
+  const int beg = s_digit * cl, end = min(p.vocab, beg + cl);
   u64 before = 0;
+  int last = -1;
   for (int i = beg; i < end && before <= at; i += kRound * kThreads) {
     // kRound ids in a row a thread: one scan a round
     float v[kRound];
@@ -609,16 +713,22 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
 #pragma unroll
     for (int u = 0; u < kRound; ++u) {
       const int id = i + tid * kRound + u;
-      own += q[u] = id < end ? kept_mass(v[u], id) : 0;
+      own += q[u] = id < end ? kept_mass(v[u], id, kChunkUnit) : 0;
+      if (q[u]) last = id;
     }
     u64 all;
     u64 upto = before + block_scan(own, red, &all) - own;
 #pragma unroll
     for (int u = 0; u < kRound; ++u) {
-      if (upto <= at && at < upto + q[u]) p.out[row] = i + tid * kRound + u;  // exactly one token
+      if (upto <= at && at < upto + q[u]) p.out[row] = i + tid * kRound + u;  // at most one token
       upto += q[u];
     }
     before += all;
+  }
+  if (before <= at) {  // (uniform)
+    if (last >= 0) atomicMax(&s_id, last);
+    __syncthreads();
+    if (tid == 0) p.out[row] = s_id;
   }
 }
 
@@ -626,8 +736,9 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
 
 size_t sample_filtered_workspace_bytes(int rows, int vocab) { return rows * row_bytes(vocab); }
 
-int launch_sample_filtered(const SampleParams& p, void* ws, hipStream_t st) {
-  const dim3 chunks(kChunks, p.rows);
+int launch_sample_filtered(SampleParams p, void* ws, hipStream_t st) {
+  p.chunks = row_chunks(p.rows);
+  const dim3 chunks(p.chunks, p.rows);
   hipLaunchKernelGGL(sample_hist_kernel, chunks, dim3(kThreads), 0, st, p, ws);
   hipLaunchKernelGGL(sample_gather_kernel, chunks, dim3(kThreads), 0, st, p, ws);
   hipLaunchKernelGGL(sample_finish_kernel, dim3(p.rows), dim3(kThreads), 0, st, p, ws);

@@ -329,6 +329,7 @@ struct AttnWindowParams {
   const int* block_tables;
   int table_stride, n_pages, window, n_sinks;
   int group_shift;     // log2 of the q heads per kv head
+  bool nt;             // (set by the launcher) nontemporal loads of tiles that one workgroup reads
   // set by the launcher
   float* part;         // splits' partials [slots][heads][128], then (m, l)
   float* part_ml;
@@ -337,7 +338,6 @@ struct AttnWindowParams {
   int item_end[kMaxSeqs];                  // (row block, split) items up to and with the sequence's
   int splits[kMaxSeqs], part0[kMaxSeqs];   // key splits; first partial row
 };
-constexpr int kMaxSplits = 64;
 constexpr int kAttnWindowPartRows = 4096;
 size_t attn_window_workspace_bytes(int rows, int heads);
 int launch_attn_window(AttnWindowParams p, const SeqBatch& s, void* workspace, hipStream_t st);

@@ -5,10 +5,10 @@
 // keys j <= p with j > p - window or j < n_sinks whose page is there:
 //   o = sum_j softmax_j(q . k_j / sqrt(128)) v_j,  zeros where it sees none.
 //
-// A workgroup takes one kv head and a block of query columns, a column being a (row, q head of the
-// kv head's group): consecutive columns are the group's heads, then the next row, so that a single
-// token of a 4-head group fills 4 of a wave's 16 columns and a chunk fills all of them, whatever the
-// group.  It walks the 64-key tiles that the block's rows see (a tile is a page: the sink tiles, then the
+// A workgroup of 4 waves takes one kv head and a block of query columns, 16 or 32 a wave, a column
+// being a (row, q head of the kv head's group): consecutive columns are the group's heads, then the
+// next row, so that a single token of a 4-head group fills 4 of a wave's 16 columns and a chunk fills
+// all of them, whatever the group.  It walks the 64-key tiles that the block's rows see (a tile is a page: the sink tiles, then the
 // window's), each staged once in LDS for all its waves.  Per tile and wave, with
 // v_mfma_f32_16x16x32_bf16:
 //   S^T[key][col] = K . Q^T       (A = K rows from LDS, B = Q fragments in registers)
@@ -70,39 +70,147 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
   return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
 }
 
-// A wave's query columns (lane fr of each group of 16 holds column 16 qi + fr).
-template <int QI>
-struct Columns {
-  bf16x8_t q[QI][4];  // Q^T fragments
-  int pos[QI];        // the columns' positions
-  f32x4_t o[QI][8];   // unnormalised outputs
-  float m[QI];        // running max of the raw scores (the scale is applied inside the exponent)
-  f32x4_t l[QI];      // [0]: the running sum (the ones-MFMA's other rows are not rescaled)
+// A workgroup's work: the rows r0 .. r0 + nr - 1 (positions p0 ..) of sequence b's new rows, one kv
+// head, the tiles i0 .. i1 - 1 of the run that they see.
+struct Work {
+  int g, b, row0, n_new, nqb, splits, split, r0, nr, p0, nkeys, i0, i1;
+  TileRun run;
+  const int* table;
+  __device__ __forceinline__ int tile(int i) const { return i < run.sinks ? i : run.first + i - run.sinks; }
 };
 
-// The columns over one tile: kb8 the tile's stage, key0 its first key.  MASK applies the window,
-// the sinks and the diagonal.  A column may have seen no key so far: its max stays -inf and
-// its weights are 0 (the exponent's offset is then taken from a finite stand-in).
-template <bool MASK, int QI>
-__device__ __forceinline__ void attend_tile(Columns<QI>& c, const char* kb8, int key0, int G,
-                                            const uint32_t (&koffs)[4], const uint32_t (&voffs)[8],
-                                            int window, int n_sinks) {
-  const u32x4_t ones_w = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, ones_w);
-  f32x4_t s[QI][4];
+// Workgroup -> (sequence, split, row block, kv head): kv heads go round the XCDs, whose L2 then holds the
+// head's keys for the blocks that share them; a sequence's last blocks (the longest runs) come first.
+// (the sequences' arguments in one go, a lane each: one after the other they are a wait each)
+__device__ __forceinline__ Work work_of(const AttnWindowParams& p, int columns) {
+  const int lane = threadIdx.x & 63;
+  const int item_end = p.item_end[lane], row_end = p.row_end[lane], start = p.start[lane],
+            splits = p.splits[lane];
+  Work w;
+  w.g = blockIdx.x % kKVHeads;
+  const int item = blockIdx.x / kKVHeads;
+  w.b = __popcll(__ballot(lane < p.n_seqs && item_end <= item));
+  const int before = max(w.b - 1, 0);
+  w.row0 = w.b ? __builtin_amdgcn_readlane(row_end, before) : 0;
+  w.n_new = __builtin_amdgcn_readlane(row_end, w.b) - w.row0;
+  w.splits = __builtin_amdgcn_readlane(splits, w.b);
+  const int first = __builtin_amdgcn_readlane(start, w.b);
+  const int local = item - (w.b ? __builtin_amdgcn_readlane(item_end, before) : 0);
+  const int rb = columns >> p.group_shift;
+  w.nqb = (w.n_new + rb - 1) / rb;
+  w.r0 = (w.nqb - 1 - local % w.nqb) * rb;
+  w.split = local / w.nqb;
+  w.nr = min(rb, w.n_new - w.r0);
+  w.p0 = first + w.r0;
+  w.nkeys = first + w.n_new;
+  w.run = tile_run(w.p0, w.p0 + w.nr - 1, p.window, p.n_sinks);
+  const int tps = (w.run.count + w.splits - 1) / w.splits;
+  w.i0 = min(w.run.count, w.split * tps);
+  w.i1 = min(w.run.count, w.i0 + tps);
+  w.table = p.block_tables + (size_t)w.b * p.table_stride;
+  return w;
+}
+
+// A wave's query columns: lane fr of each group of 16 holds column col0 + 16 qi + fr.
+template <int QI>
+struct Columns {
+  bf16x8_t q[QI][4];  // Q^T fragments: Q[column][32 ks + 8 G .. +8]
+  int pos[QI];        // the columns' positions
+  f32x4_t o[QI][8];   // unnormalised: [db][r] = O[column][16 db + 4 G + r]
+  float m[QI];        // running max of the raw scores (the scale is applied inside the exponent)
+  f32x4_t l[QI];      // [0]: the running sum (the ones-MFMA's other rows are not rescaled)
+
+  // columns past the rows repeat the last row
+  __device__ __forceinline__ void load(const AttnWindowParams& p, const Work& w, int col0) {
+    const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3, gs = p.group_shift;
+#pragma unroll
+    for (int qi = 0; qi < QI; ++qi) {
+      const int col = col0 + 16 * qi + fr, r = min(col >> gs, w.nr - 1);
+      pos[qi] = w.p0 + r;
+      const size_t at = ((size_t)(w.row0 + w.r0 + r) << gs << 3) + ((size_t)w.g << gs) + (col & ((1 << gs) - 1));
+      const u32x4_t* row = reinterpret_cast<const u32x4_t*>(p.q + at * kHeadDim);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) q[qi][ks] = __builtin_bit_cast(bf16x8_t, row[4 * ks + G]);
+      m[qi] = -INFINITY, l[qi] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int db = 0; db < 8; ++db) o[qi][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    // The compiler does not see what the kernels' own waits cover: without one here it would guard the
+    // fragments inside their loops, where that is a wait for the tile in flight.
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  }
+
+  __device__ __forceinline__ void store(const AttnWindowParams& p, const Work& w, int col0) const {
+    const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3, gs = p.group_shift;
+    const int heads = kKVHeads << gs;
+#pragma unroll
+    for (int qi = 0; qi < QI; ++qi) {
+      const int col = col0 + 16 * qi + fr, r = col >> gs;
+      if (r >= w.nr) continue;
+      const int h = (w.g << gs) + (col & ((1 << gs) - 1));
+      if (w.splits > 1) {
+        // this split's partial, [slot][head][128] and [slot][head](m, l), slots split by split of the
+        // sequence's rows
+        const size_t slot = ((size_t)p.part0[w.b] + (size_t)w.split * w.n_new + w.r0 + r) * heads + h;
+        float* dst = p.part + slot * kHeadDim + 4 * G;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4_t*>(dst + 16 * db) = o[qi][db];
+        if (G == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(m[qi], l[qi][0]);
+      } else {
+        const float inv = l[qi][0] == 0.f ? 0.f : 1.0f / l[qi][0];
+        uint16_t* dst = p.out + ((size_t)(w.row0 + w.r0 + r) * heads + h) * kHeadDim;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+          const u32x2_t v = {pack_bf2(o[qi][db][0] * inv, o[qi][db][1] * inv),
+                             pack_bf2(o[qi][db][2] * inv, o[qi][db][3] * inv)};
+          *reinterpret_cast<u32x2_t*>(dst + db * 16 + 4 * G) = v;
+        }
+      }
+    }
+  }
+};
+
+// Byte offsets of a lane's fragment reads in a tile of 64 rows: K fragment ks of key row fr (+ 4096 per
+// 16 keys); the transposed V read of dims 16 db + 4 (fr % 4) .. of keys 4 G + fr / 4 (+ 8192 per 32
+// keys, + 4096 for keys + 16).  ks and db are XORs of the swizzled chunk.
+struct Frags {
+  uint32_t k0, v0;
+  __device__ __forceinline__ Frags() {
+    const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3;
+    k0 = (uint32_t)kv_slot(fr, G) * 16;
+    v0 = (uint32_t)kv_slot(4 * G + (fr >> 2), (fr & 3) >> 1) * 16 + (fr & 1) * 8;
+  }
+  __device__ __forceinline__ uint32_t k(int ks) const { return k0 ^ (uint32_t)(ks * 64); }
+  __device__ __forceinline__ uint32_t v(int db) const { return v0 ^ (uint32_t)(db * 32); }
+};
+
+// s[qi][kb][r] = raw score of the column and key 16 kb + 4 G + r of the tile.
+template <int QI>
+__device__ __forceinline__ void scores(f32x4_t (&s)[QI][4], const Columns<QI>& c, const Frags& f,
+                                       const u32x4_t* ktile) {
+  const char* kb8 = reinterpret_cast<const char*>(ktile);
 #pragma unroll
   for (int kb = 0; kb < 4; ++kb) {
 #pragma unroll
     for (int qi = 0; qi < QI; ++qi) s[qi][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(kb8 + koffs[ks] + kb * 4096);
+      const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(kb8 + f.k(ks) + kb * 4096);
 #pragma unroll
       for (int qi = 0; qi < QI; ++qi)
         s[qi][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, c.q[qi][ks], s[qi][kb], 0, 0, 0);
     }
   }
-  bf16x8_t pb[QI][2];
+}
+
+// The scores to weights (bf16, as P^T operands), the outputs and sums so far rescaled.  MASK applies the
+// window, the sinks and the diagonal.  A column may have seen no key so far: its max stays -inf and its
+// weights are 0 (the exponent's offset is then taken from a finite stand-in).
+template <bool MASK, int QI>
+__device__ __forceinline__ void weights(bf16x8_t (&pb)[QI][2], Columns<QI>& c, f32x4_t (&s)[QI][4],
+                                        int key0, int window, int n_sinks) {
+  int first = 4 * (threadIdx.x >> 4 & 3);  // the lane's first key in each 16
+  if constexpr (MASK) asm volatile("" : "+v"(first));  // (opaque: nothing made of it is kept over the tiles)
 #pragma unroll
   for (int qi = 0; qi < QI; ++qi) {
     float mt = -INFINITY;
@@ -111,9 +219,9 @@ __device__ __forceinline__ void attend_tile(Columns<QI>& c, const char* kb8, int
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if constexpr (MASK) {
-          const int key = key0 + 16 * kb + 4 * G + r;
-          const bool seen = key <= c.pos[qi] && (key > c.pos[qi] - window || key < n_sinks);
-          if (!seen) s[qi][kb][r] = -INFINITY;
+          const int key = key0 + first + 16 * kb + r;
+          const bool seen = (key <= c.pos[qi]) & ((key > c.pos[qi] - window) | (key < n_sinks));
+          s[qi][kb][r] = seen ? s[qi][kb][r] : -INFINITY;
         }
         mt = fmaxf(mt, s[qi][kb][r]);
       }
@@ -137,25 +245,35 @@ __device__ __forceinline__ void attend_tile(Columns<QI>& c, const char* kb8, int
                          pack_bf2(s[qi][2 * ks2 + 1][0], s[qi][2 * ks2 + 1][1]),
                          pack_bf2(s[qi][2 * ks2 + 1][2], s[qi][2 * ks2 + 1][3])};
       pb[qi][ks2] = __builtin_bit_cast(bf16x8_t, w);
-      c.l[qi] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[qi][ks2], c.l[qi], 0, 0, 0);
     }
   }
-  auto v_frag = [&](int db, int ks2) {
-    const char* va = kb8 + voffs[db] + ks2 * 8192;
-    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)va);
-    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(va + 4096));
-    const short4_t both[2] = {lo, hi};
-    return __builtin_bit_cast(u32x4_t, both);
-  };
+}
+
+// o += V^T . P^T and the sums.  MASK: 0 x (an infinity or NaN) of a key that a column does not see must
+// stay 0: such values are kept out of the product and added to the columns that see them.
+template <bool MASK, int QI>
+__device__ __forceinline__ void values(Columns<QI>& c, const bf16x8_t (&pb)[QI][2], const Frags& f,
+                                       const u32x4_t* vtile, int key0, int window, int n_sinks) {
+  const u32x4_t ones_w = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, ones_w);
+  const char* vb8 = reinterpret_cast<const char*>(vtile);
+#pragma unroll
+  for (int qi = 0; qi < QI; ++qi)
+#pragma unroll
+    for (int ks2 = 0; ks2 < 2; ++ks2)
+      c.l[qi] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[qi][ks2], c.l[qi], 0, 0, 0);
   uint32_t bad = 0;
 #pragma unroll
-  for (int db = 0; db < 8; ++db)
+  for (int db = 0; db < 8; ++db) {
+    if constexpr (MASK) __builtin_amdgcn_sched_barrier(0);  // (fewer fragments at once: registers)
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
-      u32x4_t w = v_frag(db, ks2);
+      const char* va = vb8 + f.v(db) + ks2 * 8192;
+      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)va);
+      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(va + 4096));
+      const short4_t both[2] = {lo, hi};
+      u32x4_t w = __builtin_bit_cast(u32x4_t, both);
       if constexpr (MASK) {
-        // 0 x (infinity or NaN) of a key that the column does not see must stay 0: such values are
-        // kept out of the product here and added below to the columns that see them
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t n = nonfinite2(w[e]);
@@ -168,221 +286,156 @@ __device__ __forceinline__ void attend_tile(Columns<QI>& c, const char* kb8, int
       for (int qi = 0; qi < QI; ++qi)
         c.o[qi][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[qi][ks2], c.o[qi][db], 0, 0, 0);
     }
+  }
   if constexpr (MASK) {
     if (__builtin_expect(__ballot(bad != 0) != 0, 0)) {
-      // 1 where the column's weight is positive x (1 where V is +inf, -inf, NaN), by MFMA
-      bf16x8_t seen[QI][2];
+      int G = threadIdx.x >> 4 & 3;
+      asm volatile("" : "+v"(G));
 #pragma unroll
-      for (int qi = 0; qi < QI; ++qi)
+      for (int qi = 0; qi < QI; ++qi) {
+#pragma unroll 1
+        for (int key = 0; key < BKEY; ++key) {
+          const int k = key0 + key;
+          const bool seen = k <= c.pos[qi] && (k > c.pos[qi] - window || k < n_sinks);
 #pragma unroll
-        for (int ks2 = 0; ks2 < 2; ++ks2) {
-          u32x4_t w = __builtin_bit_cast(u32x4_t, pb[qi][ks2]);
+          for (int db = 0; db < 8; ++db) {
+            // V[key][16 db + 4 G ..+3]
+            const u32x2_t v = *reinterpret_cast<const u32x2_t*>(
+                vb8 + kv_slot(key, 2 * db + (G >> 1)) * 16 + (G & 1) * 8);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = (w[e] & 0xFFFFu ? 0x3F80u : 0u) | (w[e] >> 16 ? 0x3F800000u : 0u);
-          seen[qi][ks2] = __builtin_bit_cast(bf16x8_t, w);
-        }
-#pragma unroll
-      for (int db = 0; db < 8; ++db)
-#pragma unroll
-        for (int kind = 0; kind < 3; ++kind) {
-          u32x4_t hit[2];
-#pragma unroll
-          for (int ks2 = 0; ks2 < 2; ++ks2) {
-            const u32x4_t w = v_frag(db, ks2);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const auto is = [&](uint32_t h) {
-                return kind == 0   ? h == 0x7F80u
-                       : kind == 1 ? h == 0xFF80u
-                                   : (h & 0x7FFFu) > 0x7F80u;
-              };
-              hit[ks2][e] = (is(w[e] & 0xFFFFu) ? 0x3F80u : 0u) | (is(w[e] >> 16) ? 0x3F800000u : 0u);
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t n = seen ? nonfinite2(v[e]) : 0;
+              if (n & 0x8000u) c.o[qi][db][2 * e] += bf_lo(v[e]);
+              if (n >> 16) c.o[qi][db][2 * e + 1] += bf_hi(v[e]);
             }
           }
-          const float value = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
-#pragma unroll
-          for (int qi = 0; qi < QI; ++qi) {
-            f32x4_t n = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks2 = 0; ks2 < 2; ++ks2)
-              n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, hit[ks2]),
-                                                          seen[qi][ks2], n, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (n[r] > 0.f) c.o[qi][db][r] += value;
-          }
         }
-    }
-  }
-}
-
-// One tile's loads into a stage (K at stage[0..TC), V at stage[TC..2TC)) by NW waves: this wave's
-// groups of 4 rows.
-template <int NW>
-__device__ __forceinline__ void issue_tile(u32x4_t* stage, __amdgpu_buffer_rsrc_t krs,
-                                           __amdgpu_buffer_rsrc_t vrs,
-                                           const uint32_t (&voff)[16 / NW], int wave) {
-#pragma unroll
-  for (int j = 0; j < 16 / NW; ++j) {
-    u32x4_t* kd = stage + (wave + NW * j) * 64;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_void*)kd, 16, voff[j], 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void*)(kd + TC), 16, voff[j], 0, 0, 0);
-  }
-}
-
-template <int QI, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_window_kernel(AttnWindowParams p) {
-  __shared__ u32x4_t lds0[2 * TC];  // ring stage 0: [K | V][key][16 chunks], 32 KiB
-  __shared__ u32x4_t lds1[2 * TC];  // ring stage 1
-  constexpr int CW = 16 * QI;       // columns per wave
-  constexpr int CB = CW * NW;       // columns per workgroup
-  constexpr int NL = 16 / NW;       // 1 KiB loads of K (and V) a wave and tile
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int fr = lane & 15, G = lane >> 4;
-  const int gs = p.group_shift;
-  // workgroup -> (sequence, split, row block, kv head): kv heads go round the XCDs, whose L2 then holds
-  // the head's keys for the blocks that share them
-  const int g = blockIdx.x % kKVHeads, item = blockIdx.x / kKVHeads;
-  const int b = __popcll(__ballot(lane < p.n_seqs && p.item_end[lane] <= item));
-  const int start = p.start[b], row0 = b ? p.row_end[b - 1] : 0, n_new = p.row_end[b] - row0;
-  const int splits = p.splits[b];
-  const int local = item - (b ? p.item_end[b - 1] : 0);
-  const int rb = CB >> gs;  // rows per workgroup
-  const int nqb = (n_new + rb - 1) / rb;
-  const int qb = nqb - 1 - local % nqb, split = local / nqb;
-  const int r0 = qb * rb, nr = min(rb, n_new - r0);
-  const int p0 = start + r0, nkeys = start + n_new;
-  const TileRun run = tile_run(p0, p0 + nr - 1, p.window, p.n_sinks);
-  const int tps = (run.count + splits - 1) / splits;
-  const int i0 = min(run.count, split * tps), i1 = min(run.count, i0 + tps);
-  // this wave's rows (positions wp0 .. wp1; none: wp1 < wp0)
-  const int wr0 = (wave * CW) >> gs;
-  const int wp0 = p0 + wr0, wp1 = p0 + min(nr, wr0 + (CW >> gs)) - 1;
-
-  const int* table = p.block_tables + (size_t)b * p.table_stride;
-  // load j of this wave: tile rows 4 (wave + NW j) + lane/16; a lane fills slot lane%16 of its row
-  // from chunk (lane%16) ^ swz(row)
-  uint32_t voff[NL];
-#pragma unroll
-  for (int j = 0; j < NL; ++j) {
-    const int r = 4 * (wave + NW * j) + G;
-    voff[j] = (uint32_t)(r * kRowBytes + ((fr ^ kv_swz(r)) * 16));
-  }
-  auto tile_of = [&](int i) { return i < run.sinks ? i : run.first + i - run.sinks; };
-
-  // Q^T fragments: c.q[qi][ks] = Q[column][32 ks + 8 G .. +8]; columns past the rows repeat the last row
-  Columns<QI> c;
-#pragma unroll
-  for (int qi = 0; qi < QI; ++qi) {
-    const int col = wave * CW + 16 * qi + fr;
-    const int r = min(col >> gs, nr - 1);
-    c.pos[qi] = p0 + r;
-    const size_t at = ((size_t)(row0 + r0 + r) << gs << 3) + ((size_t)g << gs) + (col & ((1 << gs) - 1));
-    const u32x4_t* qrow = reinterpret_cast<const u32x4_t*>(p.q + at * kHeadDim);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) c.q[qi][ks] = __builtin_bit_cast(bf16x8_t, qrow[4 * ks + G]);
-  }
-
-#pragma unroll
-  for (int qi = 0; qi < QI; ++qi) {
-    c.m[qi] = -INFINITY, c.l[qi] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int db = 0; db < 8; ++db) c.o[qi][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-
-  const int kr = fr >> 2, dq = fr & 3;
-  uint32_t koffs[4], voffs[8];
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) koffs[ks] = (uint32_t)kv_slot(fr, 4 * ks + G) * 16;
-#pragma unroll
-  for (int db = 0; db < 8; ++db)
-    voffs[db] = (uint32_t)(TC + kv_slot(4 * G + kr, 2 * db + (dq >> 1))) * 16 + (dq & 1) * 8;
-
-  // Loads of tile i (page `page`) into a stage; a page outside the pool has no bytes (zeros).
-  auto issue = [&](u32x4_t* stage, int i, int page) {
-    const bool ok = page >= 0 && page < p.n_pages;
-    const size_t base = (size_t)(ok ? page : 0) * kPageElems + (size_t)g * kPageHead;
-    const int bytes = __builtin_amdgcn_readfirstlane(
-        ok ? min(BKEY, nkeys - tile_of(i) * BKEY) * kRowBytes : 0);
-    const __amdgpu_buffer_rsrc_t krs =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(p.k + base), 0, bytes, kBufferFlags);
-    const __amdgpu_buffer_rsrc_t vrs =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(p.v + base), 0, bytes, kBufferFlags);
-    issue_tile<NW>(stage, krs, vrs, voff, wave);
-  };
-  // page of the tile in flight, and of the one after it (loaded a step ahead)
-  int page = -1, next = -1;
-  if (i0 < i1) {
-    page = __builtin_amdgcn_readfirstlane(table[tile_of(i0)]);
-    issue(lds0, i0, page);
-    next = table[tile_of(min(i0 + 1, i1 - 1))];
-  }
-
-  auto step = [&](int i, const u32x4_t* cur, u32x4_t* nxt) {
-    // tile i has landed (the only loads in flight) and every wave is done with tile i - 1
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const bool there = page >= 0 && page < p.n_pages;
-    // tile i + 1 is issued unconditionally: past the last tile it has no bytes
-    page = i + 1 < i1 ? __builtin_amdgcn_readfirstlane(next) : -1;
-    issue(nxt, i + 1, page);
-    next = table[tile_of(min(i + 2, i1 - 1))];
-    const int key0 = tile_of(i) * BKEY, last = key0 + BKEY - 1;
-    // (wave-uniform) no row of the wave sees the tile / every row sees all of it
-    if (!there || wp1 < wp0 || key0 > wp1 || (last <= wp0 - p.window && key0 >= p.n_sinks)) return;
-    const char* kb8 = reinterpret_cast<const char*>(cur);
-    if (last <= wp0 && (key0 > wp1 - p.window || last < p.n_sinks))
-      attend_tile<false, QI>(c, kb8, key0, G, koffs, voffs, p.window, p.n_sinks);
-    else
-      attend_tile<true, QI>(c, kb8, key0, G, koffs, voffs, p.window, p.n_sinks);
-  };
-  for (int i = i0; i < i1; i += 2) {
-    step(i, lds0, lds1);
-    if (i + 1 < i1) step(i + 1, lds1, lds0);
-  }
-
-  // ---- c.o[qi][db][r] = O[column 16 qi + fr][d = 16 db + 4 G + r] (unnormalised)
-  const int heads = kKVHeads << gs;
-#pragma unroll
-  for (int qi = 0; qi < QI; ++qi) {
-    const int col = wave * CW + 16 * qi + fr, r = col >> gs;
-    if (r >= nr) continue;
-    const int h = (g << gs) + (col & ((1 << gs) - 1));
-    if (splits > 1) {
-      // this split's partial, [slot][head][128] and [slot][head](m, l), slots split by split of the
-      // sequence's rows
-      const size_t slot = ((size_t)p.part0[b] + (size_t)split * n_new + r0 + r) * heads + h;
-      float* dst = p.part + slot * kHeadDim + 4 * G;
-#pragma unroll
-      for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4_t*>(dst + 16 * db) = c.o[qi][db];
-      if (G == 0)
-        *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(c.m[qi], c.l[qi][0]);
-    } else {
-      const float inv = c.l[qi][0] == 0.f ? 0.f : 1.0f / c.l[qi][0];
-      uint16_t* dst = p.out + ((size_t)(row0 + r0 + r) * heads + h) * kHeadDim;
-#pragma unroll
-      for (int db = 0; db < 8; ++db) {
-        const u32x2_t w = {pack_bf2(c.o[qi][db][0] * inv, c.o[qi][db][1] * inv),
-                           pack_bf2(c.o[qi][db][2] * inv, c.o[qi][db][3] * inv)};
-        *reinterpret_cast<u32x2_t*>(dst + db * 16 + 4 * G) = w;
       }
     }
   }
 }
 
+// The part of one tile (K or V) that a wave of NW loads: rows 4 (wave + NW j) + lane / 16, a lane filling slot
+// lane % 16 of its row from chunk (lane % 16) ^ swz(row).
+template <int NW>
+struct TileLoad {
+  uint32_t voff[16 / NW];
+  int wave;
+  __device__ __forceinline__ TileLoad(int w) : wave(w) {
+#pragma unroll
+    for (int j = 0; j < 16 / NW; ++j) {
+      const int r = 4 * (wave + NW * j) + ((int)threadIdx.x >> 4 & 3);
+      voff[j] = (uint32_t)(r * kRowBytes + (((threadIdx.x & 15) ^ kv_swz(r)) * 16));
+    }
+  }
+};
+template <int NW, int AUX>
+__device__ __forceinline__ void issue_tile(u32x4_t* stage, __amdgpu_buffer_rsrc_t rs, const TileLoad<NW>& ld) {
+#pragma unroll
+  for (int j = 0; j < 16 / NW; ++j)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(stage + (ld.wave + NW * j) * 64), 16, ld.voff[j], 0, 0, AUX);
+}
+// The 64 rows of the head's plane in a page (a tile's K or V), `rows` of them there; a page outside the
+// pool has none (zeros).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rows(const AttnWindowParams& p, const uint16_t* plane,
+                                                            int g, int page, int rows) {
+  const bool ok = page >= 0 && page < p.n_pages;
+  const size_t base = (size_t)(ok ? page : 0) * kPageElems + (size_t)g * kPageHead;
+  const int bytes = __builtin_amdgcn_readfirstlane(ok ? min(BKEY, rows) * kRowBytes : 0);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(plane + base), 0, bytes, kBufferFlags);
+}
+
+// How the rows at positions wp0 .. wp1 see the tile from key0 on.
+enum Sight { kNone, kSome, kAll };
+__device__ __forceinline__ Sight sight(int key0, int wp0, int wp1, int window, int n_sinks) {
+  const int last = key0 + BKEY - 1;
+  if (wp1 < wp0 || key0 > wp1 || (last <= wp0 - window && key0 >= n_sinks)) return kNone;
+  return last <= wp0 && (key0 > wp1 - window || last < n_sinks) ? kAll : kSome;
+}
+
+// 4 waves of 16 QI columns, the tiles double-buffered (64 KiB: two workgroups a CU).
+template <int QI>
+__device__ __forceinline__ void attend(const AttnWindowParams& p) {
+  constexpr int NW = 4, CW = 16 * QI;
+  __shared__ u32x4_t k0[TC], v0[TC], k1[TC], v1[TC];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Work w = work_of(p, CW * NW);
+  const int wr0 = (wave * CW) >> p.group_shift;
+  const int wp0 = w.p0 + wr0, wp1 = w.p0 + min(w.nr, wr0 + (CW >> p.group_shift)) - 1;
+  const bool nt = p.nt && w.nqb == 1;
+  const TileLoad<NW> ld(wave);
+  auto issue = [&](u32x4_t* ks, u32x4_t* vs, int i, int page) {
+    const int rows = w.nkeys - w.tile(i) * BKEY;
+    const auto krs = page_rows(p, p.k, w.g, page, rows), vrs = page_rows(p, p.v, w.g, page, rows);
+    if (nt) {
+      issue_tile<NW, 2>(ks, krs, ld);
+      issue_tile<NW, 2>(vs, vrs, ld);
+    } else {
+      issue_tile<NW, 0>(ks, krs, ld);
+      issue_tile<NW, 0>(vs, vrs, ld);
+    }
+  };
+  // page of the tile in flight, and of the one after it (loaded a step ahead)
+  int page = -1, next = -1;
+  if (w.i0 < w.i1) {
+    const int here = w.table[w.tile(w.i0)];
+    next = w.table[w.tile(min(w.i0 + 1, w.i1 - 1))];
+    page = __builtin_amdgcn_readfirstlane(here);
+    issue(k0, v0, w.i0, page);
+  }
+  Columns<QI> c;
+  c.load(p, w, wave * CW);
+  const Frags f;
+
+  auto step = [&](int i, const u32x4_t* kc, const u32x4_t* vc, u32x4_t* kn, u32x4_t* vn) {
+    // tile i has landed (the only loads in flight) and every wave is done with tile i - 1
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const bool there = page >= 0 && page < p.n_pages;
+    // tile i + 1 is issued unconditionally: past the last tile it has no bytes
+    page = i + 1 < w.i1 ? __builtin_amdgcn_readfirstlane(next) : -1;
+    issue(kn, vn, i + 1, page);
+    next = w.table[w.tile(min(i + 2, w.i1 - 1))];
+    const int key0 = w.tile(i) * BKEY;
+    const Sight see = there ? sight(key0, wp0, wp1, p.window, p.n_sinks) : kNone;
+    if (see == kNone) return;  // (wave-uniform)
+    f32x4_t s[QI][4];
+    bf16x8_t pb[QI][2];
+    scores(s, c, f, kc);
+    __builtin_amdgcn_sched_barrier(0);  // (8192 rows over 4096 keys: 611 us without, 598 with)
+    if (see == kAll) {
+      weights<false>(pb, c, s, key0, p.window, p.n_sinks);
+      values<false>(c, pb, f, vc, key0, p.window, p.n_sinks);
+    } else {
+      weights<true>(pb, c, s, key0, p.window, p.n_sinks);
+      __builtin_amdgcn_sched_barrier(0);  // (no fragments held over the softmax: registers)
+      values<true>(c, pb, f, vc, key0, p.window, p.n_sinks);
+    }
+  };
+  for (int i = w.i0; i < w.i1; i += 2) {
+    step(i, k0, v0, k1, v1);
+    if (i + 1 < w.i1) step(i + 1, k1, v1, k0, v0);
+  }
+  c.store(p, w, wave * CW);
+}
+
+__global__ __launch_bounds__(256, 2) void attn_window_16_kernel(AttnWindowParams p) { attend<1>(p); }
+__global__ __launch_bounds__(256, 2) void attn_window_32_kernel(AttnWindowParams p) { attend<2>(p); }
+
 // Combines the splits of each (row, q head) of the sequences that have them: 32 lanes each, 4
 // dims a lane, in split order.  A split without keys for the row (l = 0) is passed over.
 __global__ __launch_bounds__(256) void attn_window_merge_kernel(AttnWindowParams p) {
   const int lane = threadIdx.x & 63;
+  const int row_end = p.row_end[lane], lane_splits = p.splits[lane], part0 = p.part0[lane];
   const int heads = kKVHeads << p.group_shift;
   const int row = blockIdx.x * 8 / heads;  // (8 heads a workgroup: heads is a multiple of 8)
-  const int b = __popcll(__ballot(lane < p.n_seqs && p.row_end[lane] <= row));
-  const int splits = p.splits[b];
+  const int b = __popcll(__ballot(lane < p.n_seqs && row_end <= row));
+  const int splits = __builtin_amdgcn_readlane(lane_splits, b);
   if (splits < 2) return;
-  const int row0 = b ? p.row_end[b - 1] : 0, n_new = p.row_end[b] - row0;
+  const int row0 = b ? __builtin_amdgcn_readlane(row_end, max(b - 1, 0)) : 0;
+  const int n_new = __builtin_amdgcn_readlane(row_end, b) - row0;
   const int h = blockIdx.x * 8 % heads + (threadIdx.x >> 5), d = (threadIdx.x & 31) * 4;
-  const size_t slot0 = ((size_t)p.part0[b] + row - row0) * heads + h, step = (size_t)n_new * heads;
+  const size_t slot0 = ((size_t)__builtin_amdgcn_readlane(part0, b) + row - row0) * heads + h;
+  const size_t step = (size_t)n_new * heads;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   float M = -INFINITY, L = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -417,61 +470,112 @@ __global__ __launch_bounds__(256) void attn_window_merge_kernel(AttnWindowParams
   *reinterpret_cast<u32x2_t*>(p.out + ((size_t)row * heads + h) * kHeadDim + d) = w;
 }
 
-constexpr int kSlots = 512;  // workgroups that run at once (two a CU)
-
 }  // namespace
 
 // Partial rows (a row and split) that a workspace for `rows` rows holds.
-int attn_window_part_rows(int rows) { return rows >= kAttnWindowPartRows ? 0 : kAttnWindowPartRows; }
+static int attn_window_part_rows(int rows) { return rows >= kAttnWindowPartRows ? 0 : kAttnWindowPartRows; }
 
 size_t attn_window_workspace_bytes(int rows, int heads) {
   return (size_t)attn_window_part_rows(rows) * heads * (kHeadDim + 2) * sizeof(float);
 }
 
+namespace {
+
+// A form (columns a wave) and its tiles a split.
+struct Plan {
+  int qi, tps;
+  double cost;
+};
+
+// The form and split with the least modelled time, us: a workgroup's step over a tile takes c1 where it
+// has a CU for itself and c2 where two share one (measured at 64 rows over 65 tiles and at 8192 rows over 66:
+// 1.12 and 1.39 for 16 columns a wave, 1.63 and 2.24 for 32), and 512 run at once; a launch 3.5, the merge
+// 4 and its partials 1 / 150 a row and split (32 heads).  Within 6% of the best of 10 split counts and both
+// forms over 27 batches (1-4000 rows, 10-940 tiles): 1 token at 20000 381 us unsplit, 24 in 32
+// splits; 200 rows over 16384 keys 296 unsplit, 104 in 4 (16 columns), 89 in 8 (32); 16 tokens over 4096 keys
+// 98 and 48; 6 x 333 rows over 1500 keys 71 unsplit, 75 in 3; 2 x 1000 over 4096 keys 172 and 151 unsplit,
+// 130 in 3 (32 columns).
+Plan plan_of(const AttnWindowParams& p, const SeqBatch& s, int rows, int room) {
+  Plan best{1, 1, 1e30};
+  for (int qi = 1; qi <= 2; ++qi) {
+    const int rb = (64 * qi) >> p.group_shift;
+    int nqb[kMaxSeqs], longest = 1;
+    int first[kMaxSeqs], last[kMaxSeqs];  // tiles of a sequence's first and last row block
+    for (int b = 0; b < s.n; ++b) {
+      const int n = s.n_new[b];
+      nqb[b] = (n + rb - 1) / rb;
+      first[b] = last[b] = 0;
+      if (!n) continue;
+      const int at = s.start[b];
+      first[b] = tile_run(at, at + std::min(rb, n) - 1, p.window, p.n_sinks).count;
+      last[b] = tile_run(at + (nqb[b] - 1) * rb, at + n - 1, p.window, p.n_sinks).count;
+      longest = std::max({longest, first[b], last[b]});
+    }
+    const double c1 = qi == 1 ? 1.12 : 1.63, c2 = qi == 1 ? 1.39 : 2.24;
+    int tried = 0;
+    for (const int n : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64}) {
+      const int tps = (longest + n - 1) / n;
+      if (n > longest || tps == tried) continue;
+      tried = tps;
+      long long items = 0, part = 0;
+      double steps = 0;
+      for (int b = 0; b < s.n; ++b) {
+        const int k = std::max(1, (std::max(first[b], last[b]) + tps - 1) / tps);
+        items += (long long)nqb[b] * k * kKVHeads;
+        steps += 0.5 * (first[b] + last[b]) * nqb[b] * kKVHeads;
+        if (k > 1) part += (long long)s.n_new[b] * k;
+      }
+      if (part > room) break;
+      const double t = items ? steps / items : 0;  // a workgroup's tiles, on average
+      const long long rest = items % 512;
+      const double turns = (double)(items / 512) * t * c2 + (rest == 0 ? 0 : rest <= 256 ? t * c1 : t * c2);
+      const double cost = std::max(turns, tps * c1) + 3.5 +
+                          (part ? 4 + 0.04 * n + part * (kKVHeads << p.group_shift) / (32 * 150.0) : 0);
+      if (cost < best.cost) best = Plan{qi, tps, cost};
+      else if (items > 1024) break;  // (more of them only cost more)
+    }
+  }
+  return best;
+}
+
+}  // namespace
+
 int launch_attn_window(AttnWindowParams p, const SeqBatch& s, void* workspace, hipStream_t st) {
-  constexpr int QI = 1, NW = 4;
-  const int rb = (16 * QI * NW) >> p.group_shift;
-  int rows = 0, longest = 0, nqb[kMaxSeqs], tiles[kMaxSeqs];
+  int rows = 0;
+  long long keys = 0;
   for (int b = 0; b < s.n; ++b) {
-    const int n = s.n_new[b];
-    rows += n;
+    rows += s.n_new[b];
     p.start[b] = s.start[b];
     p.row_end[b] = rows;
-    nqb[b] = (n + rb - 1) / rb;
-    tiles[b] = 0;
-    // the last block's run is the longest but for rounding to tiles
-    if (n) tiles[b] = tile_run(s.start[b] + (nqb[b] - 1) * rb, s.start[b] + n - 1, p.window, p.n_sinks).count;
-    longest = std::max(longest, tiles[b]);
+    keys += std::min(s.start[b] + s.n_new[b], p.window + p.n_sinks + s.n_new[b]);
   }
   if (!rows) return IE_OK;
-  // tiles a split: the least (rounds of the chip) x (a split's tiles + its fixed cost, 2) + the merge
-  const int room = workspace ? attn_window_part_rows(rows) : 0;
-  int best = std::max(longest, 1);
-  double best_cost = 1e30;
-  for (int n = 1; n <= kMaxSplits && n <= std::max(longest, 1); ++n) {
-    const int tps = (longest + n - 1) / n;
-    long long items = 0, part = 0;
-    for (int b = 0; b < s.n; ++b) {
-      const int k = std::max(1, (tiles[b] + tps - 1) / tps);
-      items += (long long)nqb[b] * k * kKVHeads;
-      if (k > 1) part += (long long)s.n_new[b] * k;
-    }
-    if (part > room) break;
-    const double cost = (double)((items + kSlots - 1) / kSlots) * (tps + 2) + (part ? 4 + part / 128.0 : 0);
-    if (cost < best_cost) best = tps, best_cost = cost;
-  }
+  const Plan plan = plan_of(p, s, rows, attn_window_part_rows(rows));
+  const int rb = (64 * plan.qi) >> p.group_shift;
   int items = 0, part = 0;
   for (int b = 0; b < s.n; ++b) {
-    p.splits[b] = std::max(1, (tiles[b] + best - 1) / best);
-    items += nqb[b] * p.splits[b];
+    const int n = s.n_new[b], nqb = (n + rb - 1) / rb;
+    int tiles = 0;
+    if (n)
+      tiles = std::max(tile_run(s.start[b], s.start[b] + std::min(rb, n) - 1, p.window, p.n_sinks).count,
+                       tile_run(s.start[b] + (nqb - 1) * rb, s.start[b] + n - 1, p.window, p.n_sinks).count);
+    p.splits[b] = std::max(1, (tiles + plan.tps - 1) / plan.tps);
+    items += nqb * p.splits[b];
     p.item_end[b] = items;
     p.part0[b] = part;
-    if (p.splits[b] > 1) part += s.n_new[b] * p.splits[b];
+    if (p.splits[b] > 1) part += n * p.splits[b];
   }
   p.n_seqs = s.n;
+  // a batch whose keys of all layers exceed the 256 MB cache finds none of them there: such keys, where one
+  // workgroup reads them, pass it by (16 tokens over 4096 keys: 55.7 us without, 47.9 with)
+  p.nt = keys > 2048;
   p.part = static_cast<float*>(workspace);
   p.part_ml = p.part + (size_t)part * (kKVHeads << p.group_shift) * kHeadDim;
-  hipLaunchKernelGGL((attn_window_kernel<QI, NW>), dim3(items * kKVHeads), dim3(64 * NW), 0, st, p);
+  const dim3 grid(items * kKVHeads), block(256);
+  if (plan.qi == 1)
+    hipLaunchKernelGGL(attn_window_16_kernel, grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL(attn_window_32_kernel, grid, block, 0, st, p);
   IE_CHECK_LAUNCH();
   if (part) {
     hipLaunchKernelGGL(attn_window_merge_kernel, dim3(rows << p.group_shift), dim3(256), 0, st, p);

@@ -104,3 +104,18 @@ def test_workspace_sizes(hip):
     assert lib.ie_attn_window_workspace_size(100000, 32) > 0
     assert lib.ie_kv_compact_workspace_size(1000) >= 8000
     assert lib.ie_sample_filtered_workspace_size(64, V) >= lib.ie_sample_filtered_workspace_size(1, V) > 0
+
+
+def test_window_attention_descriptors_stay_scalar(tmp_path):
+    """The window attention's K and V tile descriptors are in scalar registers: one that the compiler took
+    through a vector register would turn every load of a tile into a readfirstlane loop."""
+    import re
+    import shutil
+    from test_kernel_code import BUILD, LLVM, kernels
+    obj = BUILD / "k_attn_window.o"
+    if not obj.exists() or not shutil.which(LLVM / "llvm-objdump"):
+        pytest.skip("no object of the build, or no disassembler")
+    code = {k: v for k, v in kernels(obj, tmp_path).items() if "buffer_load" in v}
+    assert len(code) == 2
+    counts = {k: len(re.findall(r"\bv_readfirstlane_b32\b", v)) for k, v in code.items()}
+    assert max(counts.values()) <= 16, counts

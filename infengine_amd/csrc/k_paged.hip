@@ -13,23 +13,39 @@ namespace {
 // ---------------------------------------------------------------- norms, rotation, append
 // q' = rot(q * rsqrt(mean(q^2) + 1e-5) * w), the same for k (without a weight no norm), v as it
 // is; in fp32, rounded once.  16 lanes a head, 8 dims each; dim j and its partner j + 64 are 8
-// lanes apart.  A workgroup takes 16 heads of one row.
+// lanes apart.  A workgroup takes a row: GROUPS of 16 heads, the last one K and V.  A lane keeps its dims'
+// angles and weights over its heads (a workgroup for 16 heads, each with its own loads of the
+// angles, 64 bytes a lane beside 16 of the row, took 24.4 us for 7500 normed rows of 48 heads).
+template <int GROUPS>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p) {
-  const int tid = threadIdx.x, lane = tid & 63, li = tid & 15;
-  const int row = blockIdx.x, head = blockIdx.y * 16 + (tid >> 4);
-  const int b = __popcll(__ballot(lane < p.n_seqs && p.row_end[lane] <= row));
-  const int pos = p.start[b] + row - (b ? p.row_end[b - 1] : 0);
-  const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p.qkv + (size_t)row * p.qkv_stride +
-                                                      (size_t)head * kHeadDim + 8 * li);
-  const bool is_q = head < p.heads, is_v = head >= p.heads + kKVHeads;
-  u32x4_t y = x;
-  if (!is_v) {
-    float v[8];
+  const int tid = threadIdx.x, lane = tid & 63, li = tid & 15, hg = tid >> 4;
+  const int row = blockIdx.x;
+  // (the sequences' arguments in one go, a lane each)
+  const int row_end = p.row_end[lane], start = p.start[lane];
+  const u32x4_t* src = reinterpret_cast<const u32x4_t*>(p.qkv + (size_t)row * p.qkv_stride) + tid;
+  u32x4_t x[GROUPS];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[2 * e] = bf_lo(x[e]), v[2 * e + 1] = bf_hi(x[e]);
-    const uint16_t* w = is_q ? p.q_norm : p.k_norm;
-    if (w) {
-      const u32x4_t wv = *reinterpret_cast<const u32x4_t*>(w + 8 * li);
+  for (int j = 0; j < GROUPS; ++j) x[j] = ld_stream(src + 256 * j);
+  const u32x4_t none = {0, 0, 0, 0};
+  const u32x4_t wq = p.q_norm ? reinterpret_cast<const u32x4_t*>(p.q_norm)[li] : none;
+  const u32x4_t wk = p.k_norm ? reinterpret_cast<const u32x4_t*>(p.k_norm)[li] : none;
+  const int b = __popcll(__ballot(lane < p.n_seqs && row_end <= row));
+  const int before = b ? __builtin_amdgcn_readlane(row_end, max(b - 1, 0)) : 0;
+  const int pos = __builtin_amdgcn_readlane(start, b) + row - before;
+  const int page = p.block_tables[(size_t)b * p.table_stride + pos / kPagePos];
+  const float4* c4 = reinterpret_cast<const float4*>(p.rope_cos + (size_t)pos * 64 + 8 * (li & 7));
+  const float4* s4 = reinterpret_cast<const float4*>(p.rope_sin + (size_t)pos * 64 + 8 * (li & 7));
+  const float4 ca = c4[0], cb = c4[1], sa = s4[0], sb = s4[1];
+  const float c[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
+  const float s[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
+#pragma unroll
+  for (int j = 0; j < GROUPS; ++j) {
+    const bool is_q = j < GROUPS - 1, is_v = !is_q && hg >= kKVHeads;
+    float v[8], t[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[2 * e] = bf_lo(x[j][e]), v[2 * e + 1] = bf_hi(x[j][e]);
+    if (is_q ? p.q_norm : p.k_norm) {
+      const u32x4_t wv = is_q ? wq : wk;
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
@@ -40,61 +56,65 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p) {
         v[2 * e + 1] *= r * bf_hi(wv[e]);
       }
     }
-    const float4* c4 = reinterpret_cast<const float4*>(p.rope_cos + (size_t)pos * 64 + 8 * (li & 7));
-    const float4* s4 = reinterpret_cast<const float4*>(p.rope_sin + (size_t)pos * 64 + 8 * (li & 7));
-    const float4 ca = c4[0], cb = c4[1], sa = s4[0], sb = s4[1];
-    const float c[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
-    const float s[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
-    float t[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float other = dpp_f<0x128>(v[e]);  // row_ror 8: the partner dim
       t[e] = li < 8 ? rope_lo(v[e], other, c[e], s[e]) : rope_hi(other, v[e], c[e], s[e]);
     }
+    u32x4_t y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = pack_bf2(t[2 * e], t[2 * e + 1]);
+    if (is_q) {
+      reinterpret_cast<u32x4_t*>(p.q_out + (size_t)row * p.heads * kHeadDim)[256 * j + tid] = y;
+    } else if (page >= 0 && page < p.n_pages) {
+      uint16_t* dst = (is_v ? p.v : p.k) + (size_t)page * kPageElems +
+                      ((size_t)(hg & (kKVHeads - 1)) * kPagePos + pos % kPagePos) * kHeadDim;
+      reinterpret_cast<u32x4_t*>(dst)[li] = is_v ? x[j] : y;
+    }
   }
-  uint16_t* dst;
-  if (is_q) {
-    dst = p.q_out + ((size_t)row * p.heads + head) * kHeadDim;
-  } else {
-    const int page = p.block_tables[(size_t)b * p.table_stride + pos / kPagePos];
-    if (page < 0 || page >= p.n_pages) return;
-    const int kvh = (head - p.heads) & (kKVHeads - 1);
-    dst = (is_v ? p.v : p.k) + (size_t)page * kPageElems +
-          ((size_t)kvh * kPagePos + pos % kPagePos) * kHeadDim;
-  }
-  *reinterpret_cast<u32x4_t*>(dst + 8 * li) = y;
 }
 
 // ---------------------------------------------------------------- fork
+// The forks in groups that copy the same positions of the same row (continuations of one prompt).
 struct ForkParams {
   uint16_t* pages;
   int* tables;
   int n_pages, stride;
-  int src[kMaxSeqs], dst[kMaxSeqs], n_pos[kMaxSeqs], page[kMaxSeqs];
+  int src[kMaxSeqs], n_pos[kMaxSeqs], end[kMaxSeqs];  // by group; `end`: one past its last fork
+  int dst[kMaxSeqs], page[kMaxSeqs];                  // by fork
 };
 constexpr int kPlanes = kLayers * 2 * kKVHeads;  // [64][128] planes of a page
+constexpr int kPlanePieces = (int)(kPageHead / 8);  // 16-byte pieces of a plane
+static_assert(kPlanes >= kMaxSeqs, "a workgroup for every table row of a group");
 
-// blockIdx.y: the fork.  The first n_pos % 64 positions of the source's last page, plane by plane;
-// the first workgroup also writes the table row.
+// blockIdx.x: a plane, blockIdx.y: a group.  The first n_pos % 64 positions of the plane in the source's
+// last page are read once and written to every fork's page; the first workgroups also write a table
+// row each.  Bound by the stores (16 forks of 58 positions, 122 MB: 31 us with a copy per
+// fork).
 __global__ __launch_bounds__(256) void kv_fork_kernel(ForkParams p) {
-  const int f = blockIdx.y, full = p.n_pos[f] / kPagePos, part = p.n_pos[f] % kPagePos;
-  const int* from = p.tables + (size_t)p.src[f] * p.stride;
-  if (blockIdx.x == 0) {
-    int* to = p.tables + (size_t)p.dst[f] * p.stride;
+  const int g = blockIdx.y, plane = blockIdx.x;
+  const int first = g ? p.end[g - 1] : 0, end = p.end[g];
+  const int full = p.n_pos[g] / kPagePos, part = p.n_pos[g] % kPagePos;
+  const int* from = p.tables + (size_t)p.src[g] * p.stride;
+  if (first + plane < end) {
+    int* to = p.tables + (size_t)p.dst[first + plane] * p.stride;
     for (int i = threadIdx.x; i < p.stride; i += 256)
-      to[i] = i < full ? from[i] : i == full && part ? p.page[f] : -1;
+      to[i] = i < full ? from[i] : i == full && part ? p.page[first + plane] : -1;
   }
   if (!part) return;
   const int src = from[full];
   if (src < 0 || src >= p.n_pages) return;
-  const u32x4_t* s = reinterpret_cast<const u32x4_t*>(p.pages + (size_t)src * kPageElems);
-  u32x4_t* d = reinterpret_cast<u32x4_t*>(p.pages + (size_t)p.page[f] * kPageElems);
-  const int n = part * (kHeadDim / 8);  // 16-byte pieces a plane
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < n * kPlanes; i += gridDim.x * 256) {
-    const int at = i / n * (kPagePos * kHeadDim / 8) + i % n;
-    d[at] = s[at];
+  const int n = part * (kHeadDim / 8);
+  const size_t at = (size_t)plane * kPlanePieces + threadIdx.x;
+  u32x4_t v[kPlanePieces / 256];
+#pragma unroll
+  for (int u = 0; u < kPlanePieces / 256; ++u)
+    v[u] = reinterpret_cast<const u32x4_t*>(p.pages + (size_t)src * kPageElems)[at + min(256 * u, n - 1)];
+  for (int f = first; f < end; ++f) {
+    u32x4_t* d = reinterpret_cast<u32x4_t*>(p.pages + (size_t)p.page[f] * kPageElems) + at;
+#pragma unroll
+    for (int u = 0; u < kPlanePieces / 256; ++u)
+      if ((int)threadIdx.x + 256 * u < n) __builtin_nontemporal_store(v[u], d + 256 * u);
   }
 }
 
@@ -217,7 +237,13 @@ int launch_qk_norm_rope(QkNormRopeParams p, const SeqBatch& s, hipStream_t st) {
   if (!rows) return IE_OK;
   p.n_seqs = s.n;
   p.rows = rows;
-  hipLaunchKernelGGL(qk_norm_rope_kernel, dim3(rows, (p.heads + 2 * kKVHeads) / 16), dim3(256), 0, st, p);
+  const dim3 grid(rows), block(256);
+  if (p.heads == 16)
+    hipLaunchKernelGGL((qk_norm_rope_kernel<2>), grid, block, 0, st, p);
+  else if (p.heads == 32)
+    hipLaunchKernelGGL((qk_norm_rope_kernel<3>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((qk_norm_rope_kernel<5>), grid, block, 0, st, p);
   IE_CHECK_LAUNCH();
   return IE_OK;
 }
@@ -230,13 +256,21 @@ int launch_kv_fork(int n_forks, const int* src_rows, const int* dst_rows, const 
   p.tables = tables;
   p.n_pages = n_pages;
   p.stride = stride;
+  int groups = 0, n = 0;
+  bool done[kMaxSeqs] = {};
   for (int f = 0; f < n_forks; ++f) {
-    p.src[f] = src_rows[f];
-    p.dst[f] = dst_rows[f];
-    p.n_pos[f] = n_pos[f];
-    p.page[f] = new_pages[f];
+    if (done[f]) continue;
+    p.src[groups] = src_rows[f];
+    p.n_pos[groups] = n_pos[f];
+    for (int i = f; i < n_forks; ++i) {
+      if (src_rows[i] != src_rows[f] || n_pos[i] != n_pos[f]) continue;
+      done[i] = true;
+      p.dst[n] = dst_rows[i];
+      p.page[n++] = new_pages[i];
+    }
+    p.end[groups++] = n;
   }
-  hipLaunchKernelGGL(kv_fork_kernel, dim3(128, n_forks), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(kv_fork_kernel, dim3(kPlanes, groups), dim3(256), 0, st, p);
   IE_CHECK_LAUNCH();
   return IE_OK;
 }

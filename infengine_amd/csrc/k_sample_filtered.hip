@@ -36,6 +36,7 @@ typedef unsigned long long u64;
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kChunks = 16, kBins = 256;    // (at most 16 chunks)
 constexpr int kRound = 8;                   // logits a thread and round
+constexpr int kSmall = 64;                  // tokens listed whole, one a lane of the finish
 constexpr double kUnit = 4398046511104.0;   // 2^42: masses of listed tokens (2^21 fit 63 bits)
 constexpr double kChunkUnit = 35184372088832.0;  // 2^45: of a chunk's tokens (2^18 fit 63 bits)
 static_assert(kSampleMaxVocab <= 1 << 21 && kSampleMaxVocab / (kChunks / 2) <= 1 << 18, "sums in 64 bits");
@@ -47,6 +48,7 @@ struct Row {
   u64 total[kChunks];         // rows without cuts: the chunk's mass, relative to its max
   double kept[kChunks];       // mass of the chunk's tokens in bins above the cuts'
   int p_lo, p_hi, k_bin;
+  int small;                  // -1, or: every token that can be kept is listed (bins up to this one)
   u64 k_above;                // tokens in the bins above k_bin
   double mass_k, mass_p;      // masses of the bins above k_bin, above p_lo
   unsigned int count[kChunks][kBins];
@@ -362,6 +364,7 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
   __shared__ double part_m[4][kBins];
   __shared__ double powers[64];
   __shared__ CutBins s_cut;
+  __shared__ bool s_small;
   __shared__ int s_cnt[kWaves];
   const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -377,78 +380,96 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
   __syncthreads();
   const bool cuts = s.top_k || s.p;
   CutBins cut{kBins, -1, -2, -1};
-  if (cuts) {
-    // the row's histogram: thread (bin, quarter of the chunks), then the quarters in order
-    const int b = tid & (kBins - 1), q = tid / kBins;
+  // the row's histogram: thread (bin, quarter of the chunks), then the quarters in order
+  const int b = tid & (kBins - 1), q = tid / kBins;
+  bool small = false;
+  if (s.top_k) {
     u64 count = 0;
-    double mass = 0.0;
     for (int j = 0; j < p.chunks / 4; ++j) {
       const int ch = q * (p.chunks / 4) + j;
-      const float cm = R.pmax[ch];
-      const int from = b - bin(cm);  // (bin(-inf) = kBins: none)
-      if (from < 0) continue;
-      if (s.top_k) count += R.count[ch][from];
-      if (s.p) mass += (double)R.mass[ch][from] * weight(cm);
+      const int from = b - bin(R.pmax[ch]);  // (bin(-inf) = kBins: none)
+      if (from >= 0) count += R.count[ch][from];
     }
     part_c[q][b] = count;
-    part_m[q][b] = mass;
     __syncthreads();
     if (wave == 0) {  // lane l: bins 4 l .. 4 l + 3
-      u64 n[4], nsum = 0;
-      double m[4], msum = 0.0;
+      u64 n[4], nsum = 0, above;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int b4 = 4 * lane + j;
         nsum += n[j] = (part_c[0][b4] + part_c[1][b4]) + (part_c[2][b4] + part_c[3][b4]);
-        msum += m[j] = ((part_m[0][b4] + part_m[1][b4]) + (part_m[2][b4] + part_m[3][b4])) * (1.0 / kChunkUnit);
       }
       const u64 ninc = wave_scan_inc(nsum);
-      const double minc = wave_scan_inc(msum);
-      u64 k_above = 0;
-      double mass_k = lane_value(minc, 63), mass_k_incl = mass_k, mass_p = 0.0, none;
-      if (s.top_k) {
-        cut.k_bin = first_bin(ninc, nsum, n, (u64)s.top_k, &k_above);
-        if (cut.k_bin == kBins) {
-          cut.k_bin = -1;  // the first top_k reach past every token that weighs anything
-        } else {
-          // masses up to that bin, without it and with it
-          double below = minc - msum, own = 0.0;
+      const int k_bin = first_bin(ninc, nsum, n, (u64)s.top_k, &above);
+      u64 upto = ninc - nsum;  // tokens up to and with that bin, in its lane
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (4 * lane + j < cut.k_bin) below += m[j];
-            if (4 * lane + j == cut.k_bin) own = m[j];
-          }
-          mass_k = lane_value(below, cut.k_bin >> 2);
-          mass_k_incl = mass_k + lane_value(own, cut.k_bin >> 2);
-          cut.lo = cut.k_bin;
-        }
-      }
-      if (s.p) {
-        // Z lies between the masses without and with k_bin (which part of it is kept is not known yet)
-        const double tiny = 1.0 / kUnit, last = mass_k_incl;
-        cut.p_lo = first_bin(minc, msum, m, fmin(fmax(mass_k * s.top_p * (1.0 - 1e-12), tiny), last), &mass_p);
-        cut.p_hi = first_bin(minc, msum, m, fmin(fmax(mass_k_incl * s.top_p * (1.0 + 1e-12), tiny), last), &none);
-        const int most = cut.k_bin >= 0 ? cut.k_bin : kBins - 1;
-        cut.p_hi = min(cut.p_hi, most);
-        cut.p_lo = min(cut.p_lo, cut.p_hi);
-        cut.lo = cut.p_lo;
-      }
+      for (int j = 0; j < 4; ++j)
+        if (4 * lane + j <= k_bin) upto += n[j];
+      upto = lane_value(upto, min(k_bin >> 2, 63));
       if (lane == 0) {
-        s_cut = cut;
-        if (c == 0) {
-          R.k_above = k_above;
-          R.mass_k = mass_k;
-          R.mass_p = mass_p;
-        }
+        // (kBins: the first top_k reach past every token that weighs anything)
+        s_cut.k_bin = k_bin < kBins ? k_bin : -1;
+        s_small = upto <= kSmall;
+        if (c == 0) R.k_above = above, R.small = upto <= kSmall ? (int)min(k_bin, kBins - 1) : -1;
       }
     }
     __syncthreads();
-    cut = s_cut;
+    cut.k_bin = s_cut.k_bin;
+    small = s_small;
+    // a row whose first tokens are few has them all listed: nothing else of it is needed
+    if (small) cut = CutBins{0, 0, cut.k_bin < 0 ? kBins - 1 : cut.k_bin, cut.k_bin};
+    else if (cut.k_bin >= 0) cut.lo = cut.k_bin;
+  } else if (c == 0 && tid == 0) {
+    R.small = -1;
+  }
+  if (s.p && !small) {
+    double mass = 0.0;
+    for (int j = 0; j < p.chunks / 4; ++j) {
+      const int ch = q * (p.chunks / 4) + j;
+      const float cm = R.pmax[ch];
+      const int from = b - bin(cm);
+      if (from >= 0) mass += (double)R.mass[ch][from] * weight(cm);
+    }
+    part_m[q][b] = mass;
+    __syncthreads();
+    if (wave == 0) {
+      double m[4], msum = 0.0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int b4 = 4 * lane + j;
+        msum += m[j] = ((part_m[0][b4] + part_m[1][b4]) + (part_m[2][b4] + part_m[3][b4])) * (1.0 / kChunkUnit);
+      }
+      const double minc = wave_scan_inc(msum);
+      double mass_k = lane_value(minc, 63), mass_k_incl = mass_k, mass_p = 0.0, none;
+      if (cut.k_bin >= 0) {
+        // masses up to that bin, without it and with it
+        double below = minc - msum, own = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (4 * lane + j < cut.k_bin) below += m[j];
+          if (4 * lane + j == cut.k_bin) own = m[j];
+        }
+        mass_k = lane_value(below, cut.k_bin >> 2);
+        mass_k_incl = mass_k + lane_value(own, cut.k_bin >> 2);
+      }
+      // Z lies between the masses without and with k_bin (which part of it is kept is not known yet)
+      const double tiny = 1.0 / kUnit, last = mass_k_incl;
+      const int p_lo = first_bin(minc, msum, m, fmin(fmax(mass_k * s.top_p * (1.0 - 1e-12), tiny), last), &mass_p);
+      const int p_hi = first_bin(minc, msum, m, fmin(fmax(mass_k_incl * s.top_p * (1.0 + 1e-12), tiny), last), &none);
+      if (lane == 0) {
+        s_cut.p_hi = min(p_hi, cut.k_bin >= 0 ? cut.k_bin : kBins - 1);
+        s_cut.p_lo = min(p_lo, s_cut.p_hi);
+        if (c == 0) R.mass_k = mass_k, R.mass_p = mass_p;
+      }
+    }
+    __syncthreads();
+    cut.lo = cut.p_lo = s_cut.p_lo;
+    cut.p_hi = s_cut.p_hi;
   }
   if (c == 0 && tid == 0) R.p_lo = cut.p_lo, R.p_hi = cut.p_hi, R.k_bin = cut.k_bin;
   // The chunk's certain mass: from the histogram (or the total) where there is one and no min-p, else
   // token by token
-  const bool summed = !s.m && (s.p || !cuts);
+  const bool summed = !s.m && !small && (s.p || !cuts);
   double low = 0.0;
   if (summed) {
     const float cm = R.pmax[c];
@@ -529,11 +550,57 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 }
 
 constexpr int kDigits = 2048;
-constexpr int kInLds = 4096;  // listed tokens kept in LDS
+constexpr int kHeld = 4;          // listed tokens a thread holds
+constexpr int kScan = 16;         // logits a thread and round of the last scan
+
+// A row whose tokens are all listed, at most one a lane: one wave, no barrier.
+__device__ __forceinline__ int finish_small(const SampleParams& p, const Setting& s, Row& R, int row, int cl,
+                                            const Weigher& weight, u64* by_rank) {
+  const int lane = threadIdx.x & 63;
+  const int own_n = lane < p.chunks ? R.n_listed[lane] : 0, upto = wave_scan_inc(own_n);
+  const int n = lane_value(upto, 63);
+  int c = 0, before = 0;
+  for (int k = 0; k < p.chunks - 1; ++k) {
+    const int end = lane_value(upto, k);
+    if (lane >= end) c = k + 1, before = end;
+  }
+  Listed t{-INFINITY, -1};
+  if (lane < n) t = row_list(R, c, cl)[lane - before];
+  // places in the order (the list is in id order)
+  int rank = 0;
+  for (int j = 0; j < n; ++j) {
+    const float l = lane_value(t.l, j);
+    rank += l > t.l || (l == t.l && j < lane);
+  }
+  const double w = weight(t.l);
+  const bool in_k = lane < n && (!s.top_k || rank < s.top_k);
+  u64 q = in_k ? in_units(w, kUnit) : 0;
+  bool keep = in_k && (!s.m || w >= (double)s.min_p);
+  if (s.p) {
+    // the masses in the order: those before a token short of the share of them all
+    // (one wave: its LDS accesses are in order; the fences hold the compiler to it)
+    by_rank[lane] = 0;
+    __builtin_amdgcn_wave_barrier();
+    if (lane < n) by_rank[rank] = q;
+    __builtin_amdgcn_wave_barrier();
+    const u64 sorted = by_rank[lane], inc = wave_scan_inc(sorted), z = lane_value(inc, 63);
+    __builtin_amdgcn_wave_barrier();
+    by_rank[lane] = inc - sorted;
+    __builtin_amdgcn_wave_barrier();
+    const double share = ceil((double)z * (double)s.top_p);
+    const u64 want = share < 1.0 ? 1 : share > (double)z ? z : (u64)share;
+    keep = keep && by_rank[min(rank, 63)] < want;
+  }
+  keep = keep || (lane < n && rank == 0);
+  if (!keep) q = 0;
+  const u64 inc = wave_scan_inc(q), z = lane_value(inc, 63);
+  const double x = (double)z * fmax((double)p.uniform[row], 0.0);  // (a NaN too: 0)
+  const u64 at = x < (double)z ? min((u64)x, z - 1) : z - 1;
+  return lane_value(t.id, __ffsll((long long)__ballot(inc > at)) - 1);
+}
 
 __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p, void* ws) {
   __shared__ u64 hist[kDigits];
-  __shared__ Listed held[kInLds];
   __shared__ u64 red[kWaves];
   __shared__ u64 listed_of[kChunks];
   __shared__ double powers[64];
@@ -550,66 +617,85 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     if (tid == 0) p.out[row] = -1;
     return;
   }
+  if (tid < 64) powers[tid] = kPowers.v[tid];
   const Binner bin(mx, s.inv_t);
   const Weigher weight(powers, mx, s.inv_t);
   const int cl = chunk_len(p.vocab, p.chunks);
+  if (R.small >= 0) {
+    if (tid >= 64) return;
+    const int token = finish_small(p, s, R, row, cl, weight, hist);
+    if (tid == 0) p.out[row] = token;
+    return;
+  }
   const int p_lo = R.p_lo, p_hi = R.p_hi, k_bin = R.k_bin;
   if (tid < 64) {
-    const int n = tid < p.chunks ? R.n_listed[tid] : 0;
-    const int inc = wave_scan_inc(n);
+    const int inc = wave_scan_inc(tid < p.chunks ? R.n_listed[tid] : 0);
     if (tid < kChunks) {
       offset[tid + 1] = inc;
       listed_of[tid] = 0;
     }
-    powers[tid] = kPowers.v[tid];
     if (tid == 0) offset[0] = 0;
   }
   __syncthreads();
   const int n = offset[kChunks];
-  const bool in_lds = n <= kInLds;
-  // listed token j, in id order
-  const auto fetch = [&](int j) {
+  const auto chunk_of = [&](int j) {
     int c = 0;
 #pragma unroll
     for (int k = 1; k < kChunks; ++k) c += j >= offset[k];
-    return row_list(R, c, cl)[j - offset[c]];
+    return c;
   };
-  if (in_lds)
-    for (int j = tid; j < n; j += kThreads) held[j] = fetch(j);
-  __syncthreads();
-  const auto token = [&](int j) { return in_lds ? held[j] : fetch(j); };
+  // The listed tokens in rounds of kHeld a thread, in id order slab by slab; most rows have one round, whose
+  // tokens stay in registers.  (past the end: bin kBins)
+  Listed held[kHeld];
+  const auto load_held = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const int j = j0 + u * kThreads + tid, c = chunk_of(j);
+      held[u] = j < n ? row_list(R, c, cl)[j - offset[c]] : Listed{-INFINITY, -1};
+    }
+  };
+  const bool one_round = n <= kHeld * kThreads;
+  if (one_round) load_held(0);
 
-  // The cut where the sum of f over the listed tokens that `in` takes, in the order, reaches target >= 1
+  // The cut where the sum of f over the listed tokens (0: not among them), in the order, reaches target >= 1
   // (never: all of them stay): a radix select of the key from the first bits in which they differ, then,
   // among equal keys (equal f), the id of the last one needed.
-  const auto select = [&](auto in, auto f, u64 target) {
+  const auto select = [&](auto f, u64 target) {
     if (tid == 0) s_min = 0xFFFFFFFFu, s_max = 0;
     __syncthreads();
-    uint32_t kmin = 0xFFFFFFFFu, kmax = 0;
-    for (int j = tid; j < n; j += kThreads) {
-      const Listed t = token(j);
-      if (!in(t)) continue;
-      const uint32_t k = logit_key(t.l);
-      kmin = min(kmin, k), kmax = max(kmax, k);
+    uint32_t key[kHeld], kmin = 0xFFFFFFFFu, kmax = 0;
+    u64 q[kHeld];
+    const auto weigh = [&]() {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) key[u] = logit_key(held[u].l), q[u] = f(held[u]);
+    };
+    for (int j0 = 0; j0 < n; j0 += kHeld * kThreads) {
+      if (!one_round) load_held(j0);
+      weigh();
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u)
+        if (q[u]) kmin = min(kmin, key[u]), kmax = max(kmax, key[u]);
     }
     if (kmin <= kmax) atomicMin(&s_min, kmin), atomicMax(&s_max, kmax);
     __syncthreads();
+    if (s_min > s_max) return Cut{-INFINITY, 0x7FFFFFFF};  // (they weigh nothing)
     uint32_t base = s_min, span = s_max - s_min;  // keys base .. base + span are left
     while (span) {
       const int shift = max(0, 32 - __clz(span) - 11);
-      for (int d = tid; d < kDigits; d += kThreads) hist[d] = 0;
+      hist[tid] = 0, hist[tid + kThreads] = 0;
       __syncthreads();
-      for (int j = tid; j < n; j += kThreads) {
-        const Listed t = token(j);
-        const uint32_t k = logit_key(t.l) - base;
-        if (in(t) && k <= span) atomicAdd(&hist[k >> shift], f(t));
+      for (int j0 = 0; j0 < n; j0 += kHeld * kThreads) {
+        if (!one_round) load_held(j0), weigh();
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+          if (q[u] && key[u] - base <= span) atomicAdd(&hist[(key[u] - base) >> shift], q[u]);
       }
       __syncthreads();
       // digits from the largest: thread t has kDigits - 1 - 2 t and the one below
+      static_assert(kDigits == 2 * kThreads, "two digits a thread");
       const u64 h0 = hist[kDigits - 1 - 2 * tid], h1 = hist[kDigits - 2 - 2 * tid];
       u64 all;
       const u64 inc = block_scan(h0 + h1, red, &all);
-      if (all == 0) return Cut{-INFINITY, 0x7FFFFFFF};  // (they weigh nothing)
       if (target > all) target = all;
       if (inc >= target && inc - (h0 + h1) < target) {  // exactly one thread
         const bool first = inc - h1 >= target;
@@ -625,19 +711,17 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     // the tokens with that key, in id order
     if (tid == 0) s_id = 0x7FFFFFFE;
     u64 before = 0;
-    for (int j0 = 0; j0 < n && before < target; j0 += kThreads) {
-      const int j = j0 + tid;
-      u64 q = 0;
-      int id = 0;
-      if (j < n) {
-        const Listed t = token(j);
-        id = t.id;
-        if (in(t) && logit_key(t.l) == base) q = f(t);
+    for (int j0 = 0; j0 < n && before < target; j0 += kHeld * kThreads) {
+      if (!one_round) load_held(j0), weigh();
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        if (j0 + u * kThreads >= n) break;  // (the workgroup's)
+        const u64 own = key[u] == base ? q[u] : 0;
+        u64 all;
+        const u64 inc = before + block_scan(own, red, &all);
+        if (own && inc >= target && inc - own < target) s_id = held[u].id;
+        before += all;
       }
-      u64 all;
-      const u64 inc = before + block_scan(q, red, &all);
-      if (q && inc >= target && inc - q < target) s_id = id;
-      before += all;
     }
     __syncthreads();
     const Cut c{key_logit(base), s_id + 1};
@@ -648,26 +732,27 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
 
   Cut k_cut{-INFINITY, 0x7FFFFFFF}, cut = k_cut;
   if (k_bin >= 0) {
-    k_cut = select([&](Listed t) { return bin(t.l) == k_bin; }, [](Listed) { return (u64)1; },
-                   (u64)s.top_k - R.k_above);
+    k_cut = select([&](const Listed& t) { return (u64)(bin(t.l) == k_bin); }, (u64)s.top_k - R.k_above);
     cut = k_cut;
   }
   if (s.p) {
     double z = R.mass_k;  // of the bins above k_bin (of all: no such cut)
     if (k_bin >= 0) {
       u64 in_bin = 0;
-      for (int j = tid; j < n; j += kThreads) {
-        const Listed t = token(j);
-        if (bin(t.l) == k_bin && k_cut.keeps(t.l, t.id)) in_bin += mass(t.l);
+      for (int j0 = 0; j0 < n; j0 += kHeld * kThreads) {
+        if (!one_round) load_held(j0);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+          if (bin(held[u].l) == k_bin && k_cut.keeps(held[u].l, held[u].id)) in_bin += mass(held[u].l);
       }
       z += (double)block_sum(in_bin, red) * (1.0 / kUnit);
     }
     const double want = ceil((z * (double)s.top_p - R.mass_p) * kUnit);
-    cut = select([&](Listed t) {
+    cut = select([&](const Listed& t) -> u64 {
                    const int b = bin(t.l);
-                   return b >= p_lo && b <= p_hi && k_cut.keeps(t.l, t.id);
+                   return b >= p_lo && b <= p_hi && k_cut.keeps(t.l, t.id) ? mass(t.l) : 0;
                  },
-                 [&](Listed t) { return mass(t.l); }, want > 1.0 ? (u64)want : (u64)1);
+                 want > 1.0 ? (u64)want : (u64)1);
   }
   // (what is kept lies at or above the cut, the bins above it with it; a cut keeps all that weighs
   // something where there is none)
@@ -677,14 +762,13 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     return !s.m || w >= (double)s.min_p ? in_units(w, unit) : 0;
   };
   // the chunks' kept masses
-  for (int j = tid; j < n; j += kThreads) {
-    const Listed t = token(j);
-    const u64 q = kept_mass(t.l, t.id, kUnit);
-    if (!q) continue;
-    int c = 0;
+  for (int j0 = 0; j0 < n; j0 += kHeld * kThreads) {
+    if (!one_round) load_held(j0);
 #pragma unroll
-    for (int k = 1; k < kChunks; ++k) c += j >= offset[k];
-    atomicAdd(&listed_of[c], q);
+    for (int u = 0; u < kHeld; ++u) {
+      const u64 q = held[u].id >= 0 ? kept_mass(held[u].l, held[u].id, kUnit) : 0;
+      if (q) atomicAdd(&listed_of[chunk_of(j0 + u * kThreads + tid)], q);
+    }
   }
   __syncthreads();
   if (tid < 64) {
@@ -704,23 +788,23 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   const int beg = s_digit * cl, end = min(p.vocab, beg + cl);
   u64 before = 0;
   int last = -1;
-  for (int i = beg; i < end && before <= at; i += kRound * kThreads) {
-    // kRound ids in a row a thread: one scan a round
-    float v[kRound];
-    u64 q[kRound], own = 0;
+  for (int i = beg; i < end && before <= at; i += kScan * kThreads) {
+    // kScan ids in a row a thread: one scan a round
+    float v[kScan];
+    u64 q[kScan], own = 0;
 #pragma unroll
-    for (int u = 0; u < kRound; ++u) v[u] = L[min(i + tid * kRound + u, end - 1)];
+    for (int u = 0; u < kScan; ++u) v[u] = L[min(i + tid * kScan + u, end - 1)];
 #pragma unroll
-    for (int u = 0; u < kRound; ++u) {
-      const int id = i + tid * kRound + u;
+    for (int u = 0; u < kScan; ++u) {
+      const int id = i + tid * kScan + u;
       own += q[u] = id < end ? kept_mass(v[u], id, kChunkUnit) : 0;
       if (q[u]) last = id;
     }
     u64 all;
     u64 upto = before + block_scan(own, red, &all) - own;
 #pragma unroll
-    for (int u = 0; u < kRound; ++u) {
-      if (upto <= at && at < upto + q[u]) p.out[row] = i + tid * kRound + u;  // at most one token
+    for (int u = 0; u < kScan; ++u) {
+      if (upto <= at && at < upto + q[u]) p.out[row] = i + tid * kScan + u;  // at most one token
       upto += q[u];
     }
     before += all;

@@ -45,7 +45,7 @@ static_assert(kSampleMaxVocab <= 1 << 21 && kSampleMaxVocab / (kChunks / 2) <= 1
 struct Row {
   float pmax[kChunks];
   int n_listed[kChunks];
-  u64 total[kChunks];         // rows without cuts: the chunk's mass, relative to its max
+  u64 total[kChunks];         // rows without top_k: the chunk's mass, relative to its max
   double kept[kChunks];       // mass of the chunk's tokens in bins above the cuts'
   int p_lo, p_hi, k_bin;
   int small;                  // -1, or: every token that can be kept is listed (bins up to this one)
@@ -82,6 +82,7 @@ struct Setting {
   float top_p;     // used when p
   float min_p;
   int m_bins;      // no token of a bin past it reaches min_p (used when m)
+  int p_bins;      // no bin past it holds top_p's cut (used when p without top_k)
   bool p, m;
 };
 __device__ __forceinline__ Setting setting(const SampleParams& p, int row) {
@@ -97,6 +98,9 @@ __device__ __forceinline__ Setting setting(const SampleParams& p, int row) {
   s.m = !greedy && mp > 0.f;
   s.min_p = mp;
   s.m_bins = s.m ? (int)fminf(-8.0f * __logf(mp), (float)kBins) + 2 : 0;
+  // the tokens past d nats below the largest weigh at most vocab exp(-d), which is less than the share
+  // left out, (1 - top_p) of at least 1, from here on
+  s.p_bins = s.p ? (int)fminf(8.0f * (__logf((float)p.vocab) - __logf(fmaxf(1.0f - s.top_p, 1e-7f))), (float)kBins - 3) + 2 : 0;
   return s;
 }
 
@@ -204,6 +208,16 @@ __device__ __forceinline__ T lane_value(T v, int lane) {
   }
 }
 
+// Smallest of the wave, on every lane.
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
+  const auto step = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
+  v = step(v, __builtin_amdgcn_update_dpp(~0, (int)v, kDppQuadXor1, 0xF, 0xF, false));
+  v = step(v, __builtin_amdgcn_update_dpp(~0, (int)v, kDppQuadXor2, 0xF, 0xF, false));
+  v = step(v, __builtin_amdgcn_update_dpp(~0, (int)v, kDppRowHalfMirror, 0xF, 0xF, false));
+  v = step(v, __builtin_amdgcn_update_dpp(~0, (int)v, kDppRowMirror, 0xF, 0xF, false));
+  return step(step(lane_value(v, 0), lane_value(v, 16)), step(lane_value(v, 32), lane_value(v, 48)));
+}
+
 // Inclusive scan over the workgroup and its total; `red` is a scratch of kWaves values.
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, T* red, T* total) {
@@ -284,23 +298,12 @@ __global__ __launch_bounds__(kThreads, 8) void sample_hist_kernel(SampleParams p
   if (tid == 0) R.pmax[c] = mx;
   const Weigher weight(powers, mx, s.inv_t);
   const bool one_round = end - beg <= kRound * kThreads;
-  if (!s.top_k && !s.p) {
-    if (s.m) return;
-    u64 sum = 0;
-    if (mx > -INFINITY)
-      for (int i = beg; i < end; i += kRound * kThreads) {
-        if (!one_round) load_round(L, i, end, v);
-#pragma unroll
-        for (int u = 0; u < kRound; ++u) sum += in_units(weight(v[u]), kChunkUnit);
-      }
-    sum = block_sum(sum, red);
-    if (tid == 0) R.total[c] = sum;
-    return;
-  }
+  if (!s.top_k && !s.p && s.m) return;
+  u64 sum = 0;
   if (mx > -INFINITY) {
     const Binner bin(mx, s.inv_t);
     const int copy = (lane & (kCopies - 1)) * kBins;
-    int last = kBins - 1;
+    int last = s.p ? s.p_bins : -1;  // bins counted
     if (s.top_k) {
       // as many threads' largest tokens as top_k lie in the bins up to `last`: the chunk's first top_k do
       // too, and the bins behind need no count (they keep those threads' part of it)
@@ -328,13 +331,24 @@ __global__ __launch_bounds__(kThreads, 8) void sample_hist_kernel(SampleParams p
 #pragma unroll
       for (int u = 0; u < kRound; ++u) {
         const int b = bin(v[u]);
-        if (b > last) continue;
-        const bool again = !counted && v[u] == own_max;
-        counted |= again;
-        if (s.top_k && !again) atomicAdd(&count[copy + b], 1u);
-        if (s.p) atomicAdd(&mass[copy + b], in_units(weight(v[u]), kChunkUnit));
+        if (s.top_k) {
+          if (b > last) continue;
+          const bool again = !counted && v[u] == own_max;
+          counted |= again;
+          if (!again) atomicAdd(&count[copy + b], 1u);
+          if (s.p) atomicAdd(&mass[copy + b], in_units(weight(v[u]), kChunkUnit));
+        } else {
+          const u64 q = in_units(weight(v[u]), kChunkUnit);
+          sum += q;
+          if (b <= last) atomicAdd(&mass[copy + b], q);
+        }
       }
     }
+  }
+  if (!s.top_k) {
+    sum = block_sum(sum, red);
+    if (tid == 0) R.total[c] = sum;
+    if (!s.p) return;
   }
   __syncthreads();
   if (tid < kBins) {
@@ -440,7 +454,13 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
         msum += m[j] = ((part_m[0][b4] + part_m[1][b4]) + (part_m[2][b4] + part_m[3][b4])) * (1.0 / kChunkUnit);
       }
       const double minc = wave_scan_inc(msum);
-      double mass_k = lane_value(minc, 63), mass_k_incl = mass_k, mass_p = 0.0, none;
+      double mass_k = lane_value(minc, 63);
+      if (!s.top_k) {  // (bins past those that can hold the cut are not summed)
+        const float cm = lane < p.chunks ? R.pmax[lane] : -INFINITY;
+        const double own = cm > -INFINITY ? (double)R.total[lane] * weight(cm) * (1.0 / kChunkUnit) : 0.0;
+        mass_k = fmax(mass_k, lane_value(wave_scan_inc(own), 63));
+      }
+      double mass_k_incl = mass_k, mass_p = 0.0, none;
       if (cut.k_bin >= 0) {
         // masses up to that bin, without it and with it
         double below = minc - msum, own = 0.0;
@@ -453,7 +473,7 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
         mass_k_incl = mass_k + lane_value(own, cut.k_bin >> 2);
       }
       // Z lies between the masses without and with k_bin (which part of it is kept is not known yet)
-      const double tiny = 1.0 / kUnit, last = mass_k_incl;
+      const double tiny = 1.0 / kUnit, last = lane_value(minc, 63);
       const int p_lo = first_bin(minc, msum, m, fmin(fmax(mass_k * s.top_p * (1.0 - 1e-12), tiny), last), &mass_p);
       const int p_hi = first_bin(minc, msum, m, fmin(fmax(mass_k_incl * s.top_p * (1.0 + 1e-12), tiny), last), &none);
       if (lane == 0) {
@@ -492,6 +512,9 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
   }
   Listed* list = row_list(R, c, cl);
   const int sum_bins = summed ? 0 : s.m ? min(cut.lo, s.m_bins) : cut.lo;  // bins summed token by token
+  // no bin past `needed` matters: floor(l x scale) >= top - needed is l x scale >= it
+  const int needed = max(max(sum_bins - 1, cut.k_bin), cut.p_hi);
+  const float least = bin.top - (float)needed;
   u64 sum = 0;
   int listed = 0;
   // (beg and end are the workgroup's: every thread runs every round and its barriers)
@@ -502,6 +525,9 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
     int before = 0, place[kRound];
 #pragma unroll
     for (int u = 0; u < kRound; ++u) {
+      place[u] = 0;
+      // (most rows need few tokens: one product and comparison for the others)
+      if (!__ballot(v[u] * bin.scale >= least)) continue;
       const int b = bin(v[u]);
       if (b < sum_bins && b < kBins) {
         const double w = weight(v[u]);
@@ -676,7 +702,9 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
       for (int u = 0; u < kHeld; ++u)
         if (q[u]) kmin = min(kmin, key[u]), kmax = max(kmax, key[u]);
     }
-    if (kmin <= kmax) atomicMin(&s_min, kmin), atomicMax(&s_max, kmax);
+    // (a wave's first: 1024 additions to one place wait for each other, 16000 cycles)
+    kmin = wave_min_u32(kmin), kmax = ~wave_min_u32(~kmax);
+    if (lane == 0 && kmin <= kmax) atomicMin(&s_min, kmin), atomicMax(&s_max, kmax);
     __syncthreads();
     if (s_min > s_max) return Cut{-INFINITY, 0x7FFFFFFF};  // (they weigh nothing)
     uint32_t base = s_min, span = s_max - s_min;  // keys base .. base + span are left
@@ -687,8 +715,23 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
       for (int j0 = 0; j0 < n; j0 += kHeld * kThreads) {
         if (!one_round) load_held(j0), weigh();
 #pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-          if (q[u] && key[u] - base <= span) atomicAdd(&hist[(key[u] - base) >> shift], q[u]);
+        for (int u = 0; u < kHeld; ++u) {
+          if (j0 + u * kThreads >= n) break;  // (the workgroup's)
+          bool left = q[u] && key[u] - base <= span;
+          // logits that were 16-bit numbers have few values: equal ones are added together while a wave has
+          // several (64 additions to one place wait for each other)
+          for (u64 todo = __ballot(left); todo; todo = __ballot(left)) {
+            const int first = __ffsll((long long)todo) - 1;
+            const uint32_t k = lane_value(key[u], first);
+            const u64 same = __ballot(left && key[u] == k);
+            if (__popcll(same) < 4) {
+              if (left) atomicAdd(&hist[(key[u] - base) >> shift], q[u]);
+              break;
+            }
+            if (lane == first) atomicAdd(&hist[(k - base) >> shift], q[u] * (u64)__popcll(same));
+            left = left && key[u] != k;
+          }
+        }
       }
       __syncthreads();
       // digits from the largest: thread t has kDigits - 1 - 2 t and the one below
@@ -783,31 +826,51 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   }
   __syncthreads();
   // the chunk's first id whose kept cumulative mass exceeds the draw (its last kept id where the sums'
-  // roundings, or a uniform past 1, leave none)
+  // roundings, or a uniform past 1, leave none): first the 1024 ids that hold it, a wave's of the
+  // round, then the 64 of those, a wave each
   const u64 at = s_at;
   const int beg = s_digit * cl, end = min(p.vocab, beg + cl);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // from a value a wave: what lies before this wave's, and whether it holds `at`; adds all to `before`
+  const auto place = [&](u64 own, u64& before) {
+    __syncthreads();
+    if (lane == 0) red[wave] = own;
+    __syncthreads();
+    const u64 mine = red[lane & (kWaves - 1)], inc = row_scan_inc(mine);
+    const u64 upto = before + lane_value(inc - mine, wave);
+    before += lane_value(inc, kWaves - 1);
+    return upto;
+  };
   u64 before = 0;
   int last = -1;
+  if (tid == 0) s_min = 0xFFFFFFFFu;
   for (int i = beg; i < end && before <= at; i += kScan * kThreads) {
-    // kScan ids in a row a thread: one scan a round
+    const int id0 = i + wave * (64 * kScan) + lane;  // 64 a load
     float v[kScan];
-    u64 q[kScan], own = 0;
+    u64 own = 0;
 #pragma unroll
-    for (int u = 0; u < kScan; ++u) v[u] = L[min(i + tid * kScan + u, end - 1)];
-#pragma unroll
-    for (int u = 0; u < kScan; ++u) {
-      const int id = i + tid * kScan + u;
-      own += q[u] = id < end ? kept_mass(v[u], id, kChunkUnit) : 0;
-      if (q[u]) last = id;
-    }
-    u64 all;
-    u64 upto = before + block_scan(own, red, &all) - own;
+    for (int u = 0; u < kScan; ++u) v[u] = L[min(id0 + u * 64, end - 1)];
 #pragma unroll
     for (int u = 0; u < kScan; ++u) {
-      if (upto <= at && at < upto + q[u]) p.out[row] = i + tid * kScan + u;  // at most one token
-      upto += q[u];
+      const int id = id0 + u * 64;
+      if (!__ballot(v[u] >= cut.l)) continue;
+      const u64 q = id < end ? kept_mass(v[u], id, kChunkUnit) : 0;
+      own += q;
+      if (q) last = id;
     }
-    before += all;
+    own = lane_value(wave_scan_inc(own), 63);
+    const u64 upto = place(own, before);
+    if (lane == 0 && upto <= at && at < upto + own) s_min = (uint32_t)(id0), s_above = upto;
+  }
+  __syncthreads();
+  if (before > at) {  // (uniform)
+    static_assert(kScan == kWaves, "64 ids a wave");
+    const int id = (int)s_min + wave * 64 + lane;
+    const float v = L[min(id, end - 1)];
+    const u64 q = id < end ? kept_mass(v, id, kChunkUnit) : 0, inc = wave_scan_inc(q);
+    u64 from = s_above;
+    const u64 upto = place(lane_value(inc, 63), from);
+    if (upto + inc - q <= at && at < upto + inc) p.out[row] = id;  // one token
   }
   if (before <= at) {  // (uniform)
     if (last >= 0) atomicMax(&s_id, last);

@@ -430,8 +430,9 @@ IE_API int ie_qk_norm_rope_paged(ie_context* ctx, int n_seqs, const int* start_p
  * gets zeros.  Values at keys that a row does not see never reach it, infinities and NaN included.
  * d_q, d_out: [rows][n_q_heads][128] (bf16).  Softmax and sums in fp32; the weights are rounded to bf16
  * for their product with V.  Few rows over many keys are split over the keys by a rule on all the
- * lengths, on which the rounding depends.  workspace: ie_attn_window_workspace_size(rows,
- * n_q_heads) bytes for at least the batch's rows, contents of no account. */
+ * lengths, on which the rounding depends.  d_out may be d_q.  workspace:
+ * ie_attn_window_workspace_size(rows, n_q_heads) bytes for at least the batch's rows, contents of no account
+ * (the size never falls as rows grow). */
 IE_API size_t ie_attn_window_workspace_size(int rows, int n_q_heads);
 IE_API int ie_attn_window_paged(ie_context* ctx, int n_seqs, const int* start_pos,
                                 const int* n_new, int window, int n_sinks, int n_q_heads,

@@ -338,7 +338,8 @@ struct AttnWindowParams {
   int item_end[kMaxSeqs];                  // (row block, split) items up to and with the sequence's
   int splits[kMaxSeqs], part0[kMaxSeqs];   // key splits; first partial row
 };
-constexpr int kAttnWindowPartRows = 4096;
+constexpr int kAttnWindowPartRows = 4096;  // (row, split) partials at most
+constexpr int kAttnWindowMaxSplits = 64;
 size_t attn_window_workspace_bytes(int rows, int heads);
 int launch_attn_window(AttnWindowParams p, const SeqBatch& s, void* workspace, hipStream_t st);
 

@@ -472,8 +472,11 @@ __global__ __launch_bounds__(256) void attn_window_merge_kernel(AttnWindowParams
 
 }  // namespace
 
-// Partial rows (a row and split) that a workspace for `rows` rows holds.
-static int attn_window_part_rows(int rows) { return rows >= kAttnWindowPartRows ? 0 : kAttnWindowPartRows; }
+// Partial rows (a row and split) that a workspace for `rows` rows holds: every row's in 64 splits, up to
+// kAttnWindowPartRows.  It never falls with the rows: a workspace serves all smaller batches.
+static int attn_window_part_rows(int rows) {
+  return std::min(rows, kAttnWindowPartRows / kAttnWindowMaxSplits) * kAttnWindowMaxSplits;
+}
 
 size_t attn_window_workspace_bytes(int rows, int heads) {
   return (size_t)attn_window_part_rows(rows) * heads * (kHeadDim + 2) * sizeof(float);
@@ -513,7 +516,7 @@ Plan plan_of(const AttnWindowParams& p, const SeqBatch& s, int rows, int room) {
     }
     const double c1 = qi == 1 ? 1.12 : 1.63, c2 = qi == 1 ? 1.39 : 2.24;
     int tried = 0;
-    for (const int n : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64}) {
+    for (const int n : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, kAttnWindowMaxSplits}) {
       const int tps = (longest + n - 1) / n;
       if (n > longest || tps == tried) continue;
       tried = tps;

@@ -147,6 +147,27 @@ def test_append_without_norm_is_apply_rope(hip, ctx):
     assert torch.equal(out.transpose(0, 1), q)
 
 
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_append_one_norm_alone(hip, ctx, which):
+    say(f"append with a norm of the {which} heads alone")
+    g = gen(4)
+    n_pages, tables = make_tables(g, [150])
+    pool = make_pool(g, n_pages)
+    qkv = bf16(g, 70, 48 * D)
+    w = bf16(g, D, mean=1.0, std=0.2)
+    wq, wk = (w, None) if which == "q" else (None, w)
+    cos, sin = rope(150)
+    q = torch.empty(70, 32, D, dtype=torch.bfloat16, device="cuda")
+    append(hip, ctx, [80], [70], 32, qkv, wq, wk, cos, sin, q, pool, tables)
+    torch.cuda.synchronize()
+    x = qkv.view(70, 48, D)
+    pos = torch.arange(80, 150, device="cuda")
+    k = pool[tables[0, pos // PAGE].long(), LAYER, 0, :, pos % PAGE]
+    for got, heads, wt in ((q, x[:, :32], wq), (k, x[:, 32:40], wk)):
+        want, size = turned64(heads, wt, cos[pos], sin[pos])
+        assert ((got.double() - want).abs() <= want.abs() * 2**-8 + size * 2**-18).all()
+
+
 def test_append_bad_pages_are_not_written(hip, ctx):
     say("append with page ids outside the pool")
     g = gen(4)
@@ -252,6 +273,78 @@ def test_attend(hip, ctx, i):
     assert (out[rows:] == 7.0).all()
     want, tol = attend64(start, new, window, sinks, heads, q, pool, tables)
     check_attend(out[:rows], want, tol)
+
+
+def test_attend_workspace_of_a_larger_batch(hip, ctx):
+    """A workspace made for more rows holds the partials of fewer; a single token beside a chunk of more
+    than 4096 rows is split like one alone."""
+    say("attend: one workspace for a large and a small batch")
+    g = gen(21)
+    start, new = [3000, 100], [1, 4200]
+    n_pages, tables = make_tables(g, [a + b for a, b in zip(start, new)])
+    pool = make_pool(g, n_pages)
+    size = hip.lib.ie_attn_window_workspace_size(sum(new), 32)
+    ws = torch.full((size // 4 + 1024,), 7.0, device="cuda")
+    for st, n in ((start, new), (start[:1], [1])):
+        rows = sum(n)
+        q = bf16(g, rows, 32, D)
+        out = torch.empty_like(q)
+        hip.check(hip.lib.ie_attn_window_paged(
+            ctx.handle, len(n), ints(st), ints(n), 2500, 4, 32, ptr(q), ptr(pool), n_pages, ptr(tables),
+            tables.shape[1], LAYER, ptr(out), ptr(ws)))
+        torch.cuda.synchronize()
+        assert (ws[size // 4:] == 7.0).all()
+        want, tol = attend64(st, n, 2500, 4, 32, q, pool, tables)
+        check_attend(out, want, tol)
+
+
+@pytest.mark.parametrize("start,new,heads", [([6000, 20, 3], [1, 1, 1], 32), ([0, 900], [333, 65], 32),
+                                             ([0], [2100], 16), ([3000], [40], 64)])
+def test_attend_in_place(hip, ctx, start, new, heads):
+    say(f"attend into the queries' own buffer {start} {new} heads={heads}")
+    g = gen(heads)
+    n_pages, tables = make_tables(g, [a + b for a, b in zip(start, new)])
+    pool = make_pool(g, n_pages)
+    q = bf16(g, sum(new), heads, D)
+    out = torch.empty_like(q)
+    attend(hip, ctx, start, new, 700, 4, heads, q, pool, tables, out)
+    attend(hip, ctx, start, new, 700, 4, heads, q, pool, tables, q)
+    torch.cuda.synchronize()
+    assert torch.equal(q, out)
+
+
+def test_no_new_rows_is_no_work(hip, ctx):
+    say("batches without new rows")
+    g = gen(9)
+    n_pages, tables = make_tables(g, [100, 5])
+    pool = make_pool(g, n_pages)
+    before = pool.clone()
+    q = torch.full((2, 32, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = q.clone()
+    cos, sin = rope(128)
+    append(hip, ctx, [100, 5], [0, 0], 32, bf16(g, 1, 48 * D), None, None, cos, sin, q, pool, tables)
+    attend(hip, ctx, [100, 5], [0, 0], 10, 0, 32, q, pool, tables, out)
+    torch.cuda.synchronize()
+    assert (q == 7.0).all() and (out == 7.0).all() and torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("layer", [0, 31])
+def test_layers(hip, ctx, layer):
+    """The first and the last layer's planes of the pages, in pages far apart."""
+    say(f"append and attend, layer {layer}")
+    g = gen(layer)
+    pool = torch.full((300, LAYERS, 2, KVH, PAGE, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+    tables = torch.tensor([[299, 0], [1, 298]], dtype=torch.int32, device="cuda")
+    cos, sin = rope(128)
+    qkv = bf16(g, 170, 48 * D)
+    q, out = (torch.empty(170, 32, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    append(hip, ctx, [0, 0], [70, 100], 32, qkv, None, None, cos, sin, q, pool, tables, layer)
+    attend(hip, ctx, [0, 0], [70, 100], 30, 2, 32, q, pool, tables, out, layer=layer)
+    torch.cuda.synchronize()
+    want, tol = attend64([0, 0], [70, 100], 30, 2, 32, q, pool, tables, layer)
+    check_attend(out, want, tol)
+    pool[:, layer] = float("nan")
+    assert torch.isnan(pool).all()               # no other layer was written
 
 
 @pytest.mark.parametrize("start,new", [([900, 300, 5000], [1, 1, 1]), ([900, 0], [100, 700])])
@@ -622,6 +715,38 @@ def test_sample_many_draws_follow_the_distribution(hip, ctx):
     w = np.exp(l.double().cpu().numpy())
     w[[0, 2]] = 0
     assert (np.abs(got - n * w / w.sum()) <= 1).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(40, V), (33, 100003), (2, 2**21), (35, 2**18)])
+def test_sample_many_rows_and_large_vocabularies(hip, ctx, rows, vocab):
+    """32 rows and more are cut into fewer chunks; chunks of several rounds; the largest vocabulary."""
+    say(f"sample {rows} rows of {vocab}")
+    g = gen(rows)
+    logits = torch.empty(rows, vocab, device="cuda").normal_(0.0, 2.0, generator=g)
+    if rows % 2:
+        logits = logits.bfloat16().float()
+    settings = [SETTINGS[r % len(SETTINGS)] for r in range(rows)]
+    t, k, p, m = map(list, zip(*settings))
+    check_sample(hip, ctx, logits, t, k, p, m, torch.rand(rows, generator=g, device="cuda").tolist())
+
+
+def test_sample_rounds_of_small_and_large_cuts(hip, ctx):
+    """Rows at the border between the forms of the last step: 63, 64 and 65 tokens to choose from, ties
+    across it, and with each filter the one that decides."""
+    say("sample: borders of the listed tokens")
+    n, rows = 3000, []
+    for top in (62, 63, 64, 65, 66, 300):
+        l = np.full(n, -8.0, np.float32)
+        l[np.random.default_rng(top).permutation(n)[:top]] = np.linspace(0, 3, top, dtype=np.float32)
+        tie = l.copy()
+        tie[tie > -8] = 1.0
+        for row in (l, tie):
+            for k in (1, 40, 63, 64, 65, 200):
+                for p, m in ((1.0, 0.0), (0.6, 0.0), (1.0, 0.3), (0.9, 0.01)):
+                    rows.append((row, (0.9, k, p, m), 0.77))
+    logits = torch.from_numpy(np.stack([r[0] for r in rows])).cuda()
+    t, k, p, m = map(list, zip(*[r[1] for r in rows]))
+    check_sample(hip, ctx, logits, t, k, p, m, [r[2] for r in rows])
 
 
 # ------------------------------------------------------------------------------- together

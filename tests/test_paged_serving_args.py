@@ -106,6 +106,23 @@ def test_workspace_sizes(hip):
     assert lib.ie_sample_filtered_workspace_size(64, V) >= lib.ie_sample_filtered_workspace_size(1, V) > 0
 
 
+def test_workspaces_never_shrink(hip):
+    """A workspace for a size serves every smaller one."""
+    lib = hip.lib
+    rows = sorted({r + d for r in (1, 2, 16, 63, 64, 65, 1000, 4095, 4096, 8192, 100000, 2**24) for d in (0, 1)})
+    for heads in (16, 32, 64):
+        sizes = [lib.ie_attn_window_workspace_size(r, heads) for r in rows]
+        assert sizes == sorted(sizes) and sizes[0] > 0
+        # every split of every row that a launch may make
+        assert all(s >= min(64 * r, 4096) * heads * 130 * 4 for r, s in zip(rows, sizes))
+    pages = [1, 2, 63, 64, 65, 1000, 65535, 65536]
+    sizes = [lib.ie_kv_compact_workspace_size(n) for n in pages]
+    assert sizes == sorted(sizes)
+    for vocab in (1, 64, 65, 1000, V, V + 1, 2**21):
+        sizes = [lib.ie_sample_filtered_workspace_size(r, vocab) for r in range(1, 65)]
+        assert sizes == sorted(sizes) and sizes[0] > 0
+
+
 def test_window_attention_descriptors_stay_scalar(tmp_path):
     """The window attention's K and V tile descriptors are in scalar registers: one that the compiler took
     through a vector register would turn every load of a tile into a readfirstlane loop."""

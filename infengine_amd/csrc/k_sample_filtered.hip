@@ -817,12 +817,20 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   if (tid < 64) {
     const double own =
         tid < p.chunks ? R.kept[tid] + (double)listed_of[tid] * (1.0 / kUnit) : 0.0;
-    const double inc = wave_scan_inc(own), z = lane_value(inc, 63), u = p.uniform[row];
-    const double x = z * fmax(u, 0.0);  // (a NaN too: 0)
+    // added one after the other: sums that never fall, which a scan's, rounded in another order a lane,
+    // may do
+    double z = 0.0, before = 0.0;
+    for (int k = 0; k < p.chunks; ++k) {
+      if (tid == k) before = z;
+      z += lane_value(own, k);
+    }
+    const double u = p.uniform[row], x = z * fmax(u, 0.0);  // (a NaN too: 0)
     // (u >= 1, or a product rounded up: the last chunk that keeps anything)
-    const u64 more = __ballot(inc > x), some = __ballot(own > 0.0);
+    const u64 some = __ballot(own > 0.0), more = __ballot(before + own > x) & some;
     const int c = more ? __ffsll((long long)more) - 1 : some ? 63 - __clzll((long long)some) : 0;
-    if (lane == c) s_digit = c, s_at = (u64)fmin(fmax(x - (inc - own), 0.0) * kChunkUnit, 9e18), s_id = -1;
+    // (u >= 1: past all of its tokens, wherever the sums were rounded)
+    const double draw = u >= 1.0 ? 9e18 : fmin(fmax(x - before, 0.0) * kChunkUnit, 9e18);
+    if (tid == c) s_digit = c, s_at = (u64)draw, s_id = -1;
   }
   __syncthreads();
   // the chunk's first id whose kept cumulative mass exceeds the draw (its last kept id where the sums'

@@ -694,6 +694,19 @@ def test_sample_odd_rows(hip, ctx):
     assert nan_off == off
 
 
+@pytest.mark.parametrize("low", [15.0, 26.0, 28.0])
+def test_sample_uniform_of_one_draws_the_last(hip, ctx, low):
+    say(f"sample: a uniform of one, last tokens {low} nats down")
+    g = gen(1)
+    for rows in (30, 60):
+        logits = torch.empty(rows, 20000, device="cuda").normal_(0.0, 0.1, generator=g)
+        logits[:, -300:] = logits.max(1, keepdim=True).values - low
+        for p in (1.0, 0.9999999):
+            got = sample(hip, ctx, logits, None, None, [p] * rows, None, [1.0, 2.0, float("inf")] * (rows // 3))
+            assert set(got) == {19999} if p == 1 else min(got) > 19000, (rows, p, [
+                (i, x) for i, x in enumerate(got) if x != 19999][:6])
+
+
 def test_sample_settings_off(hip, ctx):
     """NULL settings are off; a vocabulary of equal logits gives floor(u x vocab)."""
     say("sample: settings off")

@@ -11,7 +11,7 @@
 // Greedy rows (T not > 0, min_p > 1) are top_k = 1.  Weights are computed in fp64 and added in 64-bit
 // fixed point within a chunk of the row (exact, free of order), the chunks' sums in fp64 in
 // order: a draw next to a border of the distribution falls as it does in 64 bits.  Tokens below
-// exp(-30) of the largest weigh nothing.
+// 2^-46 of the largest (some: 2^-43) round to no unit and weigh nothing.
 //
 // A row is cut into 8 or 16 chunks, a workgroup each, over three launches:
 //   hist    the chunk's max, and its tokens binned by B(l) = floor(8 l / T), which is the same scale
@@ -493,7 +493,9 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
   double low = 0.0;
   if (summed) {
     const float cm = R.pmax[c];
-    const double scale = cm > -INFINITY ? weight(cm) * (1.0 / kChunkUnit) : 0.0;
+    // (a chunk whose largest token rounds to no unit has none that a draw could find)
+    const double top = cm > -INFINITY ? weight(cm) : 0.0;
+    const double scale = in_units(top, kChunkUnit) ? top * (1.0 / kChunkUnit) : 0.0;
     if (scale > 0.0) {
       if (!cuts) {
         low = (double)R.total[c] * scale;

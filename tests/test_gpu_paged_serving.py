@@ -694,6 +694,20 @@ def test_sample_odd_rows(hip, ctx):
     assert nan_off == off
 
 
+def test_sample_chunk_that_weighs_next_to_nothing(hip, ctx):
+    """A first chunk about 32 nats below the largest logit, and a draw of zero: a token all the same."""
+    say("sample: a first chunk of next to no weight")
+    depths = np.arange(29.0, 34.0, 0.05, dtype=np.float32)
+    logits = np.full((depths.size, 1000), -100.0, np.float32)
+    logits[:, :60] = -depths[:, None]
+    logits[:, 500] = 0.0
+    for rows in (31, depths.size):
+        for top_p in (1.0, 0.999999):
+            got = sample(hip, ctx, torch.from_numpy(logits[:rows].copy()).cuda(), [1.0] * rows, [0] * rows,
+                         [top_p] * rows, [0.0] * rows, [0.0] * rows)
+            assert set(got) <= {0, 500}, got
+
+
 @pytest.mark.parametrize("low", [15.0, 26.0, 28.0])
 def test_sample_uniform_of_one_draws_the_last(hip, ctx, low):
     say(f"sample: a uniform of one, last tokens {low} nats down")

@@ -152,16 +152,29 @@ __device__ __forceinline__ u64 in_units(double w, double unit) {
 }
 
 // The token's bin below that of `mx`, kBins for those that weigh nothing (further below, -inf, NaN).
-// Non-decreasing in falling l, and the same steps whatever mx: B(l) = floor(l x scale) in fp32, whose
-// rounding is monotone, and whose differences below kBins are exact at any size of l.  scale = 8 / T,
-// held finite: below that T bins are wider than 1/8 nat, and tokens past kBins only weigh less.
+// Non-decreasing in falling l, and the same steps whatever mx: B(l) = floor(l x scale) of the exact product,
+// held as the floor of its fp32 rounding plus, where that is a whole number, the floor of what the rounding
+// left out (8 l / T passes 24 bits for small T: with the rounded product alone neighbouring logits come to
+// lie many bins off); differences below kBins are exact at any size of l.  scale = 8 / T, held finite: below
+// that T bins are wider than 1/8 nat, and tokens past kBins only weigh less.
 struct Binner {
-  float mx, scale, top;
-  __device__ Binner(float m, double inv_t)
-      : mx(m), scale((float)fmin(8.0 * inv_t, 3.4e38)), top(floorf(m * scale)) {}
+  float mx, scale, top, top_rest;
+  __device__ Binner(float m, double inv_t) : mx(m), scale((float)fmin(8.0 * inv_t, 3.4e38)) { parts(m, top, top_rest); }
+  __device__ __forceinline__ void parts(float l, float& whole, float& rest) const {
+    const float x = l * scale;
+    whole = floorf(x);
+    rest = whole == x ? floorf(fmaf(l, scale, -x)) : 0.f;
+  }
   __device__ __forceinline__ int operator()(float l) const {
-    const float d = top - floorf(l * scale);
+    float whole, rest;
+    parts(l, whole, rest);
+    const float d = (top - whole) + (top_rest - rest);
     return l == mx ? 0 : l > -INFINITY && d < (float)kBins ? max((int)d, 0) : kBins;
+  }
+  // No product below it is of a bin up to `needed` (NaN: every one may be).
+  __device__ __forceinline__ float least(int needed) const {
+    const float b = (top - (float)needed) + top_rest;
+    return b - fabsf(b) * 0x1p-22f;  // (its own roundings)
   }
 };
 
@@ -514,9 +527,9 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
   }
   Listed* list = row_list(R, c, cl);
   const int sum_bins = summed ? 0 : s.m ? min(cut.lo, s.m_bins) : cut.lo;  // bins summed token by token
-  // no bin past `needed` matters: floor(l x scale) >= top - needed is l x scale >= it
+  // no bin past `needed` matters
   const int needed = max(max(sum_bins - 1, cut.k_bin), cut.p_hi);
-  const float least = bin.top - (float)needed;
+  const float least = bin.least(needed);
   u64 sum = 0;
   int listed = 0;
   // (beg and end are the workgroup's: every thread runs every round and its barriers)
@@ -529,7 +542,7 @@ __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleParams
     for (int u = 0; u < kRound; ++u) {
       place[u] = 0;
       // (most rows need few tokens: one product and comparison for the others)
-      if (!__ballot(v[u] * bin.scale >= least)) continue;
+      if (!__ballot(!(v[u] * bin.scale < least))) continue;
       const int b = bin(v[u]);
       if (b < sum_bins && b < kBins) {
         const double w = weight(v[u]);

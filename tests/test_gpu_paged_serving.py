@@ -694,6 +694,27 @@ def test_sample_odd_rows(hip, ctx):
     assert nan_off == off
 
 
+@pytest.mark.parametrize("base,t", [(30.0, 1e-6), (100.0, 2e-7), (-30.0, 1e-6), (1e7, 0.7), (-3e5, 0.01),
+                                    (1e6, 0.3), (1e10, 900.0)])
+def test_sample_logits_far_from_zero(hip, ctx, base, t):
+    """Logits of neighbouring fp32 values, some nats apart at their temperature: 8 l / T is far past the
+    24 bits of an fp32 product there."""
+    say(f"sample: logits next to {base} at temperature {t}")
+    rng = np.random.default_rng(3)
+    steps = rng.integers(0, 12, 4000)
+    ulp = float(np.spacing(np.float32(abs(base))))
+    row = (base - steps * ulp).astype(np.float32)
+    row[rng.permutation(4000)[:3900]] = np.float32(base - 3000 * ulp - 4000 * t)   # nothing of those
+    rows = []
+    for share in np.exp(-np.arange(0.3, 8.0, 0.7) * ulp / t):
+        rows += [(row, (t, 0, 1.0, float(share)), u) for u in (0.05, 0.5, 0.95, 0.9999)]
+    for top_p in (0.2, 0.5, 0.9, 0.99, 0.99999):
+        rows += [(row, (t, k, top_p, 0.0), u) for u in (0.05, 0.5, 0.95, 0.9999) for k in (0, 30, 70, 90)]
+    logits = torch.from_numpy(np.stack([r[0] for r in rows])).cuda()
+    tt, k, p, m = map(list, zip(*[r[1] for r in rows]))
+    check_sample(hip, ctx, logits, tt, k, p, m, [r[2] for r in rows])
+
+
 def test_sample_chunk_that_weighs_next_to_nothing(hip, ctx):
     """A first chunk about 32 nats below the largest logit, and a draw of zero: a token all the same."""
     say("sample: a first chunk of next to no weight")
@@ -719,6 +740,16 @@ def test_sample_uniform_of_one_draws_the_last(hip, ctx, low):
             got = sample(hip, ctx, logits, None, None, [p] * rows, None, [1.0, 2.0, float("inf")] * (rows // 3))
             assert set(got) == {19999} if p == 1 else min(got) > 19000, (rows, p, [
                 (i, x) for i, x in enumerate(got) if x != 19999][:6])
+
+
+def test_sample_infinite_logits_and_temperature(hip, ctx):
+    say("sample: infinite logits at an infinite temperature")
+    logits = torch.zeros(2, 3000, device="cuda")
+    logits[:, [700, 2100]] = float("inf")
+    logits[:, 5] = -float("inf")
+    for k, p, m in ((0, 1.0, 0.0), (2, 1.0, 0.0), (5, 0.9, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.5), (1000, 0.9, 0.5)):
+        got = sample(hip, ctx, logits, [float("inf")] * 2, [k] * 2, [p] * 2, [m] * 2, [0.1, 0.7])
+        assert got == [700, 2100], (k, p, m, got)
 
 
 def test_sample_settings_off(hip, ctx):

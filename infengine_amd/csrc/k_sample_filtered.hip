@@ -36,6 +36,7 @@ typedef unsigned long long u64;
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kChunks = 16, kBins = 256;    // (at most 16 chunks)
 constexpr int kRound = 8;                   // logits a thread and round
+constexpr int kGroup = 4;                   // weights a thread computes together
 constexpr int kSmall = 64;                  // tokens listed whole, one a lane of the finish
 constexpr double kUnit = 4398046511104.0;   // 2^42: masses of listed tokens (2^21 fit 63 bits)
 constexpr double kChunkUnit = 35184372088832.0;  // 2^45: of a chunk's tokens (2^18 fit 63 bits)
@@ -100,7 +101,7 @@ __device__ __forceinline__ Setting setting(const SampleParams& p, int row) {
   s.m_bins = s.m ? (int)fminf(-8.0f * __logf(mp), (float)kBins) + 2 : 0;
   // the tokens past d nats below the largest weigh at most vocab exp(-d), which is less than the share
   // left out, (1 - top_p) of at least 1, from here on
-  s.p_bins = s.p ? (int)fminf(8.0f * (__logf((float)p.vocab) - __logf(fmaxf(1.0f - s.top_p, 1e-7f))), (float)kBins - 3) + 2 : 0;
+  s.p_bins = s.p ? (int)fminf(8.0f * (__logf((float)p.vocab) - __logf(1.0f - s.top_p)), (float)kBins - 3) + 2 : 0;
   return s;
 }
 
@@ -144,6 +145,31 @@ struct Weigher {
     const int n = (int)__double_as_longlong(t);
     const u64 w = (u64)__double_as_longlong(y * powers[n & 63]) + ((u64)(uint32_t)(n >> 6) << 52);
     return l == fmx ? 1.0 : z > -33.0 * 92.33248261893583 ? __longlong_as_double((long long)w) : 0.0;
+  }
+  // The same for N tokens whose weights are only counted in whole units: without a branch, so that their steps
+  // overlap (one token at a time took 276 cycles a wave's 64).  What weighs nothing here weighs less than
+  // half a unit there.
+  template <int N>
+  __device__ __forceinline__ void many(const float (&l)[N], double (&w)[N]) const {
+    constexpr double c1 = 0.010830424696249145, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4,
+                     c5 = c4 * c1 / 5, whole = 6755399441055744.0;
+    if (fmx == INFINITY) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) w[u] = l[u] == fmx ? 1.0 : 0.0;
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const double z = fmax(((double)l[u] - mx) * scale, -3100.0);  // (33.6 nats, and for NaN)
+      const double t = z + whole, f = z - (t - whole);
+      const int n = (int)__double_as_longlong(t);
+      double y = fma(f, c5, c4);
+      y = fma(y, f, c3);
+      y = fma(y, f, c2);
+      y = fma(y, f, c1);
+      y = fma(y, f, 1.0) * powers[n & 63];
+      w[u] = __hiloint2double(__double2hiint(y) + ((n & ~63) << 14), __double2loint(y));
+    }
   }
 };
 // w in whole units (2^42 or 2^45) for 0 <= w <= 1.
@@ -310,7 +336,6 @@ __global__ __launch_bounds__(kThreads, 8) void sample_hist_kernel(SampleParams p
   mx = wave_max(redf[lane & (kWaves - 1)]);
   if (tid == 0) R.pmax[c] = mx;
   const Weigher weight(powers, mx, s.inv_t);
-  const bool one_round = end - beg <= kRound * kThreads;
   if (!s.top_k && !s.p && s.m) return;
   u64 sum = 0;
   if (mx > -INFINITY) {
@@ -339,21 +364,37 @@ __global__ __launch_bounds__(kThreads, 8) void sample_hist_kernel(SampleParams p
       last = s_bin;
     }
     bool counted = false;  // the thread's largest token, once
-    for (int i = beg; i < end; i += kRound * kThreads) {
-      if (!one_round) load_round(L, i, end, v);
+    // the last round first: it is still held
+    const int rounds = (end - beg + kRound * kThreads - 1) / (kRound * kThreads);
+    for (int k = rounds - 1; k >= 0; --k) {
+      if (k < rounds - 1) load_round(L, beg + k * kRound * kThreads, end, v);
+      if (s.top_k) {
 #pragma unroll
-      for (int u = 0; u < kRound; ++u) {
-        const int b = bin(v[u]);
-        if (s.top_k) {
+        for (int u = 0; u < kRound; ++u) {
+          const int b = bin(v[u]);
           if (b > last) continue;
           const bool again = !counted && v[u] == own_max;
           counted |= again;
           if (!again) atomicAdd(&count[copy + b], 1u);
           if (s.p) atomicAdd(&mass[copy + b], in_units(weight(v[u]), kChunkUnit));
-        } else {
-          const u64 q = in_units(weight(v[u]), kChunkUnit);
-          sum += q;
-          if (b <= last) atomicAdd(&mass[copy + b], q);
+        }
+      } else {
+#pragma unroll
+        for (int u0 = 0; u0 < kRound; u0 += kGroup) {
+          float l[kGroup];
+          double w[kGroup];
+#pragma unroll
+          for (int u = 0; u < kGroup; ++u) l[u] = v[u0 + u];
+          weight.many(l, w);
+#pragma unroll
+          for (int u = 0; u < kGroup; ++u) {
+            const u64 q = in_units(w[u], kChunkUnit);
+            sum += q;
+            if (s.p) {
+              const int b = bin(l[u]);
+              if (b <= last) atomicAdd(&mass[copy + b], q);
+            }
+          }
         }
       }
     }
@@ -595,10 +636,10 @@ constexpr int kHeld = 4;          // listed tokens a thread holds
 constexpr int kScan = 16;         // logits a thread and round of the last scan
 
 // A row whose tokens are all listed, at most one a lane: one wave, no barrier.
-__device__ __forceinline__ int finish_small(const SampleParams& p, const Setting& s, Row& R, int row, int cl,
-                                            const Weigher& weight, u64* by_rank) {
+__device__ __forceinline__ int finish_small(const SampleParams& p, const Setting& s, Row& R, int own_n, double uniform,
+                                            int cl, const Weigher& weight, u64* by_rank) {
   const int lane = threadIdx.x & 63;
-  const int own_n = lane < p.chunks ? R.n_listed[lane] : 0, upto = wave_scan_inc(own_n);
+  const int upto = wave_scan_inc(own_n);
   const int n = lane_value(upto, 63);
   int c = 0, before = 0;
   for (int k = 0; k < p.chunks - 1; ++k) {
@@ -635,7 +676,7 @@ __device__ __forceinline__ int finish_small(const SampleParams& p, const Setting
   keep = keep || (lane < n && rank == 0);
   if (!keep) q = 0;
   const u64 inc = wave_scan_inc(q), z = lane_value(inc, 63);
-  const double x = (double)z * fmax((double)p.uniform[row], 0.0);  // (a NaN too: 0)
+  const double x = (double)z * fmax(uniform, 0.0);  // (a NaN too: 0)
   const u64 at = x < (double)z ? min((u64)x, z - 1) : z - 1;
   return lane_value(t.id, __ffsll((long long)__ballot(inc > at)) - 1);
 }
@@ -652,6 +693,11 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   Row& R = row_state(ws, row, p.vocab);
   const float* L = p.logits + (size_t)row * p.vocab;
+  // (what the row's state holds in one go: a load after the other is a wait each)
+  const int own_listed = lane < p.chunks ? R.n_listed[lane] : 0;
+  const double own_kept = lane < p.chunks ? R.kept[lane] : 0.0;
+  const double u_row = p.uniform[row];
+  const int small = R.small, p_lo = R.p_lo, p_hi = R.p_hi, k_bin = R.k_bin;
   const Setting s = setting(p, row);
   const float mx = row_max(R, p.chunks);
   if (!(mx > -INFINITY)) {
@@ -662,15 +708,14 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   const Binner bin(mx, s.inv_t);
   const Weigher weight(powers, mx, s.inv_t);
   const int cl = chunk_len(p.vocab, p.chunks);
-  if (R.small >= 0) {
+  if (small >= 0) {
     if (tid >= 64) return;
-    const int token = finish_small(p, s, R, row, cl, weight, hist);
+    const int token = finish_small(p, s, R, own_listed, u_row, cl, weight, hist);
     if (tid == 0) p.out[row] = token;
     return;
   }
-  const int p_lo = R.p_lo, p_hi = R.p_hi, k_bin = R.k_bin;
   if (tid < 64) {
-    const int inc = wave_scan_inc(tid < p.chunks ? R.n_listed[tid] : 0);
+    const int inc = wave_scan_inc(own_listed);
     if (tid < kChunks) {
       offset[tid + 1] = inc;
       listed_of[tid] = 0;
@@ -824,14 +869,21 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     if (!one_round) load_held(j0);
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) {
+      if (j0 + u * kThreads >= n) break;  // (the workgroup's)
       const u64 q = held[u].id >= 0 ? kept_mass(held[u].l, held[u].id, kUnit) : 0;
-      if (q) atomicAdd(&listed_of[chunk_of(j0 + u * kThreads + tid)], q);
+      if (!__ballot(q != 0)) continue;
+      // (the list goes chunk by chunk, so a wave has one or two; 64 additions to one place wait for each other)
+      const int own = chunk_of(min(j0 + u * kThreads + tid, n - 1)), to = lane_value(own, 63);
+      for (int c = lane_value(own, 0); c <= to; ++c) {
+        const u64 all = lane_value(wave_scan_inc(own == c ? q : 0), 63);
+        if (lane == 0) atomicAdd(&listed_of[c], all);
+      }
     }
   }
   __syncthreads();
   if (tid < 64) {
     const double own =
-        tid < p.chunks ? R.kept[tid] + (double)listed_of[tid] * (1.0 / kUnit) : 0.0;
+        tid < p.chunks ? own_kept + (double)listed_of[tid] * (1.0 / kUnit) : 0.0;
     // added one after the other: sums that never fall, which a scan's, rounded in another order a lane,
     // may do
     double z = 0.0, before = 0.0;
@@ -839,7 +891,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
       if (tid == k) before = z;
       z += lane_value(own, k);
     }
-    const double u = p.uniform[row], x = z * fmax(u, 0.0);  // (a NaN too: 0)
+    const double u = u_row, x = z * fmax(u, 0.0);  // (a NaN too: 0)
     // (u >= 1, or a product rounded up: the last chunk that keeps anything)
     const u64 some = __ballot(own > 0.0), more = __ballot(before + own > x) & some;
     const int c = more ? __ffsll((long long)more) - 1 : some ? 63 - __clzll((long long)some) : 0;
@@ -864,6 +916,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     before += lane_value(inc, kWaves - 1);
     return upto;
   };
+  const bool dense = !s.m && cut.l == -INFINITY;  // (nothing is dropped)
   u64 before = 0;
   int last = -1;
   if (tid == 0) s_min = 0xFFFFFFFFu;
@@ -873,13 +926,31 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     u64 own = 0;
 #pragma unroll
     for (int u = 0; u < kScan; ++u) v[u] = L[min(id0 + u * 64, end - 1)];
+    if (dense) {
 #pragma unroll
-    for (int u = 0; u < kScan; ++u) {
-      const int id = id0 + u * 64;
-      if (!__ballot(v[u] >= cut.l)) continue;
-      const u64 q = id < end ? kept_mass(v[u], id, kChunkUnit) : 0;
-      own += q;
-      if (q) last = id;
+      for (int u0 = 0; u0 < kScan; u0 += kGroup) {
+        float l[kGroup];
+        double w[kGroup];
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) l[u] = v[u0 + u];
+        weight.many(l, w);
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+          const int id = id0 + (u0 + u) * 64;
+          const u64 q = id < end ? in_units(w[u], kChunkUnit) : 0;
+          own += q;
+          if (q) last = id;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kScan; ++u) {
+        const int id = id0 + u * 64;
+        if (!__ballot(v[u] >= cut.l)) continue;
+        const u64 q = id < end ? kept_mass(v[u], id, kChunkUnit) : 0;
+        own += q;
+        if (q) last = id;
+      }
     }
     own = lane_value(wave_scan_inc(own), 63);
     const u64 upto = place(own, before);

@@ -8,8 +8,8 @@
 // A workgroup of 4 waves takes one kv head and a block of query columns, 16 or 32 a wave, a column
 // being a (row, q head of the kv head's group): consecutive columns are the group's heads, then the
 // next row, so that a single token of a 4-head group fills 4 of a wave's 16 columns and a chunk fills
-// all of them, whatever the group.  It walks the 64-key tiles that the block's rows see (a tile is a page: the sink tiles, then the
-// window's), each staged once in LDS for all its waves.  Per tile and wave, with
+// all of them, whatever the group.  It walks the 64-key tiles that the block's rows see (a tile is a page:
+// the sink tiles, then the window's), each staged once in LDS for all its waves.  Per tile and wave, with
 // v_mfma_f32_16x16x32_bf16:
 //   S^T[key][col] = K . Q^T       (A = K rows from LDS, B = Q fragments in registers)
 //   online softmax per column     (running max and sum in fp32)
@@ -21,6 +21,13 @@
 //
 // Few columns over many keys: the tiles are cut into splits, a workgroup each, whose (o, m, l) go to
 // the caller's workspace in fp32 and are combined by a second kernel.
+//
+// Measured (32 q heads): one token over 600 keys 9.6 us (6.0 and 4.0 for the merge: two launches' starts, one tile
+// of work); one token of 16 sequences over 4096 keys 47.5, of which 43 read their 268 MB at 6.2 TB/s; 8192 rows over
+// 4096 keys each 598, 0.93 PF: the MFMAs are busy 45% of the cycles and the vector units 60% (exponents, maxima,
+// rescales, packing), which two waves a SIMD overlap in part; 6 sequences of up to 333 rows over 1500 keys 72: 328
+// workgroups, so that 72 CUs hold two and set the time (cut in three over the keys the merge's 20 MB of partials a
+// split take what that gains: 75).
 #include <algorithm>
 
 #include "ie_kernels.h"

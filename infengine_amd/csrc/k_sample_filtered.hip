@@ -25,6 +25,13 @@
 //           masses, the chunk that holds the draw, its token by a scan in id order
 // The bins are 1/8 of a nat wide: of 128256 N(0, 2) logits at T = 1 at most 3200 are listed.  The list
 // has room for every token (flatter rows list more and take longer).
+//
+// What it takes, us by kernel for a row of 128256: top-k 50 hist 5.4, gather 7.8, finish 5.6; top-p 0.9 6.3,
+// 10.9, 17.4; min-p 3.1, 5.2, 9.2; no filter 5.4, 3.3, 9.1; for 64 rows 12.9, 12.2, 5.3; 18.0, 19.2, 20.0;
+// 5.8, 13.4, 11.3; 14.0, 4.0, 9.7.  One row is bound by the waits of three launches for each other's results
+// (a launch that only reads the row's state takes 3-4); 64 rows by the weights' fp64 steps and the histogram's
+// LDS additions in the first two launches, and by the barriers of the selects in the last (2000 cycles a
+// digit beside 100 of work), which one CU a row runs.
 #include "ie_kernels.h"
 
 namespace ie {
@@ -60,9 +67,10 @@ struct Listed {
   int id;
 };
 
-// Chunks a row: 16 for few rows, where a chunk's latency counts; 8 from 32 rows on, whose 1024-thread
-// workgroups then run in one turn of the chip.
-__host__ __device__ __forceinline__ int row_chunks(int rows) { return rows < 32 ? kChunks : kChunks / 2; }
+// Chunks a row: 16 while all the chunks' 1024-thread workgroups run at once, two a CU, 8 past that.  Mixed
+// settings, us in 8 and in 16 chunks: 16 rows 48.2 and 41.7, 32 rows 49.7 and 48.8, 48 rows 58.4 and 59.5, 64
+// rows 61.1 and 68.7.
+__host__ __device__ __forceinline__ int row_chunks(int rows) { return rows <= 32 ? kChunks : kChunks / 2; }
 __host__ __device__ __forceinline__ int chunk_len(int vocab, int chunks) { return (vocab + chunks - 1) / chunks; }
 __host__ __device__ __forceinline__ size_t row_bytes(int vocab) {
   return ((sizeof(Row) + 255) & ~(size_t)255) +

@@ -777,7 +777,7 @@ def test_sample_many_draws_follow_the_distribution(hip, ctx):
 
 @pytest.mark.parametrize("rows,vocab", [(40, V), (33, 100003), (2, 2**21), (35, 2**18)])
 def test_sample_many_rows_and_large_vocabularies(hip, ctx, rows, vocab):
-    """32 rows and more are cut into fewer chunks; chunks of several rounds; the largest vocabulary."""
+    """Past 32 rows each is cut into fewer chunks; chunks of several rounds; the largest vocabulary."""
     say(f"sample {rows} rows of {vocab}")
     g = gen(rows)
     logits = torch.empty(rows, vocab, device="cuda").normal_(0.0, 2.0, generator=g)

@@ -30,8 +30,9 @@
 // 10.9, 17.4; min-p 3.1, 5.2, 9.2; no filter 5.4, 3.3, 9.1; for 64 rows 12.9, 12.2, 5.3; 18.0, 19.2, 20.0;
 // 5.8, 13.4, 11.3; 14.0, 4.0, 9.7.  One row is bound by the waits of three launches for each other's results
 // (a launch that only reads the row's state takes 3-4); 64 rows by the weights' fp64 steps and the histogram's
-// LDS additions in the first two launches, and by the barriers of the selects in the last (2000 cycles a
-// digit beside 100 of work), which one CU a row runs.
+// LDS additions in the first two launches, and in the last, which one CU a row runs, by the barriers of the
+// selects (top-p 0.9, of 40000 cycles: 3200 for the smallest and largest key, 3400-4000 a digit, two of them,
+// 4000 for the id).
 #include "ie_kernels.h"
 
 namespace ie {

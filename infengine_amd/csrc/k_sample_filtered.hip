@@ -46,8 +46,8 @@ constexpr int kChunks = 16, kBins = 256;    // (at most 16 chunks)
 constexpr int kRound = 8;                   // logits a thread and round
 constexpr int kGroup = 4;                   // weights a thread computes together
 constexpr int kSmall = 64;                  // tokens listed whole, one a lane of the finish
-constexpr double kUnit = 4398046511104.0;   // 2^42: masses of listed tokens (2^21 fit 63 bits)
-constexpr double kChunkUnit = 35184372088832.0;  // 2^45: of a chunk's tokens (2^18 fit 63 bits)
+constexpr double kUnit = 4398046511104.0;   // 2^42: masses of listed tokens (2^21 of them: 2^63)
+constexpr double kChunkUnit = 35184372088832.0;  // 2^45: of a chunk's tokens (2^18 of them: 2^63)
 static_assert(kSampleMaxVocab <= 1 << 21 && kSampleMaxVocab / (kChunks / 2) <= 1 << 18, "sums in 64 bits");
 
 // A row's state in the workspace; the listed tokens follow it, chunk by chunk.
@@ -904,9 +904,9 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     // (u >= 1, or a product rounded up: the last chunk that keeps anything)
     const u64 some = __ballot(own > 0.0), more = __ballot(before + own > x) & some;
     const int c = more ? __ffsll((long long)more) - 1 : some ? 63 - __clzll((long long)some) : 0;
-    // (u >= 1: past all of its tokens, wherever the sums were rounded)
-    const double draw = u >= 1.0 ? 9e18 : fmin(fmax(x - before, 0.0) * kChunkUnit, 9e18);
-    if (tid == c) s_digit = c, s_at = (u64)draw, s_id = -1;
+    // (a chunk's sum reaches 2^63; u >= 1: past all of its tokens, wherever the sums were rounded)
+    const u64 draw = u >= 1.0 ? ~0ull : (u64)fmin(fmax(x - before, 0.0) * kChunkUnit, 1.8e19);
+    if (tid == c) s_digit = c, s_at = draw, s_id = -1;
   }
   __syncthreads();
   // the chunk's first id whose kept cumulative mass exceeds the draw (its last kept id where the sums'

@@ -775,7 +775,16 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     kmin = wave_min_u32(kmin), kmax = ~wave_min_u32(~kmax);
     if (lane == 0 && kmin <= kmax) atomicMin(&s_min, kmin), atomicMax(&s_max, kmax);
     __syncthreads();
-    if (s_min > s_max) return Cut{-INFINITY, 0x7FFFFFFF};  // (they weigh nothing)
+    if (s_min > s_max) {
+      // masses alone can all be 0 (tokens below 2^-43 in the bins of top_p's cut): none of them stays, and
+      // of the rest the bins above p_lo; the largest logit of bin p_lo or past it, by halving
+      uint32_t a = logit_key(-INFINITY), b = logit_key(mx);
+      while (b - a > 1) {
+        const uint32_t mid = a + (b - a) / 2;
+        (bin(key_logit(mid)) >= p_lo ? a : b) = mid;
+      }
+      return Cut{key_logit(a), 0};
+    }
     uint32_t base = s_min, span = s_max - s_min;  // keys base .. base + span are left
     while (span) {
       const int shift = max(0, 32 - __clz(span) - 11);

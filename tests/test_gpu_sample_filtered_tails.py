@@ -42,3 +42,21 @@ def test_flat_rows_of_the_largest_vocabulary(hip, ctx, vocab, how):
     got = sample(hip, ctx, logits, t, None, p, m, ENDS)
     want = flat_tokens(kept)
     assert got == want, [(u, g, w) for u, g, w in zip(ENDS, got, want) if g != w][:8]
+
+
+def test_top_k_holds_among_tokens_that_weigh_next_to_nothing(hip, ctx):
+    """One token, 2^20 of 2^-43.2 of its weight and as many of 2^-45; top_k ends among the last ones, top_p
+    before them.  A uniform of zero draws the first kept id: the large token (the others may count as
+    nothing) or one that both filters keep, never one of the last."""
+    say("sample: top-k and top-p among tokens of next to no weight")
+    logits = torch.full((2, MOST), -29.95, device="cuda")
+    logits[:, MOST // 2:] = -31.2
+    logits[:, MOST - 1] = 0.0
+    w = np.exp(np.float64(np.float32(-29.95)))
+    top_p = 1 - 2**-24
+    n_light = int(np.ceil((top_p * (1 + w * 2**20) - 1) / w))     # of the 2^20, those within top_p
+    assert 0 < n_light < 2**20
+    for k, p in ((2**20 + 1001, top_p), (0, top_p)):
+        got = sample(hip, ctx, logits, None, [k] * 2, [p] * 2, None, [0.0, 0.5])
+        assert got[0] < n_light or got[0] == MOST - 1, (k, p, got)
+        assert got[1] == MOST - 1

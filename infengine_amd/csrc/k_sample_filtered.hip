@@ -644,6 +644,13 @@ constexpr int kDigits = 2048;
 constexpr int kHeld = 4;          // listed tokens a thread holds
 constexpr int kScan = 16;         // logits a thread and round of the last scan
 
+// Memory accesses of a wave's lanes keep their order across it.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A row whose tokens are all listed, at most one a lane: one wave, no barrier.
 __device__ __forceinline__ int finish_small(const SampleParams& p, const Setting& s, Row& R, int own_n, double uniform,
                                             int cl, const Weigher& weight, u64* by_rank) {
@@ -669,15 +676,15 @@ __device__ __forceinline__ int finish_small(const SampleParams& p, const Setting
   bool keep = in_k && (!s.m || w >= (double)s.min_p);
   if (s.p) {
     // the masses in the order: those before a token short of the share of them all
-    // (one wave: its LDS accesses are in order; the fences hold the compiler to it)
+    // (one wave: the hardware does its LDS accesses in order; the fences hold the compiler to it)
     by_rank[lane] = 0;
-    __builtin_amdgcn_wave_barrier();
+    wave_fence();
     if (lane < n) by_rank[rank] = q;
-    __builtin_amdgcn_wave_barrier();
+    wave_fence();
     const u64 sorted = by_rank[lane], inc = wave_scan_inc(sorted), z = lane_value(inc, 63);
-    __builtin_amdgcn_wave_barrier();
+    wave_fence();
     by_rank[lane] = inc - sorted;
-    __builtin_amdgcn_wave_barrier();
+    wave_fence();
     const double share = ceil((double)z * (double)s.top_p);
     const u64 want = share < 1.0 ? 1 : share > (double)z ? z : (u64)share;
     keep = keep && by_rank[min(rank, 63)] < want;

@@ -316,8 +316,8 @@ struct QkNormRopeParams {
   uint16_t* k;             // the layer's head-0 K / V planes of page 0 (pages kPageElems apart)
   uint16_t* v;
   const int* block_tables;
-  int table_stride, n_pages, heads, n_seqs, rows;
-  int start[kMaxSeqs], row_end[kMaxSeqs];  // (set by the launcher, as n_seqs and rows)
+  int table_stride, n_pages, heads, n_seqs;
+  int start[kMaxSeqs], row_end[kMaxSeqs];  // (set by the launcher, as n_seqs)
 };
 int launch_qk_norm_rope(QkNormRopeParams p, const SeqBatch& s, hipStream_t st);
 

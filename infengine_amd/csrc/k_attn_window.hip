@@ -505,7 +505,7 @@ struct Plan {
 // splits; 200 rows over 16384 keys 296 unsplit, 104 in 4 (16 columns), 89 in 8 (32); 16 tokens over 4096 keys
 // 98 and 48; 6 x 333 rows over 1500 keys 71 unsplit, 75 in 3; 2 x 1000 over 4096 keys 172 and 151 unsplit,
 // 130 in 3 (32 columns).
-Plan plan_of(const AttnWindowParams& p, const SeqBatch& s, int rows, int room) {
+Plan plan_of(const AttnWindowParams& p, const SeqBatch& s, int room) {
   Plan best{1, 1, 1e30};
   for (int qi = 1; qi <= 2; ++qi) {
     const int rb = (64 * qi) >> p.group_shift;
@@ -560,7 +560,7 @@ int launch_attn_window(AttnWindowParams p, const SeqBatch& s, void* workspace, h
     keys += std::min(s.start[b] + s.n_new[b], p.window + p.n_sinks + s.n_new[b]);
   }
   if (!rows) return IE_OK;
-  const Plan plan = plan_of(p, s, rows, attn_window_part_rows(rows));
+  const Plan plan = plan_of(p, s, attn_window_part_rows(rows));
   const int rb = (64 * plan.qi) >> p.group_shift;
   int items = 0, part = 0;
   for (int b = 0; b < s.n; ++b) {

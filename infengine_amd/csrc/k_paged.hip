@@ -238,7 +238,6 @@ int launch_qk_norm_rope(QkNormRopeParams p, const SeqBatch& s, hipStream_t st) {
   }
   if (!rows) return IE_OK;
   p.n_seqs = s.n;
-  p.rows = rows;
   const dim3 grid(rows), block(256);
   if (p.heads == 16)
     hipLaunchKernelGGL((qk_norm_rope_kernel<2>), grid, block, 0, st, p);

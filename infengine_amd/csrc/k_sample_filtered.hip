@@ -759,8 +759,8 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
   const bool one_round = n <= kHeld * kThreads;
   if (one_round) load_held(0);
 
-  // The cut where the sum of f over the listed tokens (0: not among them), in the order, reaches target >= 1
-  // (never: all of them stay): a radix select of the key from the first bits in which they differ, then,
+  // The cut where the sum of f over the listed tokens (0: not among them; some are), in the order, reaches
+  // target >= 1 (never: all of them stay): a radix select of the key from the first bits in which they differ, then,
   // among equal keys (equal f), the id of the last one needed.
   const auto select = [&](auto f, u64 target) {
     if (tid == 0) s_min = 0xFFFFFFFFu, s_max = 0;
@@ -782,16 +782,6 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
     kmin = wave_min_u32(kmin), kmax = ~wave_min_u32(~kmax);
     if (lane == 0 && kmin <= kmax) atomicMin(&s_min, kmin), atomicMax(&s_max, kmax);
     __syncthreads();
-    if (s_min > s_max) {
-      // masses alone can all be 0 (tokens below 2^-43 in the bins of top_p's cut): none of them stays, and
-      // of the rest the bins above p_lo; the largest logit of bin p_lo or past it, by halving
-      uint32_t a = logit_key(-INFINITY), b = logit_key(mx);
-      while (b - a > 1) {
-        const uint32_t mid = a + (b - a) / 2;
-        (bin(key_logit(mid)) >= p_lo ? a : b) = mid;
-      }
-      return Cut{key_logit(a), 0};
-    }
     uint32_t base = s_min, span = s_max - s_min;  // keys base .. base + span are left
     while (span) {
       const int shift = max(0, 32 - __clz(span) - 11);
@@ -876,9 +866,10 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleParams p,
       z += (double)block_sum(in_bin, red) * (1.0 / kUnit);
     }
     const double want = ceil((z * (double)s.top_p - R.mass_p) * kUnit);
+    // (a token that rounds to no unit counts one here: a bin of such tokens holds its cut as any other)
     cut = select([&](const Listed& t) -> u64 {
                    const int b = bin(t.l);
-                   return b >= p_lo && b <= p_hi && k_cut.keeps(t.l, t.id) ? mass(t.l) : 0;
+                   return b >= p_lo && b <= p_hi && k_cut.keeps(t.l, t.id) ? max(mass(t.l), (u64)1) : 0;
                  },
                  want > 1.0 ? (u64)want : (u64)1);
   }

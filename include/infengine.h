@@ -471,9 +471,10 @@ IE_API int ie_kv_compact_paged(ie_context* ctx, int n_rows, const int* seq_lens,
  * that share of their mass; min_p (<= 0: off) the tokens of at least min_p times the largest weight;
  * the first token always stays.  The result is the first id, in id order, whose cumulative kept mass
  * exceeds uniform x the kept mass.  temperature not > 0, or min_p > 1: the first of the largest logits.
- * Weights and sums in 64 bits; weights below 2^-42 of the largest may count as nothing.  NaN logits
- * count as -inf; a row without a logit above -inf gives -1.  A NaN top_p or min_p is off; a uniform not
- * > 0 counts as 0, one >= 1 draws the last kept token.
+ * Weights and sums in 64 bits (sums in whole units of 2^-42 or less of the largest weight); weights
+ * below 2^-42 of the largest may count as nothing.  NaN logits count as -inf; a row without a logit above
+ * -inf gives -1.  A NaN top_p or min_p is off; a uniform not > 0 counts as 0, one >= 1 draws the last
+ * kept token.
  * workspace: ie_sample_filtered_workspace_size(rows, vocab) bytes. */
 IE_API size_t ie_sample_filtered_workspace_size(int rows, int vocab);
 IE_API int ie_sample_filtered(ie_context* ctx, int rows, int vocab, const float* d_logits,

@@ -16,7 +16,7 @@ namespace {
 // lanes apart.  A workgroup takes a row: GROUPS of 16 heads, the last one K and V.  A lane keeps its dims'
 // angles and weights over its heads (a workgroup for 16 heads, each with its own loads of the
 // angles, 64 bytes a lane beside 16 of the row, took 24.4 us for 4214 normed rows of 48 heads; this one
-// 18.8, 5.6 TB/s read and written, bound by them; one token of 16 sequences 5.7, the launch).
+// 18.8, 5.6 TB/s read and written, bound by them; one token of 16 sequences 5.7-6.4, the launch).
 template <int GROUPS>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p) {
   const int tid = threadIdx.x, lane = tid & 63, li = tid & 15, hg = tid >> 4;
@@ -91,7 +91,7 @@ static_assert(kPlanes >= kMaxSeqs, "a workgroup for every table row of a group")
 // blockIdx.x: a plane, blockIdx.y: a group.  The first n_pos % 64 positions of the plane in the source's
 // last page are read once and written to every fork's page; the first workgroups also write a table
 // row each.  Bound by the stores: 16 forks of 58 positions, 122 MB written, take 21.7 us, 5.6 TB/s of them (with a
-// copy per fork 31); four forks of one short prompt 5.8, the launch.
+// copy per fork 31; a nontemporal fill of as much 22); four forks of one short prompt 5.6-6.0, the launch.
 __global__ __launch_bounds__(256) void kv_fork_kernel(ForkParams p) {
   const int g = blockIdx.y, plane = blockIdx.x;
   const int first = g ? p.end[g - 1] : 0, end = p.end[g];
@@ -142,7 +142,9 @@ __device__ __forceinline__ bool entry_kept(const CompactParams& p, int n, int i)
 
 // One workgroup: marks the pages that the kept entries name in an LDS bitmap, ranks them, pairs the
 // live ids >= the live count with the free ids below it in ascending order, and writes the
-// remapped tables.  4.5 us for 4 or 8 rows: a chain of barriers and dependent loads, small beside the moves.
+// remapped tables.  4.5 us for 4 or 8 rows of up to 63 entries: a chain of barriers and dependent loads, small beside
+// the moves; the call takes 18 us for 64 rows of 128 entries, 51 of 512 and 187 of 2048 where nothing moves: 1024
+// entries a step, twice.
 __global__ __launch_bounds__(kPlanThreads) void kv_compact_plan_kernel(CompactParams p) {
   constexpr int kWords = kCompactMaxPages / 64, kPer = kWords / kPlanThreads;
   __shared__ unsigned long long live[kWords];
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_compact_plan_kernel(CompactPa
 constexpr int kMoveBytes = 64 << 10;  // of a page, a workgroup at a time
 
 // Moves the pages: sources are ids >= the live count, destinations free ids below it.  Bound by HBM: 17 pages of 8 MiB
-// 47 us, 83 252, 5.4-5.5 TB/s read and written (a plain copy of 4 GiB reaches 4.8).
+// 47 us, 6.0 TB/s read and written, 83 252, 5.5 (a nontemporal copy of as much 5.5-5.7 and 5.1-5.2).
 __global__ __launch_bounds__(256) void kv_compact_move_kernel(CompactParams p) {
   constexpr int kParts = (int)(kPageElems * 2 / kMoveBytes), kEach = kMoveBytes / 16 / 256;
   const int total = p.counts[1] * kParts;

@@ -31,8 +31,9 @@
 // 5.8, 13.4, 11.3; 14.0, 4.0, 9.7.  One row is bound by the waits of three launches for each other's results
 // (a launch that only reads the row's state takes 3-4); 64 rows by the weights' fp64 steps and the histogram's
 // LDS additions in the first two launches, and in the last, which one CU a row runs, by the barriers of the
-// selects (top-p 0.9, of 40000 cycles: 3200 for the smallest and largest key, 3400-4000 a digit, two of them,
-// 4000 for the id).
+// selects and the weights of the draw's chunk (top-p 0.9, of 45500 cycles: 3300 the row's state, 1800 its lists,
+// 16900 the select (4800 the smallest and largest key, 4000 a digit, two of them, 4000 the id), 3700 the chunks' kept
+// masses, 1150 the draw's chunk, 16500 the weights of its 16032 logits, 2200 the last 64).
 #include "ie_kernels.h"
 
 namespace ie {

@@ -1,12 +1,14 @@
 """Forms of the paged-serving kernels that only large batches and pools reach: attention by 32 columns a
-wave around infinities and NaN, and compaction of pools of more than 4096 pages."""
+wave around infinities and NaN, pages gigabytes into a pool, compaction of pools of more than 4096 pages,
+and page operators in a graph."""
 import numpy as np
 import pytest
 import torch
 
 from gpu_util import say
-from test_gpu_paged_serving import (ALL, D, KVH, LAYER, LAYERS, PAGE, attend, attend64, bf16,
-                                    check_attend, compact_plan, gen, ints, make_pool, make_tables, ptr)
+from test_gpu_paged_serving import (ALL, D, KVH, LAYER, LAYERS, PAGE, append, attend, attend64, bf16,
+                                    check_attend, compact_plan, gen, ints, make_pool, make_tables, ptr,
+                                    rope)
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +140,77 @@ def test_compact_pool_of_thousands_of_pages(hip, ctx, n_pages, held, pick, windo
     holds = torch.from_numpy(holds.astype(np.int32)).cuda()
     for a in range(0, n_pages, 500):
         assert torch.equal(pool[a:a + 500], holds[a:a + 500, None] + inside)
+
+
+def test_pages_far_into_the_pool(hip, ctx):
+    """Append, attend and fork in pages past 2^32 elements (8 GiB) from the pool's start: as in pages near it."""
+    say("pages far into the pool")
+    n_pages, near = 1100, [1, 3, 5]
+    far = [1099, 1030, 1025]
+    assert min(far) * LAYERS * 2 * KVH * PAGE * D > 2**32
+    g = gen(50)
+    pool = torch.empty(n_pages, LAYERS, 2, KVH, PAGE, D, dtype=torch.bfloat16, device="cuda")
+    tables = torch.tensor([near[:2] + [-1], far[:2] + [-1], [-1] * 3, [-1] * 3], dtype=torch.int32, device="cuda")
+    cos, sin = rope(128)
+    qkv = bf16(g, 100, 48 * D).repeat(2, 1)
+    q, out = (torch.empty(200, 32, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pool[near + far] = 0
+    append(hip, ctx, [0, 0], [100, 100], 32, qkv, None, None, cos, sin, q, pool, tables, layer=31)
+    attend(hip, ctx, [0, 0], [100, 100], 70, 3, 32, q, pool, tables, out, layer=31)
+    hip.check(hip.lib.ie_kv_fork_paged(ctx.handle, 2, ints([0, 1]), ints([2, 3]), ints([90, 90]),
+                                       ints([near[2], far[2]]), ptr(pool), n_pages, ptr(tables), 4, 3))
+    torch.cuda.synchronize()
+    want, tol = attend64([0], [100], 70, 3, 32, q[:100], pool, tables, layer=31)
+    check_attend(out[:100], want, tol)
+    assert torch.equal(out[100:], out[:100])
+    for a, b in zip(near, far):
+        assert torch.equal(pool[a], pool[b])
+    assert pool[near[2], 31, :, :, :26].ne(0).any() and not pool[near[2], :, :, :, 26:].any()
+    assert tables[2:].tolist() == [[near[0], near[2], -1], [far[0], far[2], -1]]
+
+
+def test_fork_and_compact_captured(hip, ctx):
+    """A fork and a compaction recorded into one graph and replayed over new pages and tables."""
+    say("captured fork and compaction")
+    g = gen(51)
+    n_pages, stride, lens = 24, 4, [0, 150, 150, 70]
+    pool = torch.empty(n_pages, LAYERS, 2, KVH, PAGE, D, dtype=torch.bfloat16, device="cuda")
+    tables = torch.empty(4, stride, dtype=torch.int32, device="cuda")
+    new, remap = torch.empty_like(tables), torch.empty(n_pages, dtype=torch.int32, device="cuda")
+    counts = torch.empty(2, dtype=torch.int32, device="cuda")
+    ws = torch.empty(hip.lib.ie_kv_compact_workspace_size(n_pages), dtype=torch.uint8, device="cuda")
+
+    def fill():
+        pool.normal_(0.0, 1.0, generator=g)
+        ids = torch.randperm(20, device="cuda", generator=g).int()
+        tables.fill_(-1)
+        tables[0, :3] = ids[:3]
+        tables[3, :2] = ids[3:5]
+        torch.cuda.synchronize()
+
+    def step():
+        hip.check(hip.lib.ie_kv_fork_paged(ctx.handle, 2, ints([0, 0]), ints([1, 2]), ints([150, 150]),
+                                           ints([21, 23]), ptr(pool), n_pages, ptr(tables), 4, stride))
+        hip.check(hip.lib.ie_kv_compact_paged(ctx.handle, 4, ints(lens), ALL, 0, ptr(pool), n_pages, ptr(tables),
+                                              stride, ptr(new), ptr(remap), ptr(counts), ptr(ws)))
+
+    fill()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=ctx.stream):
+        step()
+    for _ in range(4):
+        fill()
+        kept = pool.clone(), tables.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in (pool, tables, new, remap, counts)]
+        pool.copy_(kept[0])
+        tables.copy_(kept[1])
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (pool, tables, new, remap, counts)))
+        plan = compact_plan(tables.tolist(), lens, ALL, 0, n_pages)
+        assert (new.tolist(), remap.tolist(), counts.tolist()) == tuple(plan)
+        assert counts.tolist()[0] == 6                    # two shared pages, two of the forks, two of the last
+        old = tables[0, 2].long()
+        assert torch.equal(pool[new[1, 2].long(), :, :, :, :22], kept[0][old, :, :, :, :22])

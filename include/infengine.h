@@ -427,7 +427,8 @@ IE_API int ie_qk_norm_rope_paged(ie_context* ctx, int n_seqs, const int* start_p
  * latter for none; n_sinks >= 0), scaled by 1/sqrt(128).  The new rows' own keys are read from the
  * pages (ie_qk_norm_rope_paged has put them there).  Keys in pages outside [0, n_pages) are not seen
  * (evicted pages; unlike ie_attn_prefill_core_paged, which reads them as zeros); a row that sees none
- * gets zeros, and so does one whose scores are all -inf.  Values at keys that a row does not see never reach it, infinities and NaN included.
+ * gets zeros, and so does one whose scores are all -inf.  Values at keys that a row does not see
+ * never reach it, infinities and NaN included.
  * d_q, d_out: [rows][n_q_heads][128] (bf16).  Softmax and sums in fp32; the weights are rounded to bf16
  * for their product with V.  Few rows over many keys are split over the keys by a rule on all the
  * lengths, on which the rounding depends.  d_out may be d_q.  workspace:

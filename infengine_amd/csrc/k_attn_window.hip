@@ -26,9 +26,9 @@
 // tile of work); one token of 16 sequences over 4096 keys 47.5, of which 43 read their 268 MB at 6.2 TB/s; 8192 rows
 // over 4096 keys each 598, 611 and 647 on three cards, 0.86-0.93 PF: the MFMAs are busy 45% of the cycles and the
 // vector units 60% (exponents, maxima, rescales, packing), and the fragment reads of a CU's 8 waves take about 0.9
-// of a tile step's 2.24 (128 KiB at 382 B/ns and 128 at 238), which two waves a SIMD overlap in part; 6 sequences of up to 333 rows over 1500 keys 72: 328
-// workgroups, so that 72 CUs hold two and set the time (cut in three over the keys the merge's 20 MB of partials a
-// split take what that gains: 75).
+// of a tile step's 2.24 (128 KiB at 382 B/ns and 128 at 238), which two waves a SIMD overlap in part; 6 sequences
+// of up to 333 rows over 1500 keys 72: 328 workgroups, so that 72 CUs hold two and set the time (cut in three over the
+// keys the merge's 20 MB of partials a split take what that gains: 75).
 #include <algorithm>
 
 #include "ie_kernels.h"

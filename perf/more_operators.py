@@ -1,0 +1,597 @@
+"""Cases of the operators on an 8-bit paged K/V cache, and of attention over a prefix that sequences
+share:
+
+  append    ie_qk_norm_rope_paged_fp8: norms and rotation of a ragged batch's queries and keys, K/V
+            quantised into the pages
+  attend    ie_attn_window_paged_fp8: attention of ragged chunks of new tokens over those pages,
+            with a sliding window and sinks
+  shared    ie_attn_shared_paged: attention of continuations whose prompts' pages are shared, each
+            prompt's keys read once for all of them (bf16 or 8-bit pages)
+  convert   ie_kv_pages_to_fp8, ie_kv_pages_from_fp8: pages from the bf16 pool to the 8-bit one and
+            back
+
+An 8-bit row is 128 e4m3 codes and one power of two, 2^e: e is the least integer >= -110 with
+max |x| <= 448 2^e.  A page holds, layer by layer, the codes [K|V][8][64][128] and then the scales'
+exponents (e + 127, a byte) [K|V][8][64], that of row r at 4 (r % 16) + r / 16.
+
+listed() fixes eleven; draw() gives others of the same ranges.  With `own` false a pass is the
+operator's plain form in elementary torch operations, with `own` true the library's call.
+"""
+import functools
+import random
+
+import torch
+
+own = False
+
+KVH, D, PAGE, LAYERS = 8, 128, 64, 32
+MAX_LONG = 131072
+LAYER = 5         # the layer whose pages the attention reads and the append writes
+EPS = 1e-5
+KV_STD = 1.28     # keys and values of a random-init model: sqrt(4096) * 0.02
+EVERYTHING = MAX_LONG   # a window that nothing falls out of
+CODES = 2 * KVH * PAGE * D              # bytes of a layer's codes in a page
+LAYER_BYTES = CODES + 2 * KVH * PAGE    # and with their scales
+LOWEST = -110     # the least scale exponent
+
+
+# ------------------------------------------------------------------------------- cases
+def listed():
+    return [
+        # the new tokens of a full decode batch, without norms (the served model's own form)
+        {"name": "append_16x1", "kind": "append", "seqs": 16, "rows": 1, "ctx": 6000, "heads": 32,
+         "norm": False},
+        # a step that prefills five prompts at once, queries and keys normed
+        {"name": "append_5x1500", "kind": "append", "seqs": 5, "rows": 1500, "ctx": 900,
+         "heads": 32, "norm": True},
+        # one user's next token: the latency of a single chat
+        {"name": "attend_1_at_600", "kind": "attend", "seqs": 1, "rows": 1, "ctx": 600,
+         "heads": 32, "window": EVERYTHING, "sinks": 0},
+        # a full batch of long sessions, one token each, over windows of 4096
+        {"name": "attend_16_at_60000", "kind": "attend", "seqs": 16, "rows": 1, "ctx": 60000,
+         "heads": 32, "window": 4096, "sinks": 4},
+        # a mixed step: the next turns of six sessions, 1 to 333 tokens
+        {"name": "attend_6x333_at_9000", "kind": "attend", "seqs": 6, "rows": 333, "ctx": 9000,
+         "heads": 32, "window": 1500, "sinks": 5},
+        # a long document's chunk, one prefill call's worth of tokens
+        {"name": "attend_8192_at_8192", "kind": "attend", "seqs": 1, "rows": 8192, "ctx": 8192,
+         "heads": 32, "window": 4096, "sinks": 64},
+        # sixteen answers to one prompt, some way in
+        {"name": "shared_16_of_4992", "kind": "shared", "fmt": "bf16", "groups": 1, "seqs": 16,
+         "shared": 4992, "own": 300, "rows": 1, "heads": 32, "window": EVERYTHING, "sinks": 0},
+        # a full batch of users of one long document, the cache in 8 bits
+        {"name": "shared_64_of_16384", "kind": "shared", "fmt": "fp8", "groups": 1, "seqs": 64,
+         "shared": 16384, "own": 500, "rows": 1, "heads": 32, "window": EVERYTHING, "sinks": 0},
+        # users of three system prompts, a few tokens each (drafts to be checked, short turns)
+        {"name": "shared_3_groups_x5", "kind": "shared", "fmt": "fp8", "groups": 3, "seqs": 20,
+         "shared": 2048, "own": 900, "rows": 5, "heads": 32, "window": EVERYTHING, "sinks": 0},
+        # one short conversation's pages into the 8-bit pool
+        {"name": "to_fp8_3", "kind": "convert", "to": True, "pages": 3},
+        # a batch of conversations back into the bf16 pool
+        {"name": "from_fp8_80", "kind": "convert", "to": False, "pages": 80},
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, round(lo * (hi / lo) ** rng.random())))
+
+
+def draw(rng):
+    kind = rng.choice(["append", "attend", "attend", "attend", "shared", "shared", "shared",
+                       "convert"])
+    heads = rng.choice([32, 32, 32, 16, 64])
+    if kind == "append":
+        seqs = rng.randint(1, 16)
+        return {"kind": kind, "seqs": seqs, "rows": _log(rng, 1, 6000 // seqs),
+                "ctx": _log(rng, 8, 6000), "heads": heads, "norm": rng.random() < 0.5}
+    if kind == "attend":
+        seqs = _log(rng, 1, 32)
+        rows = 1 if rng.random() < 0.4 else _log(rng, 2, 6000 // seqs)
+        case = {"kind": kind, "seqs": seqs, "rows": rows, "ctx": _log(rng, 8, 60000),
+                "heads": heads, "sinks": rng.choice([0, 1, 4, 16, 64, 100]),
+                "window": 16384 if seqs <= 4 and rng.random() < 0.5 else _log(rng, 64, 4096)}
+    elif kind == "shared":
+        seqs = _log(rng, 2, 64)
+        rows = 1 if rng.random() < 0.5 else _log(rng, 2, 2000 // seqs)
+        case = {"kind": kind, "fmt": rng.choice(["bf16", "fp8"]),
+                "groups": rng.randint(1, min(4, seqs)), "seqs": seqs,
+                "shared": 64 * _log(rng, 1, 256), "own": _log(rng, 1, 1000), "rows": rows, "heads": heads, "sinks": rng.choice([0, 4, 100]),
+                "window": EVERYTHING if rng.random() < 0.7 else _log(rng, 64, 8192)}
+    else:
+        return {"kind": kind, "to": rng.random() < 0.5, "pages": _log(rng, 1, 80)}
+    while work(case)["flops"] > 5e11:     # the largest listed case's
+        case["rows"] //= 2
+    return case
+
+
+def _batch(case):
+    """(positions before the new tokens, new tokens) of each sequence: the first has the case's
+    ctx and rows, the others between an eighth of the one and all of it, and 1 to the other."""
+    r = random.Random(case["seqs"] * 1000003 + case["ctx"] * 17 + case["rows"])
+    start = [r.randint(case["ctx"] // 8, case["ctx"]) for _ in range(case["seqs"])]
+    new = [r.randint(1, case["rows"]) for _ in range(case["seqs"])]
+    start[0], new[0] = case["ctx"], case["rows"]
+    return start, new
+
+
+def _shared_batch(case):
+    """(sequences, shared positions) of each group, (start, new) of each sequence.  The first group
+    shares the case's positions, the others a quarter of them or more; sequences are between 0 and
+    `own` positions past their group's."""
+    n, k = case["seqs"], case["groups"]
+    r = random.Random(n * 1000003 + case["shared"] * 17 + case["own"] * 5 + case["rows"])
+    cuts = sorted(r.sample(range(1, n), k - 1))
+    sizes = [b - a for a, b in zip([0] + cuts, cuts + [n])]
+    top = case["shared"] // PAGE
+    lens = [PAGE * (r.randint(-(-top // 4), top) if g else top) for g in range(k)]
+    start, new = [], []
+    for size, shared in zip(sizes, lens):
+        start += [shared + r.randint(0, case["own"]) for _ in range(size)]
+        new += [r.randint(1, case["rows"]) for _ in range(size)]
+    new[0] = case["rows"]
+    return sizes, lens, start, new
+
+
+def _blocks_kept(n, window, sinks):
+    """The position blocks that a sequence of n positions still needs for its next token."""
+    return [i for i in range(-(-n // PAGE)) if i * PAGE < sinks or (i + 1) * PAGE > n - window + 1]
+
+
+def _visible(p, window, sinks):
+    """Keys that the row at position p sees."""
+    first = max(0, p - window + 1)
+    return p + 1 - first + min(first, sinks)
+
+
+def _union(start, end, window, sinks):
+    """Of the keys below `end`, those that a row from position `start` on sees."""
+    first = max(0, start - window + 1)
+    return max(0, end - first) + min(first, sinks, end)
+
+
+def work(case):
+    k = case["kind"]
+    if k == "append":
+        rows, heads = sum(_batch(case)[1]), case["heads"]
+        return {"bytes": rows * ((2 * heads + 2 * KVH) * D * 2 + 2 * KVH * (D + 1) + 4 * D),
+                "flops": rows * (heads + KVH) * D * (7 if case["norm"] else 3)}
+    if k == "convert":
+        return {"bytes": case["pages"] * LAYERS * (2 * CODES + LAYER_BYTES),
+                "flops": case["pages"] * LAYERS * CODES}
+    w, s, heads = case["window"], case["sinks"], case["heads"]
+    keys = flops = rows = 0
+    if k == "attend":
+        start, new = _batch(case)
+        row_bytes = 2 * KVH * (D + 1)
+        keys = sum(_union(a, a + n, w, s) for a, n in zip(start, new))
+    else:
+        sizes, lens, start, new = _shared_batch(case)
+        row_bytes = 2 * KVH * (2 * D if case["fmt"] == "bf16" else D + 1)
+        b = 0
+        for size, shared in zip(sizes, lens):
+            keys += _union(min(start[b:b + size]), shared, w, s)
+            keys += sum(_union(a, a + n, w, s) - _union(a, shared, w, s)
+                        for a, n in zip(start[b:b + size], new[b:b + size]))
+            b += size
+    for a, n in zip(start, new):
+        flops += 4 * heads * D * sum(_visible(p, w, s) for p in range(a, a + n))
+        rows += n
+    return {"bytes": keys * row_bytes + 2 * rows * heads * D * 2, "flops": flops}
+
+
+# ------------------------------------------------------------------------------- 8-bit rows
+def _codes(pool):
+    """The codes' bytes [pages][32][K|V][8][64][128] of an 8-bit pool."""
+    return pool.view(-1, LAYERS, LAYER_BYTES)[..., :CODES].unflatten(-1, (2, KVH, PAGE, D))
+
+
+def _scales(pool):
+    """The scales' bytes [pages][32][K|V][8][16][4], of row r at [r % 16][r // 16]."""
+    return pool.view(-1, LAYERS, LAYER_BYTES)[..., CODES:].unflatten(-1, (2, KVH, 16, 4))
+
+
+def _values(pool):
+    """The codes and the scales as the numbers that they stand for."""
+    return _codes(pool).view(torch.float8_e4m3fn), _scales(pool).view(torch.float8_e8m0fnu)
+
+
+def _quantise(x):
+    """(codes' bytes, scales' bytes) of rows [..., 128]."""
+    m, e = torch.frexp(x.abs().amax(-1))
+    e = torch.where(m <= 0.875, e - 9, e - 8).clamp(min=LOWEST)      # 448 = 0.875 * 2^9
+    codes = torch.ldexp(x, -e[..., None]).float().to(torch.float8_e4m3fn)
+    return codes.view(torch.uint8), (e + 127).to(torch.uint8)
+
+
+def _put(pool, page, layer, kv):
+    """Rows kv [pages][K|V][8][64][128] into the given pages of a layer."""
+    codes, e = _quantise(kv.float())
+    _codes(pool)[page, layer] = codes
+    _scales(pool)[page, layer] = e.unflatten(-1, (4, 16)).transpose(-1, -2)
+
+
+# ------------------------------------------------------------------------------- inputs
+class _Gen:
+    """Seeded tensors on the GPU."""
+
+    def __init__(self, seed):
+        self.g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def bf16(self, *shape, mean=0.0, std=1.0):
+        return torch.empty(*shape, dtype=torch.bfloat16, device="cuda").normal_(
+            mean, std, generator=self.g)
+
+
+@functools.cache
+def _rope():
+    """fp32 tables [131072][64] of the angles pos * 500000^(-j/64)."""
+    freq = 500000.0 ** (-torch.arange(64, device="cuda", dtype=torch.float64) / 64)
+    angle = torch.arange(MAX_LONG, device="cuda", dtype=torch.float64)[:, None] * freq
+    return angle.cos().float(), angle.sin().float()
+
+
+def _pool(n_pages, fmt):
+    if fmt == "bf16":
+        return torch.zeros(n_pages, LAYERS, 2, KVH, PAGE, D, dtype=torch.bfloat16, device="cuda")
+    return torch.zeros(n_pages, LAYERS * LAYER_BYTES, dtype=torch.uint8, device="cuda")
+
+
+def _filled(g, n_pages, fmt):
+    """A pool with keys and values of the one layer."""
+    pool = _pool(n_pages, fmt)
+    for p in range(0, n_pages, 512):
+        n = min(512, n_pages - p)
+        kv = g.bf16(n, 2, KVH, PAGE, D, std=KV_STD)
+        if fmt == "bf16":
+            pool[p:p + n, LAYER] = kv
+        else:
+            _put(pool, torch.arange(p, p + n, device="cuda"), LAYER, kv)
+    return pool
+
+
+def _tables(g, blocks, stride):
+    """A shuffled pool for sequences that hold the given position blocks: (pages, tables)."""
+    n = sum(len(b) for b in blocks)
+    order = torch.randperm(n, device="cuda", generator=g.g).to(torch.int32)
+    table = torch.full((len(blocks), stride), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, kept in enumerate(blocks):
+        kept = torch.tensor(list(kept), device="cuda", dtype=torch.long)
+        table[b, kept] = order[at:at + len(kept)]
+        at += len(kept)
+    return n, table
+
+
+def _ints(values):
+    """The lengths as the call takes them."""
+    if not own:
+        return list(values)
+    import ctypes
+    return (ctypes.c_int * len(values))(*values)
+
+
+@functools.cache
+def _stream():
+    return torch.cuda.Stream(0)
+
+
+def _context():
+    from infengine_amd.engine import Context
+    return Context(0, stream=_stream())
+
+
+def prepare(case, seed):
+    k = case["kind"]
+    ctx = _context() if own else None   # (makes its stream torch's current one)
+    g = _Gen(seed)
+    s = {"kind": k, "ctx": ctx, "case": case}
+    if k == "convert":
+        n = case["pages"]
+        # the pages of either pool lie anywhere in it
+        s["src"] = torch.randperm(n + n // 4 + 1, generator=g.g, device="cuda")[:n].to(torch.int32)
+        s["dst"] = torch.randperm(n + n // 4 + 1, generator=g.g, device="cuda")[:n].to(torch.int32)
+        s["bf16"] = _pool(n + n // 4 + 1, "bf16")
+        s["fp8"] = _pool(n + n // 4 + 1, "fp8")
+        for p in s["src"].tolist():
+            kv = g.bf16(LAYERS, 2, KVH, PAGE, D, std=KV_STD)
+            if case["to"]:
+                s["bf16"][p] = kv
+            else:
+                _put(s["fp8"], p, slice(None), kv)
+        return s
+    if k == "shared":
+        sizes, lens, start, new = _shared_batch(case)
+        s["sizes"], s["lens"] = _ints(sizes), _ints(lens)
+    else:
+        start, new = _batch(case)
+    s["start"], s["new"], s["seqs"] = _ints(start), _ints(new), len(start)
+    rows, heads = sum(new), case["heads"]
+    stride = max(-(-(a + n) // PAGE) for a, n in zip(start, new))
+    if k == "append":
+        # the blocks that the new rows fall into (the older ones are not touched)
+        n, s["tables"] = _tables(g, [range(a // PAGE, -(-(a + n) // PAGE))
+                                     for a, n in zip(start, new)], stride)
+        s["pool"] = _filled(g, n, "fp8")
+        s["qkv"] = g.bf16(rows, (heads + 2 * KVH) * D, std=KV_STD)
+        s["wq"] = g.bf16(D, mean=1.0, std=0.1) if case["norm"] else None
+        s["wk"] = g.bf16(D, mean=1.0, std=0.1) if case["norm"] else None
+        s["cos"], s["sin"] = _rope()
+        s["q"] = torch.empty(rows, heads, D, dtype=torch.bfloat16, device="cuda")
+        return s
+    if k == "attend":
+        # pages behind the window of a sequence's first new row are gone
+        blocks = []
+        for a, n in zip(start, new):
+            kept = set(_blocks_kept(a, case["window"], case["sinks"]))
+            blocks.append([i for i in range(-(-(a + n) // PAGE)) if i in kept or i >= a // PAGE])
+        n, s["tables"] = _tables(g, blocks, stride)
+    else:
+        # as forks leave them: a group's sequences name the same pages for the shared positions
+        group = [i for i, size in enumerate(sizes) for _ in range(size)]
+        blocks = [range(x // PAGE) for x in lens]
+        blocks += [range(lens[group[b]] // PAGE, -(-(a + n) // PAGE))
+                   for b, (a, n) in enumerate(zip(start, new))]
+        n, both = _tables(g, blocks, stride)
+        s["tables"] = torch.maximum(both[torch.tensor(group, device="cuda")], both[len(sizes):])
+    fmt = case.get("fmt", "fp8")
+    s["pool"] = _filled(g, n, fmt)
+    s["q"] = g.bf16(rows, heads, D, std=KV_STD)
+    s["out"] = torch.empty(rows, heads, D, dtype=torch.bfloat16, device="cuda")
+    if own:
+        from infengine_amd import lib
+        s["ws"] = torch.empty(lib.ie_attn_shared_workspace_size(rows, heads), dtype=torch.uint8,
+                              device="cuda")
+    return s
+
+
+# ------------------------------------------------------------------------------- one pass
+def run(s):
+    return (_run_own if own else _run_plain)(s)
+
+
+def _pool_out(s):
+    codes, scales = _values(s["fp8" if s["kind"] == "convert" else "pool"])
+    return {"codes": codes, "scales": scales}
+
+
+def _run_own(s):
+    from infengine_amd import check, lib
+    from infengine_amd.engine import ptr
+    k, c, h = s["kind"], s["case"], s["ctx"].handle
+    if k == "append":
+        check(lib.ie_qk_norm_rope_paged_fp8(
+            h, s["seqs"], s["start"], s["new"], c["heads"], ptr(s["qkv"]), s["qkv"].shape[1],
+            ptr(s["wq"]), ptr(s["wk"]), ptr(s["cos"]), ptr(s["sin"]), MAX_LONG, ptr(s["q"]),
+            ptr(s["pool"]), s["pool"].shape[0], ptr(s["tables"]), s["tables"].shape[1], LAYER))
+        return {"q": s["q"], **_pool_out(s)}
+    if k == "attend":
+        check(lib.ie_attn_window_paged_fp8(
+            h, s["seqs"], s["start"], s["new"], c["window"], c["sinks"], c["heads"], ptr(s["q"]),
+            ptr(s["pool"]), s["pool"].shape[0], ptr(s["tables"]), s["tables"].shape[1], LAYER,
+            ptr(s["out"]), ptr(s["ws"])))
+        return s["out"]
+    if k == "shared":
+        check(lib.ie_attn_shared_paged(
+            h, 0 if c["fmt"] == "bf16" else 1, len(s["sizes"]), s["sizes"], s["lens"], s["seqs"],
+            s["start"], s["new"], c["window"], c["sinks"], c["heads"], ptr(s["q"]), ptr(s["pool"]),
+            s["pool"].shape[0], ptr(s["tables"]), s["tables"].shape[1], LAYER, ptr(s["out"]),
+            ptr(s["ws"])))
+        return s["out"]
+    if c["to"]:
+        check(lib.ie_kv_pages_to_fp8(h, c["pages"], ptr(s["src"]), ptr(s["dst"]), ptr(s["bf16"]),
+                                     s["bf16"].shape[0], ptr(s["fp8"]), s["fp8"].shape[0]))
+        return _pool_out(s)
+    check(lib.ie_kv_pages_from_fp8(h, c["pages"], ptr(s["src"]), ptr(s["dst"]), ptr(s["fp8"]),
+                                   s["fp8"].shape[0], ptr(s["bf16"]), s["bf16"].shape[0]))
+    return s["bf16"]
+
+
+def _run_plain(s):
+    return {"append": _append, "attend": _attend, "shared": _attend,
+            "convert": _convert}[s["kind"]](s)
+
+
+def _rows_of(s):
+    """(sequence, position) of every new row, in the rows' order."""
+    new = torch.tensor(s["new"], device="cuda")
+    seq = torch.repeat_interleave(torch.arange(len(s["new"]), device="cuda"), new,
+                                  output_size=sum(s["new"]))
+    first = torch.tensor(s["start"], device="cuda") - (new.cumsum(0) - new)
+    return seq, first[seq] + torch.arange(seq.shape[0], device="cuda")
+
+
+def _append(s):
+    """In 64 bits: a value may fall next to a border of its code."""
+    heads = s["case"]["heads"]
+    seq, pos = _rows_of(s)
+    x = s["qkv"].view(-1, heads + 2 * KVH, D)
+    cos, sin = s["cos"][pos][:, None].double(), s["sin"][pos][:, None].double()
+
+    def turn(v, w):
+        v = v.double()
+        if w is not None:
+            v = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + EPS) * w.double()
+        a, b = v[..., :64], v[..., 64:]
+        return torch.cat([a * cos - b * sin, a * sin + b * cos], dim=-1)
+
+    s["q"].copy_(turn(x[:, :heads], s["wq"]))
+    page, r = s["tables"][seq, pos // PAGE].long(), pos % PAGE
+    codes, scales = _codes(s["pool"]), _scales(s["pool"])
+    for i, kv in enumerate((turn(x[:, heads:heads + KVH], s["wk"]), x[:, heads + KVH:].float())):
+        c, e = _quantise(kv)
+        codes[page, LAYER, i, :, r] = c
+        scales[page, LAYER, i, :, r % 16, r // 16] = e
+    return {"q": s["q"], **_pool_out(s)}
+
+
+def _gather(s, page, r):
+    """fp32 keys and values [keys][K|V][8][128] of the one layer: rows r of the pages."""
+    if s["case"].get("fmt") == "bf16":
+        return s["pool"][page, LAYER, :, :, r].float()
+    codes, scales = _values(s["pool"])
+    scale = scales[page, LAYER, :, :, r % 16, r // 16].float()
+    return codes[page, LAYER, :, :, r].float() * scale[..., None]
+
+
+def _attend(s):
+    c = s["case"]
+    group, w, sinks = c["heads"] // KVH, c["window"], c["sinks"]
+    row = 0
+    for b, (a, n) in enumerate(zip(s["start"], s["new"])):
+        for p0 in range(a, a + n, 512):          # 512 rows at a time
+            p1 = min(p0 + 512, a + n)
+            first = max(0, p0 - w + 1)
+            j = torch.cat([torch.arange(0, min(first, sinks), device="cuda"),
+                           torch.arange(first, p1, device="cuda")])
+            kv = _gather(s, s["tables"][b, j // PAGE].long(), j % PAGE)
+            key = kv[:, 0].permute(1, 2, 0).contiguous()         # [8][128][keys]
+            value = kv[:, 1].transpose(0, 1).contiguous()        # [8][keys][128]
+            p = torch.arange(p0, p1, device="cuda")[:, None, None]
+            hidden = (j > p) | ((j <= p - w) & (j >= sinks))     # [rows][1][keys]
+            q = s["q"][row:row + p1 - p0].float().view(-1, KVH, group, D).transpose(0, 1)
+            sc = torch.matmul(q.reshape(KVH, -1, D), key).mul_(D ** -0.5)
+            sc.view(KVH, -1, group, j.shape[0]).masked_fill_(hidden, float("-inf"))
+            e = sc.sub_(sc.amax(-1, keepdim=True)).exp_()
+            o = torch.matmul(e, value) / e.sum(-1, keepdim=True)
+            s["out"][row:row + p1 - p0].view(-1, KVH, group, D).copy_(
+                o.view(KVH, -1, group, D).transpose(0, 1))
+            row += p1 - p0
+    return s["out"]
+
+
+def _convert(s):
+    src, dst = s["src"].long(), s["dst"].long()
+    if s["case"]["to"]:
+        codes, e = _quantise(s["bf16"][src].float())
+        _codes(s["fp8"])[dst] = codes
+        _scales(s["fp8"])[dst] = e.unflatten(-1, (4, 16)).transpose(-1, -2)
+        return _pool_out(s)
+    codes, scales = _values(s["fp8"])
+    scale = scales[src].float().transpose(-1, -2).flatten(-2)
+    s["bf16"][dst] = (codes[src].float() * scale[..., None]).bfloat16()
+    return s["bf16"]
+
+
+# ------------------------------------------------------------------------------- 64 bits
+def exact(case, seed):
+    global own
+    was, own = own, False
+    try:
+        s = prepare(case, seed)
+    finally:
+        own = was
+    k = case["kind"]
+    if k == "append":
+        return _append64(s, case)
+    if k == "convert":
+        return _convert64(s, case)
+    return _attend64(s, case)
+
+
+@functools.cache
+def _e4m3():
+    """The values of the 256 codes: sign, four bits of exponent, three of mantissa."""
+    def value(c):
+        sign, e, m = 1 - 2 * (c >> 7), c >> 3 & 15, c & 7
+        if e == 15 and m == 7:
+            return float("nan")
+        return sign * (m * 2.0 ** -9 if e == 0 else (8 + m) * 2.0 ** (e - 10))
+    return torch.tensor([value(c) for c in range(256)], dtype=torch.float64, device="cuda")
+
+
+def _bytes64(layer):
+    """The values [..., K|V, 8, 64, 128] in 64 bits of bytes [..., LAYER_BYTES]."""
+    codes = _e4m3()[layer[..., :CODES].int()].unflatten(-1, (2, KVH, PAGE, D))
+    r = torch.arange(PAGE, device="cuda")
+    e = layer[..., CODES:].unflatten(-1, (2, KVH, PAGE))[..., 4 * (r % 16) + r // 16]
+    return codes * (2.0 ** (e.double() - 127))[..., None]
+
+
+def _nearest(x, borders, order):
+    """Codes of the nearest values, ties to the even code: codes in ascending order of value, and
+    the borders between neighbours."""
+    lo = torch.searchsorted(borders, x.contiguous())                 # borders < x
+    hi = torch.searchsorted(borders, x.contiguous(), right=True)     # borders <= x
+    return torch.where(lo % 2 == 0, order[lo], order[hi])
+
+
+def _rows64(x):
+    """(codes' values, scales) of rows in 64 bits, by a search among the codes' values."""
+    v = _e4m3()[:127]                                          # 0 .. 448, a code its own index
+    borders = (v[1:] + v[:-1]) / 2
+    top = x.abs().amax(-1, keepdim=True)
+    e = torch.ceil(torch.log2(top / 448)).clamp(min=LOWEST)
+    e = torch.where(top > 448 * 2.0 ** e, e + 1, e)
+    e = torch.where((top <= 448 * 2.0 ** (e - 1)) & (e > LOWEST), e - 1, e)
+    y = x / 2.0 ** e
+    nearest = _nearest(y.abs(), borders, torch.arange(127, device="cuda"))
+    return v[nearest] * y.sign(), 2.0 ** e[..., 0]
+
+
+def _append64(s, case):
+    """Sequence by sequence as complex numbers: the pair (x_j, x_{j+64}) turned by the angle."""
+    heads = case["heads"]
+    x, out, row = s["qkv"].view(-1, heads + 2 * KVH, D), [], 0
+    codes, scales = (x.double() for x in _values(s["pool"]))
+    table = s["tables"].tolist()
+    for b, (a, n) in enumerate(zip(s["start"], s["new"])):
+        v = x[row:row + n].double()
+        turn = torch.complex(s["cos"][a:a + n].double(), s["sin"][a:a + n].double())[:, None]
+        parts = []
+        for y, w in ((v[:, :heads], s["wq"]), (v[:, heads:heads + KVH], s["wk"])):
+            if w is not None:
+                y = w.double() * y / torch.sqrt((y * y).sum(-1, keepdim=True) / D + EPS)
+            z = torch.complex(y[..., :64].contiguous(), y[..., 64:].contiguous()) * turn
+            parts.append(torch.cat([z.real, z.imag], dim=-1))
+        out.append(parts[0])
+        for i, kv in enumerate((parts[1], v[:, heads + KVH:])):
+            c, e = _rows64(kv)
+            for first in range(a // PAGE * PAGE, a + n, PAGE):
+                lo, hi = max(first, a), min(first + PAGE, a + n)
+                page = table[b][first // PAGE]
+                codes[page, LAYER, i, :, lo - first:hi - first] = c[lo - a:hi - a].transpose(0, 1)
+                rows = torch.arange(lo - first, hi - first, device="cuda")
+                scales[page, LAYER, i, :, rows % 16, rows // 16] = e[lo - a:hi - a].transpose(0, 1)
+        row += n
+    return {"q": torch.cat(out), "codes": codes, "scales": scales}
+
+
+def _attend64(s, case):
+    """Over the dense keys of each sequence that are in a page, by the definition's mask."""
+    group, out, row = case["heads"] // KVH, torch.empty_like(s["q"], dtype=torch.float64), 0
+    for b, (a, n) in enumerate(zip(s["start"], s["new"])):
+        page = s["tables"][b].long()
+        held = (page >= 0).nonzero()[:, 0]
+        j = (held[:, None] * PAGE + torch.arange(PAGE, device="cuda")).reshape(-1)
+        if case.get("fmt") == "bf16":
+            kv = s["pool"][page[held], LAYER]
+        else:
+            kv = _bytes64(s["pool"].view(-1, LAYERS, LAYER_BYTES)[page[held], LAYER])
+        kv = kv.permute(1, 2, 0, 3, 4).reshape(2, KVH, -1, D)[:, :, j < a + n].double()
+        j = j[j < a + n]
+        for r0 in range(0, n, 1024):
+            r1 = min(n, r0 + 1024)
+            p = torch.arange(a + r0, a + r1, device="cuda")[:, None]
+            seen = (j <= p) & ((p - j < case["window"]) | (j < case["sinks"]))
+            for h in range(case["heads"]):
+                q = s["q"][row + r0:row + r1, h].double()
+                sc = torch.where(seen, (q @ kv[0, h // group].t()) / D ** 0.5, float("-inf"))
+                out[row + r0:row + r1, h] = torch.softmax(sc, dim=-1) @ kv[1, h // group]
+        row += n
+    return out
+
+
+def _convert64(s, case):
+    """Page by page."""
+    if case["to"]:
+        codes, scales = (x.double() for x in _values(s["fp8"]))
+        for a, b in zip(s["src"].tolist(), s["dst"].tolist()):
+            c, e = _rows64(s["bf16"][a].double())
+            codes[b] = c
+            r = torch.arange(PAGE, device="cuda")
+            scales[b, ..., r % 16, r // 16] = e
+        return {"codes": codes, "scales": scales}
+    out = s["bf16"].double()
+    for a, b in zip(s["src"].tolist(), s["dst"].tolist()):
+        out[b] = _bytes64(s["fp8"].view(-1, LAYERS, LAYER_BYTES)[a])
+    return out

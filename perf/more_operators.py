@@ -95,7 +95,8 @@ def draw(rng):
         rows = 1 if rng.random() < 0.5 else _log(rng, 2, 2000 // seqs)
         case = {"kind": kind, "fmt": rng.choice(["bf16", "fp8"]),
                 "groups": rng.randint(1, min(4, seqs)), "seqs": seqs,
-                "shared": 64 * _log(rng, 1, 256), "own": _log(rng, 1, 1000), "rows": rows, "heads": heads, "sinks": rng.choice([0, 4, 100]),
+                "shared": 64 * _log(rng, 1, 256), "own": _log(rng, 1, 1000), "rows": rows,
+                "heads": heads, "sinks": rng.choice([0, 4, 100]),
                 "window": EVERYTHING if rng.random() < 0.7 else _log(rng, 64, 8192)}
     else:
         return {"kind": kind, "to": rng.random() < 0.5, "pages": _log(rng, 1, 80)}

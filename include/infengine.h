@@ -483,6 +483,57 @@ IE_API int ie_sample_filtered(ie_context* ctx, int rows, int vocab, const float*
                               const float* d_top_p, const float* d_min_p, const float* d_uniform,
                               int* d_output, void* workspace);
 
+/* ---- an 8-bit page pool, and prefixes that sequences share (no reference counterparts).  As above: ragged
+ * batches, device block tables, 16-byte aligned buffers, the context's stream, no allocation, capturable.
+ *
+ * A page of the 8-bit pool holds 64 positions of every layer in ie_kv_page_size_fp8() bytes (4227072; the bf16
+ * page has 8388608).  A row x (the 128 values of a position, kv head, K or V) is held as e4m3 codes c and one scale:
+ *   x ~ c * 2^e,  e the least integer >= -110 with max |x| <= 448 * 2^e,  c the code nearest to x * 2^-e, ties to even,
+ * so a value is off by at most 2^-4 of itself, or 2^-10 * 2^e if that is more; all NaN if the row holds an infinity
+ * or a NaN.  Layer by layer, [32]: the codes [K|V][8][64][128], then the bytes e + 127 [K|V][8][64], position r's (of
+ * the page's 64) at index 4 * (r % 16) + r / 16.  Pools move by whole pages (ie_kv_fork_paged shares full pages
+ * of any pool; its copy of a partly filled one, and ie_kv_compact_paged, are for bf16 pools). */
+#define IE_KV_BF16 0
+#define IE_KV_FP8 1
+IE_API size_t ie_kv_page_size_fp8(void);
+/* Pages src_pages[i] of the bf16 pool (as ie_prefill_paged and the calls above write them), quantised into
+ * pages dst_pages[i] of the 8-bit pool; and back, exactly (a value past the largest bf16 to an infinity).  The lists
+ * are DEVICE arrays of n ids (0 .. 65536; a table row, say); a pair with an id outside its pool is left out; a page
+ * may be a source several times, a destination once. */
+IE_API int ie_kv_pages_to_fp8(ie_context* ctx, int n, const int* src_pages, const int* dst_pages,
+                              const void* kv_pages, int n_pages, void* fp8_pages, int n_fp8_pages);
+IE_API int ie_kv_pages_from_fp8(ie_context* ctx, int n, const int* src_pages, const int* dst_pages,
+                                const void* fp8_pages, int n_fp8_pages, void* kv_pages, int n_pages);
+/* ie_qk_norm_rope_paged with an 8-bit pool: q as there, the K and V rows quantised from fp32 (K after its norm and
+ * rotation: not rounded to bf16 before).  The rest of its contract holds. */
+IE_API int ie_qk_norm_rope_paged_fp8(ie_context* ctx, int n_seqs, const int* start_pos, const int* n_new,
+                                     int n_q_heads, const ie_bf16* d_qkv, long long qkv_stride,
+                                     const ie_bf16* d_q_norm, const ie_bf16* d_k_norm,
+                                     const float* d_rope_cos, const float* d_rope_sin, int rope_rows,
+                                     ie_bf16* d_q_out, void* fp8_pages, int n_pages,
+                                     const int* block_tables, int table_stride, int layer);
+/* ie_attn_window_paged over an 8-bit pool, to its contract, with a workspace of
+ * ie_attn_shared_workspace_size(rows, n_q_heads) bytes for at least the batch's rows, contents of no account (the
+ * size never falls as rows grow). */
+IE_API size_t ie_attn_shared_workspace_size(int rows, int n_q_heads);
+IE_API int ie_attn_window_paged_fp8(ie_context* ctx, int n_seqs, const int* start_pos, const int* n_new,
+                                    int window, int n_sinks, int n_q_heads, const ie_bf16* d_q,
+                                    const void* fp8_pages, int n_pages, const int* block_tables,
+                                    int table_stride, int layer, ie_bf16* d_out, void* workspace);
+/* The same attention for a batch in which groups of sequences share pages (kv_format IE_KV_BF16 or IE_KV_FP8: of
+ * which pool): the batch's first group_seqs[0] sequences have the pages of their first shared_len[0] positions (a
+ * multiple of 64, at most the start_pos of each that has new rows) in common, the next group_seqs[1] those of
+ * shared_len[1], and so on (HOST arrays; the n_groups groups hold all n_seqs sequences; a group may be one sequence
+ * or share 0 positions).  Those keys are read once for the group's sequences of few rows, not once for each.  The
+ * sequences' table rows name the shared pages each, as ie_kv_fork_paged leaves them; which of them is read is not
+ * specified.  Otherwise ie_attn_window_paged's contract: every row sees what it sees there. */
+IE_API int ie_attn_shared_paged(ie_context* ctx, int kv_format, int n_groups, const int* group_seqs,
+                                const int* shared_len, int n_seqs, const int* start_pos,
+                                const int* n_new, int window, int n_sinks, int n_q_heads,
+                                const ie_bf16* d_q, const void* kv_pages, int n_pages,
+                                const int* block_tables, int table_stride, int layer, ie_bf16* d_out,
+                                void* workspace);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,8 @@ HEAD_DIM = 128
 FFN_DIM = 14336
 
 IE_OK = 0
+KV_BF16 = 0
+KV_FP8 = 1
 
 _p = C.c_void_p
 
@@ -129,6 +131,16 @@ SIGNATURES: dict[str, tuple] = {
     "ie_kv_compact_paged": (_i, [_p, _i, C.POINTER(_i), _i, _i, _p, _i, _p, _i, _p, _p, _p, _p]),
     "ie_sample_filtered_workspace_size": (_sz, [_i, _i]),
     "ie_sample_filtered": (_i, [_p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "ie_kv_page_size_fp8": (_sz, []),
+    "ie_kv_pages_to_fp8": (_i, [_p, _i, _p, _p, _p, _i, _p, _i]),
+    "ie_kv_pages_from_fp8": (_i, [_p, _i, _p, _p, _p, _i, _p, _i]),
+    "ie_qk_norm_rope_paged_fp8": (_i, [_p, _i, C.POINTER(_i), C.POINTER(_i), _i, _p, C.c_longlong,
+                                       _p, _p, _p, _p, _i, _p, _p, _i, _p, _i, _i]),
+    "ie_attn_shared_workspace_size": (_sz, [_i, _i]),
+    "ie_attn_window_paged_fp8": (_i, [_p, _i, C.POINTER(_i), C.POINTER(_i), _i, _i, _i, _p, _p, _i,
+                                      _p, _i, _i, _p, _p]),
+    "ie_attn_shared_paged": (_i, [_p, _i, _i, C.POINTER(_i), C.POINTER(_i), _i, C.POINTER(_i),
+                                  C.POINTER(_i), _i, _i, _i, _p, _p, _i, _p, _i, _i, _p, _p]),
     "ie_tune_gemv_waves": (_i, [_i]),
     "ie_tune_gemv_pairs_per_wave": (_i, [_i]),
     "ie_tune_gemm_schedule": (_i, [_i]),

@@ -287,6 +287,73 @@ int check_window(const char* what, int window, int n_sinks) {
   return IE_OK;
 }
 
+// The append's arguments, checked, but for the pages' addresses.
+int append_params(const char* what, QkNormRopeParams* p, const Context* c, int n_seqs, const int* start_pos,
+                  const int* n_new, int n_q_heads, const uint16_t* d_qkv, long long qkv_stride,
+                  const uint16_t* d_q_norm, const uint16_t* d_k_norm, const float* d_rope_cos,
+                  const float* d_rope_sin, int rope_rows, uint16_t* d_q_out, const void* pages, int n_pages,
+                  const int* block_tables, int table_stride, int layer) {
+  IE_REQUIRE(c != nullptr, "%s: null context", what);
+  IE_REQUIRE(d_qkv && d_rope_cos && d_rope_sin && d_q_out && pages && block_tables, "%s: null pointer", what);
+  IE_TRY(check_batch(what, n_seqs, start_pos, n_new, table_stride));
+  IE_TRY(check_paged(what, n_q_heads, n_pages, layer));
+  IE_REQUIRE(qkv_stride >= (n_q_heads + 2 * kKVHeads) * kHeadDim && qkv_stride % 8 == 0,
+             "%s: qkv_stride %lld (at least %d, a multiple of 8)", what, qkv_stride,
+             (n_q_heads + 2 * kKVHeads) * kHeadDim);
+  IE_REQUIRE(aligned16(d_qkv, d_q_norm, d_k_norm, d_rope_cos, d_rope_sin, d_q_out, pages),
+             "%s: a pointer is not 16-byte aligned", what);
+  for (int b = 0; b < n_seqs; ++b)
+    IE_REQUIRE(n_new[b] == 0 || start_pos[b] + n_new[b] <= rope_rows,
+               "%s: sequence %d ends at position %d, past the %d RoPE table rows", what, b,
+               start_pos[b] + n_new[b], rope_rows);
+  p->qkv = d_qkv;
+  p->qkv_stride = qkv_stride;
+  p->q_norm = d_q_norm;
+  p->k_norm = d_k_norm;
+  p->rope_cos = d_rope_cos;
+  p->rope_sin = d_rope_sin;
+  p->q_out = d_q_out;
+  p->block_tables = block_tables;
+  p->table_stride = table_stride;
+  p->n_pages = n_pages;
+  p->heads = n_q_heads;
+  return IE_OK;
+}
+
+// The arguments of attention over a prefix or 8-bit pages, checked; p->pages is the pool.
+int attn_params(const char* what, AttnSharedParams* p, const Context* c, int n_seqs, const int* start_pos,
+                const int* n_new, int window, int n_sinks, int n_q_heads, const uint16_t* d_q, const void* pages,
+                int n_pages, const int* block_tables, int table_stride, int layer, uint16_t* d_out,
+                const void* workspace) {
+  IE_REQUIRE(c != nullptr, "%s: null context", what);
+  IE_REQUIRE(d_q && pages && block_tables && d_out && workspace, "%s: null pointer", what);
+  IE_TRY(check_batch(what, n_seqs, start_pos, n_new, table_stride));
+  IE_TRY(check_paged(what, n_q_heads, n_pages, layer));
+  IE_TRY(check_window(what, window, n_sinks));
+  IE_REQUIRE(aligned16(d_q, pages, d_out, workspace), "%s: a pointer is not 16-byte aligned", what);
+  p->q = d_q;
+  p->pages = static_cast<const uint8_t*>(pages);
+  p->out = d_out;
+  p->block_tables = block_tables;
+  p->table_stride = table_stride;
+  p->n_pages = n_pages;
+  p->window = window;
+  p->n_sinks = n_sinks;
+  p->group_shift = n_q_heads == 16 ? 1 : n_q_heads == 32 ? 2 : 3;
+  return IE_OK;
+}
+
+// n page ids of either pool.
+int check_convert(const char* what, const Context* c, int n, const int* src, const int* dst, const void* pages,
+                  int n_pages, const void* pages8, int n_pages8) {
+  IE_REQUIRE(c != nullptr, "%s: null context", what);
+  IE_REQUIRE(n >= 0 && n <= kCompactMaxPages, "%s: %d pages out of [0, %d]", what, n, kCompactMaxPages);
+  IE_REQUIRE(src && dst && pages && pages8, "%s: null pointer", what);
+  IE_REQUIRE(n_pages >= 1 && n_pages8 >= 1, "%s: pools of %d and %d pages", what, n_pages, n_pages8);
+  IE_REQUIRE(aligned16(pages, pages8), "%s: a pointer is not 16-byte aligned", what);
+  return IE_OK;
+}
+
 // ---- RoPE tables: rope.cu:68-96 (Llama-3 frequency scaling, theta 500000)
 void rope_tables_host(std::vector<float>& cos_t, std::vector<float>& sin_t) {
   const float theta = 500000.0f;
@@ -1680,35 +1747,13 @@ int ie_qk_norm_rope_paged(ie_context* c, int n_seqs, const int* start_pos, const
                           const float* d_rope_cos, const float* d_rope_sin, int rope_rows,
                           ie_bf16* d_q_out, void* kv_pages, int n_pages, const int* block_tables,
                           int table_stride, int layer) {
-  IE_REQUIRE(c != nullptr, "qk_norm_rope_paged: null context");
-  IE_REQUIRE(d_qkv && d_rope_cos && d_rope_sin && d_q_out && kv_pages && block_tables,
-             "qk_norm_rope_paged: null pointer");
-  IE_TRY(check_batch("qk_norm_rope_paged", n_seqs, start_pos, n_new, table_stride));
-  IE_TRY(check_paged("qk_norm_rope_paged", n_q_heads, n_pages, layer));
-  IE_REQUIRE(qkv_stride >= (n_q_heads + 2 * kKVHeads) * kHeadDim && qkv_stride % 8 == 0,
-             "qk_norm_rope_paged: qkv_stride %lld (at least %d, a multiple of 8)", qkv_stride,
-             (n_q_heads + 2 * kKVHeads) * kHeadDim);
-  IE_REQUIRE(aligned16(d_qkv, d_q_norm, d_k_norm, d_rope_cos, d_rope_sin, d_q_out, kv_pages),
-             "qk_norm_rope_paged: a pointer is not 16-byte aligned");
-  for (int b = 0; b < n_seqs; ++b)
-    IE_REQUIRE(n_new[b] == 0 || start_pos[b] + n_new[b] <= rope_rows,
-               "qk_norm_rope_paged: sequence %d ends at position %d, past the %d RoPE table rows", b,
-               start_pos[b] + n_new[b], rope_rows);
-  IE_TRY(set_device(c));
   QkNormRopeParams p{};
-  p.qkv = d_qkv;
-  p.qkv_stride = qkv_stride;
-  p.q_norm = d_q_norm;
-  p.k_norm = d_k_norm;
-  p.rope_cos = d_rope_cos;
-  p.rope_sin = d_rope_sin;
-  p.q_out = d_q_out;
+  IE_TRY(append_params("qk_norm_rope_paged", &p, c, n_seqs, start_pos, n_new, n_q_heads, d_qkv, qkv_stride, d_q_norm,
+                       d_k_norm, d_rope_cos, d_rope_sin, rope_rows, d_q_out, kv_pages, n_pages, block_tables,
+                       table_stride, layer));
+  IE_TRY(set_device(c));
   p.k = static_cast<uint16_t*>(kv_pages) + (size_t)layer * kPageLayer;
   p.v = p.k + (size_t)kKVHeads * kPageHead;
-  p.block_tables = block_tables;
-  p.table_stride = table_stride;
-  p.n_pages = n_pages;
-  p.heads = n_q_heads;
   return launch_qk_norm_rope(p, SeqBatch{n_seqs, start_pos, n_new}, c->stream);
 }
 
@@ -1825,6 +1870,88 @@ int ie_sample_filtered(ie_context* c, int rows, int vocab, const float* d_logits
   const SampleParams p{d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_output,
                        rows, vocab};
   return launch_sample_filtered(p, workspace, c->stream);
+}
+
+// ---------------------------------------------------------------- 8-bit pages, shared prefixes
+size_t ie_kv_page_size_fp8(void) { return kPage8Bytes; }
+
+int ie_kv_pages_to_fp8(ie_context* c, int n, const int* src_pages, const int* dst_pages, const void* kv_pages,
+                       int n_pages, void* fp8_pages, int n_fp8_pages) {
+  IE_TRY(check_convert("kv_pages_to_fp8", c, n, src_pages, dst_pages, kv_pages, n_pages, fp8_pages, n_fp8_pages));
+  if (n == 0) return IE_OK;
+  IE_TRY(set_device(c));
+  return launch_kv_to_fp8(n, src_pages, dst_pages, static_cast<const uint16_t*>(kv_pages), n_pages,
+                          static_cast<uint8_t*>(fp8_pages), n_fp8_pages, c->stream);
+}
+
+int ie_kv_pages_from_fp8(ie_context* c, int n, const int* src_pages, const int* dst_pages,
+                         const void* fp8_pages, int n_fp8_pages, void* kv_pages, int n_pages) {
+  IE_TRY(check_convert("kv_pages_from_fp8", c, n, src_pages, dst_pages, kv_pages, n_pages, fp8_pages, n_fp8_pages));
+  if (n == 0) return IE_OK;
+  IE_TRY(set_device(c));
+  return launch_kv_from_fp8(n, src_pages, dst_pages, static_cast<const uint8_t*>(fp8_pages), n_fp8_pages,
+                            static_cast<uint16_t*>(kv_pages), n_pages, c->stream);
+}
+
+int ie_qk_norm_rope_paged_fp8(ie_context* c, int n_seqs, const int* start_pos, const int* n_new,
+                              int n_q_heads, const ie_bf16* d_qkv, long long qkv_stride,
+                              const ie_bf16* d_q_norm, const ie_bf16* d_k_norm,
+                              const float* d_rope_cos, const float* d_rope_sin, int rope_rows,
+                              ie_bf16* d_q_out, void* fp8_pages, int n_pages,
+                              const int* block_tables, int table_stride, int layer) {
+  QkNormRopeParams p{};
+  IE_TRY(append_params("qk_norm_rope_paged_fp8", &p, c, n_seqs, start_pos, n_new, n_q_heads, d_qkv, qkv_stride,
+                       d_q_norm, d_k_norm, d_rope_cos, d_rope_sin, rope_rows, d_q_out, fp8_pages, n_pages,
+                       block_tables, table_stride, layer));
+  IE_TRY(set_device(c));
+  p.layer8 = static_cast<uint8_t*>(fp8_pages) + (size_t)layer * kPage8Layer;
+  return launch_qk_norm_rope(p, SeqBatch{n_seqs, start_pos, n_new}, c->stream);
+}
+
+size_t ie_attn_shared_workspace_size(int rows, int n_q_heads) {
+  return align256(attn_shared_workspace_bytes(std::max(rows, 1), std::max(n_q_heads, kKVHeads)));
+}
+
+int ie_attn_window_paged_fp8(ie_context* c, int n_seqs, const int* start_pos, const int* n_new,
+                             int window, int n_sinks, int n_q_heads, const ie_bf16* d_q,
+                             const void* fp8_pages, int n_pages, const int* block_tables,
+                             int table_stride, int layer, ie_bf16* d_out, void* workspace) {
+  AttnSharedParams p{};
+  IE_TRY(attn_params("attn_window_paged_fp8", &p, c, n_seqs, start_pos, n_new, window, n_sinks, n_q_heads, d_q,
+                     fp8_pages, n_pages, block_tables, table_stride, layer, d_out, workspace));
+  IE_TRY(set_device(c));
+  p.pages += (size_t)layer * kPage8Layer;
+  return launch_attn_shared(p, SeqBatch{n_seqs, start_pos, n_new}, SharedGroups{}, true, workspace, c->stream);
+}
+
+int ie_attn_shared_paged(ie_context* c, int kv_format, int n_groups, const int* group_seqs,
+                         const int* shared_len, int n_seqs, const int* start_pos, const int* n_new,
+                         int window, int n_sinks, int n_q_heads, const ie_bf16* d_q,
+                         const void* kv_pages, int n_pages, const int* block_tables,
+                         int table_stride, int layer, ie_bf16* d_out, void* workspace) {
+  AttnSharedParams p{};
+  IE_REQUIRE(kv_format == IE_KV_BF16 || kv_format == IE_KV_FP8, "attn_shared_paged: kv_format %d", kv_format);
+  IE_TRY(attn_params("attn_shared_paged", &p, c, n_seqs, start_pos, n_new, window, n_sinks, n_q_heads, d_q, kv_pages,
+                     n_pages, block_tables, table_stride, layer, d_out, workspace));
+  IE_REQUIRE(n_groups >= 1 && n_groups <= n_seqs, "attn_shared_paged: %d groups of %d sequences", n_groups, n_seqs);
+  IE_REQUIRE(group_seqs && shared_len, "attn_shared_paged: null groups");
+  int b = 0;
+  for (int i = 0; i < n_groups; ++i) {
+    IE_REQUIRE(group_seqs[i] >= 1 && group_seqs[i] <= n_seqs - b,
+               "attn_shared_paged: group %d has %d of the %d sequences left", i, group_seqs[i], n_seqs - b);
+    IE_REQUIRE(shared_len[i] >= 0 && shared_len[i] % kPagePos == 0,
+               "attn_shared_paged: group %d shares %d positions (a multiple of %d)", i, shared_len[i], kPagePos);
+    for (const int end = b + group_seqs[i]; b < end; ++b)
+      IE_REQUIRE(n_new[b] == 0 || start_pos[b] >= shared_len[i],
+                 "attn_shared_paged: sequence %d has new rows from position %d, its group shares %d", b, start_pos[b],
+                 shared_len[i]);
+  }
+  IE_REQUIRE(b == n_seqs, "attn_shared_paged: the groups have %d of %d sequences", b, n_seqs);
+  IE_TRY(set_device(c));
+  const bool fp8 = kv_format == IE_KV_FP8;
+  p.pages += (size_t)layer * (fp8 ? kPage8Layer : kPageLayer * sizeof(uint16_t));
+  return launch_attn_shared(p, SeqBatch{n_seqs, start_pos, n_new}, SharedGroups{n_groups, group_seqs, shared_len}, fp8,
+                            workspace, c->stream);
 }
 
 int ie_model_weights_from_safetensors(ie_model_weights* out, const char* const* paths,

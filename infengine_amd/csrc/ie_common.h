@@ -36,6 +36,17 @@ constexpr size_t kPageHead = (size_t)kPagePos * kHeadDim;              // one he
 constexpr size_t kPageLayer = 2 * (size_t)kKVHeads * kPageHead;        // one layer in a page
 constexpr size_t kPageElems = (size_t)kLayers * kPageLayer;            // elements per page
 
+// 8-bit paged KV cache: a row (one position, kv head, K or V) is 128 e4m3 codes and a scale 2^e, e the least
+// integer >= kScaleMin - 127 with max |x| <= 448 2^e.  Layer by layer a page holds the codes [K|V][kv head]
+// [kPagePos][128], then the bytes e + 127 [K|V][kv head][kPagePos], row r's at scale_at(r).
+constexpr size_t kPage8Head = (size_t)kPagePos * kHeadDim;                 // bytes of a plane's codes
+constexpr size_t kPage8Codes = 2 * (size_t)kKVHeads * kPage8Head;          // of a layer's codes
+constexpr size_t kPage8Layer = kPage8Codes + 2 * (size_t)kKVHeads * kPagePos;
+constexpr size_t kPage8Bytes = (size_t)kLayers * kPage8Layer;
+constexpr int kScaleMin = 17;
+// (rows r, r + 16, r + 32 and r + 48, which one lane of the matrix products takes, in one dword)
+__host__ __device__ constexpr int scale_at(int r) { return 4 * (r % 16) + r / 16; }
+
 // Decode attention splits the context of each KV head over at most this many blocks.
 constexpr int kAttnSplits = 32;
 constexpr int kAttnTile = 64;
@@ -147,6 +158,39 @@ __device__ __forceinline__ u32x4_t ld_stream(const u32x4_t* p) {
   return __builtin_nontemporal_load(p);
 }
 
+// ---------------------------------------------------------------- 8-bit rows
+// The scale byte of a row whose largest |x| has these bits (finite): with max = m 2^k, 1 <= m < 2,
+// max <= 448 2^e = 1.75 2^(8 + e) for e = k - 8 where m <= 1.75, for e = k - 7 otherwise.
+__device__ __forceinline__ int scale_byte(uint32_t max_bits) {
+  return max((int)((max_bits + 0x1FFFFFu) >> 23) - 8, kScaleMin);
+}
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+// 8 values to codes by their row's largest |x| (its bits): x 2^-e is exact, the code its nearest, ties to
+// even.  A row with an infinity or a NaN gets NaN codes.
+struct Codes8 {
+  uint32_t w[2];
+  int scale;
+};
+__device__ __forceinline__ Codes8 quantise8(const float (&x)[8], uint32_t max_bits) {
+  Codes8 c;
+  const bool bad = max_bits >= 0x7F800000u;
+  c.scale = bad ? 127 : scale_byte(max_bits);
+  const float inv = __uint_as_float((uint32_t)(254 - c.scale) << 23);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, w, true);
+    c.w[i] = bad ? 0x7F7F7F7Fu : (uint32_t)w;
+  }
+  return c;
+}
+// 4 codes times their row's scale as bf16, exact (an infinity past the largest bf16).
+typedef unsigned int u32x2v_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x2v_t dequantise4(uint32_t w, float scale) {
+  return u32x2v_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
+}
+
 // ---------------------------------------------------------------- wave reductions
 // DPP controls (GCN3+ encoding): quad_perm, row_half_mirror, row_mirror.
 constexpr int kDppQuadXor1 = 0xB1;   // quad_perm [1,0,3,2]
@@ -175,6 +219,14 @@ __device__ __forceinline__ float row16_max(float v) {
   v = fmaxf(v, dpp_f<kDppRowHalfMirror>(v));
   v = fmaxf(v, dpp_f<kDppRowMirror>(v));
   return v;
+}
+
+__device__ __forceinline__ uint32_t row16_umax(uint32_t v) {
+  const auto step = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  v = step(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppQuadXor1, 0xF, 0xF, false));
+  v = step(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppQuadXor2, 0xF, 0xF, false));
+  v = step(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppRowHalfMirror, 0xF, 0xF, false));
+  return step(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppRowMirror, 0xF, 0xF, false));
 }
 
 // x[l] op x[l ^ 16] and x[l] op x[l ^ 32] on every lane, with gfx950's v_permlane16_swap /

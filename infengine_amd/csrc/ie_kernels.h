@@ -296,7 +296,7 @@ int attn_prefill_splits(int S, int nkeys, int part_rows);
 int launch_attn_prefill(const AttnPrefillParams& p, hipStream_t st);
 
 // ------------------------------------------------------------ paged serving (k_paged.hip,
-// k_attn_window.hip, k_sample_filtered.hip)
+// k_attn_window.hip, k_attn_shared.hip, k_sample_filtered.hip)
 constexpr int kMaxSeqs = IE_MAX_SEQS;
 // A ragged batch as its host arrays: rows of the sequences one after the other.
 struct SeqBatch {
@@ -315,6 +315,7 @@ struct QkNormRopeParams {
   uint16_t* q_out;         // [rows][heads][128]
   uint16_t* k;             // the layer's head-0 K / V planes of page 0 (pages kPageElems apart)
   uint16_t* v;
+  uint8_t* layer8;         // or the layer in page 0 of an 8-bit pool (pages kPage8Bytes apart)
   const int* block_tables;
   int table_stride, n_pages, heads, n_seqs;
   int start[kMaxSeqs], row_end[kMaxSeqs];  // (set by the launcher, as n_seqs)
@@ -342,6 +343,50 @@ constexpr int kAttnWindowPartRows = 4096;  // (row, split) partials at most
 constexpr int kAttnWindowMaxSplits = 64;
 size_t attn_window_workspace_bytes(int rows, int heads);
 int launch_attn_window(AttnWindowParams p, const SeqBatch& s, void* workspace, hipStream_t st);
+
+// Attention over shared prefixes, of bf16 or 8-bit pages (k_attn_shared.hip).  The batch's rows in two kinds
+// of segments: a group's prefix (the rows of its sequences of few rows, `members`, over the blocks that
+// the group shares) and each sequence's own keys (from block lo on).
+constexpr int kMaxPrefixes = kMaxSeqs / 2;  // (a prefix has two members at least)
+struct AttnSharedParams {
+  const uint16_t* q;        // [rows][heads][128], rotated
+  const uint8_t* pages;     // the layer in page 0
+  uint16_t* out;            // [rows][heads][128]
+  const int* block_tables;
+  int table_stride, n_pages, window, n_sinks;
+  int group_shift;          // log2 of the q heads per kv head
+  // set by the launcher
+  float* part;              // partials [slots][heads][128], then (m, l)
+  float* part_ml;
+  unsigned long long* arrived;  // [seqs][8 kv heads], where the last split to arrive joins them
+  unsigned long long tag;
+  int n_seqs, n_prefixes, prefix_items;
+  bool join;                // splits are joined by the last to arrive
+  bool nt;                  // nontemporal loads of tiles that one workgroup reads
+  // by sequence: first new position; rows up to and with the sequence's, and those of members;
+  // items; key splits; first partial row; first own block; its prefix or -1
+  int start[kMaxSeqs], row_end[kMaxSeqs], member_end[kMaxSeqs];
+  int item_end[kMaxSeqs], splits[kMaxSeqs], part0[kMaxSeqs];
+  int lo[kMaxSeqs], prefix[kMaxSeqs];
+  // by prefix: items up to and with the prefix's; key splits; first partial row; first sequence and
+  // one past the last; shared blocks; the least first position
+  int p_item_end[kMaxPrefixes], p_splits[kMaxPrefixes], p_part0[kMaxPrefixes];
+  int p_first[kMaxPrefixes], p_end[kMaxPrefixes], p_blocks[kMaxPrefixes], p_start[kMaxPrefixes];
+};
+static_assert(sizeof(AttnSharedParams) <= 4096, "kernel arguments");
+struct SharedGroups {
+  int n;               // 0: no sequence shares anything
+  const int* seqs;     // sequences of each
+  const int* shared;   // positions that each shares, a multiple of 64
+};
+size_t attn_shared_workspace_bytes(int rows, int heads);
+int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups& g, bool fp8, void* workspace,
+                       hipStream_t st);
+
+int launch_kv_to_fp8(int n, const int* src, const int* dst, const uint16_t* pages, int n_pages, uint8_t* pages8,
+                     int n_pages8, hipStream_t st);
+int launch_kv_from_fp8(int n, const int* src, const int* dst, const uint8_t* pages8, int n_pages8, uint16_t* pages,
+                       int n_pages, hipStream_t st);
 
 int launch_kv_fork(int n_forks, const int* src_rows, const int* dst_rows, const int* n_pos,
                    const int* new_pages, uint16_t* pages, int n_pages, int* tables, int stride,

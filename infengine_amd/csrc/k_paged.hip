@@ -17,7 +17,9 @@ namespace {
 // angles and weights over its heads (a workgroup for 16 heads, each with its own loads of the
 // angles, 64 bytes a lane beside 16 of the row, took 24.4 us for 4214 normed rows of 48 heads; this one
 // 18.8, 5.6 TB/s read and written, bound by them; one token of 16 sequences 5.7-6.4, the launch).
-template <int GROUPS>
+//
+// F8: K and V rows as codes and a scale, by the row's largest |x| over its 16 lanes.
+template <int GROUPS, bool F8>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p) {
   const int tid = threadIdx.x, lane = tid & 63, li = tid & 15, hg = tid >> 4;
   const int row = blockIdx.x;
@@ -67,6 +69,24 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p) {
     for (int e = 0; e < 4; ++e) y[e] = pack_bf2(t[2 * e], t[2 * e + 1]);
     if (is_q) {
       reinterpret_cast<u32x4_t*>(p.q_out + (size_t)row * p.heads * kHeadDim)[256 * j + tid] = y;
+    } else if constexpr (F8) {
+      float z[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        z[2 * e] = is_v ? bf_lo(x[j][e]) : t[2 * e];
+        z[2 * e + 1] = is_v ? bf_hi(x[j][e]) : t[2 * e + 1];
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(z[e]) & 0x7FFFFFFFu);
+      const Codes8 c = quantise8(z, row16_umax(top));
+      if (page >= 0 && page < p.n_pages) {
+        // (K planes then V planes: hg is the plane)
+        uint8_t* layer = p.layer8 + (size_t)page * kPage8Bytes;
+        const int r = pos % kPagePos;
+        reinterpret_cast<uint2*>(layer + hg * kPage8Head + r * kHeadDim)[li] = make_uint2(c.w[0], c.w[1]);
+        if (li == 0) layer[kPage8Codes + hg * kPagePos + scale_at(r)] = (uint8_t)c.scale;
+      }
     } else if (page >= 0 && page < p.n_pages) {
       uint16_t* dst = (is_v ? p.v : p.k) + (size_t)page * kPageElems +
                       ((size_t)(hg & (kKVHeads - 1)) * kPagePos + pos % kPagePos) * kHeadDim;
@@ -116,6 +136,62 @@ __global__ __launch_bounds__(256) void kv_fork_kernel(ForkParams p) {
 #pragma unroll
     for (int u = 0; u < kPlanePieces / 256; ++u)
       if ((int)threadIdx.x + 256 * u < n) __builtin_nontemporal_store(v[u], d + 256 * u);
+  }
+}
+
+// ---------------------------------------------------------------- bf16 pages <-> 8-bit pages
+// A workgroup takes a plane of a page: 16 lanes a row, 8 values a lane, 16 rows at a time.
+constexpr int kPlaneRounds = kPagePos / 16;
+
+__global__ __launch_bounds__(256) void kv_to_fp8_kernel(const int* src, const int* dst, const uint16_t* pages,
+                                                        int n_pages, uint8_t* pages8, int n_pages8) {
+  const int i = blockIdx.x / kPlanes, plane = blockIdx.x % kPlanes;
+  const int from = src[i], to = dst[i];
+  if (from < 0 || from >= n_pages || to < 0 || to >= n_pages8) return;
+  const int li = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const u32x4_t* s = reinterpret_cast<const u32x4_t*>(pages + (size_t)from * kPageElems + plane * kPageHead) + threadIdx.x;
+  uint8_t* layer = pages8 + (size_t)to * kPage8Bytes + (plane / (2 * kKVHeads)) * kPage8Layer;
+  const int head = plane % (2 * kKVHeads);
+  uint2* codes = reinterpret_cast<uint2*>(layer + head * kPage8Head) + threadIdx.x;
+  u32x4_t x[kPlaneRounds];
+#pragma unroll
+  for (int u = 0; u < kPlaneRounds; ++u) x[u] = ld_stream(s + 256 * u);
+  uint32_t scales = 0;  // of rows r + 16 u, in the order in which they lie
+#pragma unroll
+  for (int u = 0; u < kPlaneRounds; ++u) {
+    float v[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[2 * e] = bf_lo(x[u][e]), v[2 * e + 1] = bf_hi(x[u][e]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    const Codes8 c = quantise8(v, row16_umax(top));
+    codes[256 * u] = make_uint2(c.w[0], c.w[1]);
+    scales |= (uint32_t)c.scale << (8 * u);
+  }
+  if (li == 0) reinterpret_cast<uint32_t*>(layer + kPage8Codes + head * kPagePos)[r] = scales;
+}
+
+__global__ __launch_bounds__(256) void kv_from_fp8_kernel(const int* src, const int* dst, const uint8_t* pages8,
+                                                          int n_pages8, uint16_t* pages, int n_pages) {
+  const int i = blockIdx.x / kPlanes, plane = blockIdx.x % kPlanes;
+  const int from = src[i], to = dst[i];
+  if (from < 0 || from >= n_pages8 || to < 0 || to >= n_pages) return;
+  const int r = threadIdx.x >> 4;
+  const uint8_t* layer = pages8 + (size_t)from * kPage8Bytes + (plane / (2 * kKVHeads)) * kPage8Layer;
+  const int head = plane % (2 * kKVHeads);
+  const uint2* codes = reinterpret_cast<const uint2*>(layer + head * kPage8Head) + threadIdx.x;
+  u32x4_t* d = reinterpret_cast<u32x4_t*>(pages + (size_t)to * kPageElems + plane * kPageHead) + threadIdx.x;
+  uint2 w[kPlaneRounds];
+#pragma unroll
+  for (int u = 0; u < kPlaneRounds; ++u) w[u] = codes[256 * u];
+  const uint32_t scales = reinterpret_cast<const uint32_t*>(layer + kPage8Codes + head * kPagePos)[r];
+#pragma unroll
+  for (int u = 0; u < kPlaneRounds; ++u) {
+    const float scale = scale_of(scales >> (8 * u) & 0xFF);
+    const u32x2v_t a = dequantise4(w[u].x, scale), b = dequantise4(w[u].y, scale);
+    const u32x4_t y = {a[0], a[1], b[0], b[1]};
+    __builtin_nontemporal_store(y, d + 256 * u);
   }
 }
 
@@ -241,12 +317,19 @@ int launch_qk_norm_rope(QkNormRopeParams p, const SeqBatch& s, hipStream_t st) {
   if (!rows) return IE_OK;
   p.n_seqs = s.n;
   const dim3 grid(rows), block(256);
-  if (p.heads == 16)
-    hipLaunchKernelGGL((qk_norm_rope_kernel<2>), grid, block, 0, st, p);
-  else if (p.heads == 32)
-    hipLaunchKernelGGL((qk_norm_rope_kernel<3>), grid, block, 0, st, p);
-  else
-    hipLaunchKernelGGL((qk_norm_rope_kernel<5>), grid, block, 0, st, p);
+#define IE_APPEND(GROUPS)                                                                 \
+  if (p.layer8)                                                                           \
+    hipLaunchKernelGGL((qk_norm_rope_kernel<GROUPS, true>), grid, block, 0, st, p);       \
+  else                                                                                    \
+    hipLaunchKernelGGL((qk_norm_rope_kernel<GROUPS, false>), grid, block, 0, st, p)
+  if (p.heads == 16) {
+    IE_APPEND(2);
+  } else if (p.heads == 32) {
+    IE_APPEND(3);
+  } else {
+    IE_APPEND(5);
+  }
+#undef IE_APPEND
   IE_CHECK_LAUNCH();
   return IE_OK;
 }
@@ -274,6 +357,20 @@ int launch_kv_fork(int n_forks, const int* src_rows, const int* dst_rows, const 
     p.end[groups++] = n;
   }
   hipLaunchKernelGGL(kv_fork_kernel, dim3(kPlanes, groups), dim3(256), 0, st, p);
+  IE_CHECK_LAUNCH();
+  return IE_OK;
+}
+
+int launch_kv_to_fp8(int n, const int* src, const int* dst, const uint16_t* pages, int n_pages, uint8_t* pages8,
+                     int n_pages8, hipStream_t st) {
+  hipLaunchKernelGGL(kv_to_fp8_kernel, dim3(n * kPlanes), dim3(256), 0, st, src, dst, pages, n_pages, pages8, n_pages8);
+  IE_CHECK_LAUNCH();
+  return IE_OK;
+}
+
+int launch_kv_from_fp8(int n, const int* src, const int* dst, const uint8_t* pages8, int n_pages8, uint16_t* pages,
+                       int n_pages, hipStream_t st) {
+  hipLaunchKernelGGL(kv_from_fp8_kernel, dim3(n * kPlanes), dim3(256), 0, st, src, dst, pages8, n_pages8, pages, n_pages);
   IE_CHECK_LAUNCH();
   return IE_OK;
 }

@@ -59,8 +59,9 @@ struct ColumnState {
 // keys, + 4096 for keys + 16).  ks and db are XORs of the swizzled chunk.
 struct Frags {
   uint32_t k0, v0;
-  __device__ __forceinline__ Frags() {
-    const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3;
+  __device__ __forceinline__ Frags() : Frags(threadIdx.x) {}
+  __device__ __forceinline__ explicit Frags(int tid) {
+    const int fr = tid & 15, G = tid >> 4 & 3;
     k0 = (uint32_t)kv_slot(fr, G) * 16;
     v0 = (uint32_t)kv_slot(4 * G + (fr >> 2), (fr & 3) >> 1) * 16 + (fr & 1) * 8;
   }
@@ -133,10 +134,71 @@ __device__ __forceinline__ void weights(bf16x8_t (&pb)[QI][2], ColumnState<QI>& 
   }
 }
 
-// o += V^T . P^T and the sums.  MASK: 0 x (an infinity or NaN) of a key that a column does not see must
+// The same with a reference in place of the maximum: a column keeps it while its scores stay below 2^kLazy times it,
+// so that most tiles rescale nothing (a weight is then up to 2^kLazy, in bf16 as exact as one up to 1).  Its own
+// scores alone decide.  m is then that reference.
+constexpr float kLazy = 8.f;
+template <bool MASK, int QI, int KB>
+__device__ __forceinline__ void weights_lazy(bf16x8_t (&pb)[QI][KB / 2], ColumnState<QI>& c,
+                                             f32x4_t (&s)[QI][KB], int key0, int window, int n_sinks) {
+  int first = 4 * (threadIdx.x >> 4 & 3);  // the lane's first key in each 16
+  if constexpr (MASK) asm volatile("" : "+v"(first));  // (opaque: nothing made of it is kept over the tiles)
+  float mn[QI];
+  bool moved = false;
+#pragma unroll
+  for (int qi = 0; qi < QI; ++qi) {
+    float mt = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (MASK) {
+          const int key = key0 + first + 16 * kb + r;
+          const bool seen = (key <= c.pos[qi]) & ((key > c.pos[qi] - window) | (key < n_sinks));
+          s[qi][kb][r] = seen ? s[qi][kb][r] : -INFINITY;
+        }
+        mt = fmaxf(mt, s[qi][kb][r]);
+      }
+    mt = xor32_max(xor16_max(mt));
+    mn[qi] = mt > c.m[qi] + kLazy / kScoreScale ? mt : c.m[qi];
+    moved |= mn[qi] != c.m[qi];
+  }
+  if (__ballot(moved) != 0) {
+#pragma unroll
+    for (int qi = 0; qi < QI; ++qi) {
+      const float nb = -fmaxf(mn[qi], -3.0e38f) * kScoreScale;
+      const float alpha = __builtin_amdgcn_exp2f(fmaf(c.m[qi], kScoreScale, nb));  // m = -inf: 0
+      c.m[qi] = mn[qi];
+#pragma unroll
+      for (int db = 0; db < 8; ++db) c.o[qi][db] *= alpha;
+      c.l[qi][0] *= alpha;
+    }
+  }
+#pragma unroll
+  for (int qi = 0; qi < QI; ++qi) {
+    const float nb = -fmaxf(mn[qi], -3.0e38f) * kScoreScale;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        s[qi][kb][r] = __builtin_amdgcn_exp2f(fmaf(s[qi][kb][r], kScoreScale, nb));
+#pragma unroll
+    for (int ks2 = 0; ks2 < KB / 2; ++ks2) {
+      const u32x4_t w = {pack_bf2(s[qi][2 * ks2][0], s[qi][2 * ks2][1]),
+                         pack_bf2(s[qi][2 * ks2][2], s[qi][2 * ks2][3]),
+                         pack_bf2(s[qi][2 * ks2 + 1][0], s[qi][2 * ks2 + 1][1]),
+                         pack_bf2(s[qi][2 * ks2 + 1][2], s[qi][2 * ks2 + 1][3])};
+      pb[qi][ks2] = __builtin_bit_cast(bf16x8_t, w);
+    }
+  }
+}
+
+// o += V^T . P^T and the sums, of 32 KS keys.  MASK: 0 x (an infinity or NaN) of a key that a column does not see must
 // stay 0: such values are kept out of the product and added to the columns that see them.
-template <bool MASK, int QI>
-__device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[QI][2], const Frags& f,
+// APART: the dims' products in groups of so many, whose fragments are not read before the group (0: as the
+// compiler likes).
+template <bool MASK, int APART = 0, int QI, int KS>
+__device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[QI][KS], const Frags& f,
                                        const u32x4_t* vtile, int key0, int window, int n_sinks) {
   const u32x4_t ones_w = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
   const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, ones_w);
@@ -144,14 +206,17 @@ __device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[
 #pragma unroll
   for (int qi = 0; qi < QI; ++qi)
 #pragma unroll
-    for (int ks2 = 0; ks2 < 2; ++ks2)
+    for (int ks2 = 0; ks2 < KS; ++ks2)
       c.l[qi] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[qi][ks2], c.l[qi], 0, 0, 0);
   uint32_t bad = 0;
 #pragma unroll
   for (int db = 0; db < 8; ++db) {
     if constexpr (MASK) __builtin_amdgcn_sched_barrier(0);  // (fewer fragments at once: registers)
+    if constexpr (!MASK && APART) {
+      if (db % APART == 0) __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-    for (int ks2 = 0; ks2 < 2; ++ks2) {
+    for (int ks2 = 0; ks2 < KS; ++ks2) {
       const char* va = vb8 + f.v(db) + ks2 * 8192;
       const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)va);
       const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(va + 4096));
@@ -178,7 +243,7 @@ __device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[
 #pragma unroll
       for (int qi = 0; qi < QI; ++qi) {
 #pragma unroll 1
-        for (int key = 0; key < BKEY; ++key) {
+        for (int key = 0; key < 32 * KS; ++key) {
           const int k = key0 + key;
           const bool seen = k <= c.pos[qi] && (k > c.pos[qi] - window || k < n_sinks);
 #pragma unroll
@@ -219,10 +284,11 @@ __device__ __forceinline__ void issue_tile(u32x4_t* stage, __amdgpu_buffer_rsrc_
   for (int j = 0; j < 16 / NW; ++j)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(stage + (ld.wave + NW * j) * 64), 16, ld.voff[j], 0, 0, AUX);
 }
-// How the rows at positions wp0 .. wp1 see the tile from key0 on.
+// How the rows at positions wp0 .. wp1 see the keys from key0 on.
 enum Sight { kNone, kSome, kAll };
+template <int KEYS = BKEY>
 __device__ __forceinline__ Sight sight(int key0, int wp0, int wp1, int window, int n_sinks) {
-  const int last = key0 + BKEY - 1;
+  const int last = key0 + KEYS - 1;
   if (wp1 < wp0 || key0 > wp1 || (last <= wp0 - window && key0 >= n_sinks)) return kNone;
   return last <= wp0 && (key0 > wp1 - window || last < n_sinks) ? kAll : kSome;
 }

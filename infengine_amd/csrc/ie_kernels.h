@@ -358,15 +358,14 @@ struct AttnSharedParams {
   // set by the launcher
   float* part;              // partials [slots][heads][128], then (m, l)
   float* part_ml;
-  unsigned long long* arrived;  // [seqs][8 kv heads], where the last split to arrive joins them
+  unsigned long long* arrived;  // [seqs][4 blocks][8 kv heads]: the last split to arrive joins them
   unsigned long long tag;
   int n_seqs, n_prefixes, prefix_items;
-  bool join;                // splits are joined by the last to arrive
   bool nt;                  // nontemporal loads of tiles that one workgroup reads
-  // by sequence: first new position; rows up to and with the sequence's, and those of members;
-  // items; key splits; first partial row; first own block; its prefix or -1
+  // by sequence: first new position; rows up to and with the sequence's, and those of members; items of the narrow
+  // and of the wide form; key splits; first partial row; first own block; its prefix or -1
   int start[kMaxSeqs], row_end[kMaxSeqs], member_end[kMaxSeqs];
-  int item_end[kMaxSeqs], splits[kMaxSeqs], part0[kMaxSeqs];
+  int narrow_end[kMaxSeqs], wide_end[kMaxSeqs], splits[kMaxSeqs], part0[kMaxSeqs];
   int lo[kMaxSeqs], prefix[kMaxSeqs];
   // by prefix: items up to and with the prefix's; key splits; first partial row; first sequence and
   // one past the last; shared blocks; the least first position

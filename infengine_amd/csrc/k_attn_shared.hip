@@ -32,9 +32,9 @@ namespace ie {
 
 namespace {
 
-constexpr int NW = 4;
+constexpr int NN = 4;  // waves of the narrow form's workgroups
 constexpr int kNarrowCols = 16;
-constexpr int kOutStride = kHeadDim + 4;  // of a column's sums in LDS, floats (no bank conflicts)
+constexpr int kNarrowBlocks = 4;  // of a sequence, at most
 
 // A workgroup's work: rows r0 .. r0 + nr - 1 of a segment of n rows, one kv head, the tiles i0 .. i1 - 1
 // of the segment's run: na blocks from a0 on (sinks), then those from b0 on.
@@ -47,6 +47,7 @@ struct Work {
   int seq;          // own: the sequence, whose table is read (prefix: the first's)
   bool prefix;
   bool whole;       // its rows have no other partials
+  bool with_prefix; // they have a prefix's
   const int* table;
   __device__ __forceinline__ int tile(int i) const { return i < na ? a0 + i : b0 + i - na; }
 };
@@ -70,50 +71,64 @@ __host__ __device__ __forceinline__ Run run_of(int p0, int p1, int lo, int hi, i
   return r;
 }
 
-// Rows of a block of a segment of n rows.
-__host__ __device__ __forceinline__ int block_rows(int n, int gs, int qi) {
-  return (n << gs) <= kNarrowCols ? n : (64 * qi) >> gs;
+// Sequences of up to so many columns share a prefix; others fill blocks of the wide form by themselves.
+constexpr int kMemberCols = 64;
+// A sequence's own keys go to the narrow form: up to 16 columns; and those of members (few beside the prefix's, and
+// joined to it by the narrow form), in blocks of 16.  A prefix never does.
+__host__ __device__ __forceinline__ bool is_narrow(int n, int gs, bool member) {
+  return (n << gs) <= (member ? kMemberCols : kNarrowCols);
 }
+// Rows of a block of the wide form.
+__host__ __device__ __forceinline__ int block_rows(int gs, int waves) { return (16 * waves) >> gs; }
 
 // Workgroup -> (segment, split, row block, kv head): kv heads go round the XCDs, whose L2 then holds the head's
 // keys for the blocks that share them; prefixes come first, then the sequences, of each the last blocks (the
 // longest runs) first.  (the segments' arguments in one go, a lane each)
-__device__ __forceinline__ Work work_of(const AttnSharedParams& p, int qi) {
+template <bool NARROW>
+__device__ __forceinline__ Work work_of(const AttnSharedParams& p, int waves) {
   const int lane = threadIdx.x & 63, gs = p.group_shift;
   Work w;
   w.g = blockIdx.x % kKVHeads;
   int item = blockIdx.x / kKVHeads;
-  w.prefix = item < p.prefix_items;
+  w.prefix = !NARROW && item < p.prefix_items;
   int lo, hi, pmax;
+  const int member_end = p.member_end[lane];
   if (w.prefix) {
-    const int l32 = lane & 31;
-    const int item_end = p.p_item_end[l32];
+    const int l = lane & 31;
+    const int item_end = p.p_item_end[l], firsts = p.p_first[l], ends = p.p_end[l], splits = p.p_splits[l],
+              part0 = p.p_part0[l], starts = p.p_start[l], blocks = p.p_blocks[l];
     const int k = __popcll(__ballot(lane < p.n_prefixes && item_end <= item));
-    w.first = p.p_first[k], w.end = p.p_end[k];
-    w.splits = p.p_splits[k], w.part0 = p.p_part0[k];
-    w.row0 = w.first ? p.member_end[max(w.first - 1, 0)] : 0;  // (members before the prefix's)
-    w.n = p.member_end[w.end - 1] - w.row0;
-    item -= k ? p.p_item_end[max(k - 1, 0)] : 0;
-    w.p0 = p.p_start[k];
-    lo = 0, hi = p.p_blocks[k];
+    w.first = __builtin_amdgcn_readlane(firsts, k), w.end = __builtin_amdgcn_readlane(ends, k);
+    w.splits = __builtin_amdgcn_readlane(splits, k), w.part0 = __builtin_amdgcn_readlane(part0, k);
+    // (members before the prefix's)
+    w.row0 = w.first ? __builtin_amdgcn_readlane(member_end, max(w.first - 1, 0)) : 0;
+    w.n = __builtin_amdgcn_readlane(member_end, w.end - 1) - w.row0;
+    item -= k ? __builtin_amdgcn_readlane(item_end, max(k - 1, 0)) : 0;
+    w.p0 = __builtin_amdgcn_readlane(starts, k);
+    lo = 0, hi = __builtin_amdgcn_readlane(blocks, k);
     w.nkeys = hi * BKEY;
     w.seq = w.first;
+    w.whole = w.with_prefix = false;
     pmax = w.nkeys - 1;
   } else {
-    item -= p.prefix_items;
-    const int item_end = p.item_end[lane];
-    const int b = __popcll(__ballot(lane < p.n_seqs && item_end <= item));
+    item -= NARROW ? 0 : p.prefix_items;
+    const int item_end = NARROW ? p.narrow_end[lane] : p.wide_end[lane], row_end = p.row_end[lane],
+              starts = p.start[lane], splits = p.splits[lane], part0 = p.part0[lane], los = p.lo[lane],
+              prefixes = p.prefix[lane];
+    const int b = __popcll(__ballot(lane < p.n_seqs && item_end <= item)), before = max(b - 1, 0);
     w.seq = b, w.first = b, w.end = b + 1;
-    w.splits = p.splits[b], w.part0 = p.part0[b];
-    w.row0 = b ? p.row_end[max(b - 1, 0)] : 0;
-    w.n = p.row_end[b] - w.row0;
-    item -= b ? p.item_end[max(b - 1, 0)] : 0;
-    w.p0 = p.start[b];
-    lo = p.lo[b], hi = kMaxLongCtx / BKEY;
+    w.splits = __builtin_amdgcn_readlane(splits, b), w.part0 = __builtin_amdgcn_readlane(part0, b);
+    w.row0 = b ? __builtin_amdgcn_readlane(row_end, before) : 0;
+    w.n = __builtin_amdgcn_readlane(row_end, b) - w.row0;
+    item -= b ? __builtin_amdgcn_readlane(item_end, before) : 0;
+    w.p0 = __builtin_amdgcn_readlane(starts, b);
+    lo = __builtin_amdgcn_readlane(los, b), hi = kMaxLongCtx / BKEY;
     w.nkeys = w.p0 + w.n;
+    w.with_prefix = __builtin_amdgcn_readlane(prefixes, b) >= 0;
+    w.whole = w.splits == 1 && !w.with_prefix;
     pmax = 0;
   }
-  const int rb = block_rows(w.n, gs, qi);
+  const int rb = NARROW ? kNarrowCols >> gs : block_rows(gs, waves);
   w.nqb = (w.n + rb - 1) / rb;
   w.r0 = (w.nqb - 1 - item % w.nqb) * rb;
   w.split = item / w.nqb;
@@ -128,7 +143,6 @@ __device__ __forceinline__ Work work_of(const AttnSharedParams& p, int qi) {
   const int tps = (r.count + w.splits - 1) / w.splits;
   w.i0 = min(r.count, w.split * tps);
   w.i1 = min(r.count, w.i0 + tps);
-  w.whole = !w.prefix && w.splits == 1 && p.prefix[w.seq] < 0;
   w.table = p.block_tables + (size_t)w.seq * p.table_stride;
   return w;
 }
@@ -139,46 +153,88 @@ struct RowPos {
   int row, pos;
 };
 __device__ __forceinline__ RowPos row_of(const AttnSharedParams& p, const Work& w, int r) {
-  RowPos x{w.row0 + r, w.p0 + r};
-  if (w.prefix) {
-    // members' rows one after the other, row `at` of them
-    const int at = w.row0 + w.r0 + r;
-    int before = w.row0;
-    for (int b = w.first; b < w.end; ++b) {
-      const int upto = p.member_end[b];
-      if (at >= before && at < upto) {
-        x.row = (b ? p.row_end[max(b - 1, 0)] : 0) + at - before;
-        x.pos = p.start[b] + at - before;
-      }
-      before = upto;
-    }
-  }
-  return x;
+  if (!w.prefix) return RowPos{w.row0 + r, w.p0 + r};
+  // members' rows one after the other, row `at` of them all: the first sequence b with member_end > at
+  const int lane = threadIdx.x & 63;
+  const int member_end = lane < p.n_seqs ? p.member_end[lane] : INT32_MAX, row_end = p.row_end[lane],
+            start = p.start[lane];
+  const int at = w.row0 + w.r0 + r;
+  int b = 0;
+#pragma unroll
+  for (int s = 32; s; s >>= 1) b += __shfl(member_end, b + s - 1, 64) <= at ? s : 0;
+  const int m = __shfl(member_end, max(b - 1, 0), 64), e = __shfl(row_end, max(b - 1, 0), 64);
+  const int before = b ? m : 0, rows = b ? e : 0;
+  return RowPos{rows + at - before, __shfl(start, b, 64) + at - before};
 }
 
-template <int QI>
-struct Columns : ColumnState<QI> {
-  using ColumnState<QI>::q, ColumnState<QI>::pos, ColumnState<QI>::o, ColumnState<QI>::m, ColumnState<QI>::l;
-  int least, most;  // of the wave's positions
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
-  // Columns past the rows repeat the last row.  PERM: Q's dims in the order in which the narrow form
-  // takes 8-bit keys.
-  template <bool PERM>
+// 32 values q as two e4m3 operands: q 2^-e = c1 + 2^-4 c2 with c1 the nearest codes (4 bits of the 8 that a bf16
+// has) and c2 those of what is left (the others).  Values of at least 2^-15 of the column's largest are exact, smaller
+// ones off by at most 2^-22 of it: as much as the fp32 sums of their products.
+struct Query8 {
+  i32x8_t c1, c2;
+  int e1, e2;  // the exponents' bytes
+  // w: the lane's 32 values; a column's 128 are in lanes 16 apart
+  __device__ __forceinline__ void set(const u32x4_t (&w)[4]) {
+    float v[32];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t x = w[i >> 2][i & 3];
+      v[2 * i] = bf_lo(x), v[2 * i + 1] = bf_hi(x);
+      top = max(top, max(__float_as_uint(v[2 * i]) & 0x7FFFFFFFu, __float_as_uint(v[2 * i + 1]) & 0x7FFFFFFFu));
+    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    const bool bad = top >= 0x7F800000u;  // an infinity or a NaN: the column's scores become NaN
+    e1 = bad ? 127 : scale_byte(top);
+    e2 = e1 - 4;
+    const float inv = __uint_as_float((uint32_t)(254 - e1) << 23);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float r[4];
+      int a = 0, b = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = v[4 * i + j] * inv;
+      a = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], a, false);
+      a = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], a, true);
+      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
+      b = __builtin_amdgcn_cvt_pk_fp8_f32((r[0] - lo[0]) * 16.f, (r[1] - lo[1]) * 16.f, b, false);
+      b = __builtin_amdgcn_cvt_pk_fp8_f32((r[2] - hi[0]) * 16.f, (r[3] - hi[1]) * 16.f, b, true);
+      c1[i] = bad ? 0x7F7F7F7F : a;
+      c2[i] = bad ? 0x7F7F7F7F : b;
+    }
+  }
+};
+
+template <bool F8>
+struct Columns : ColumnState<1> {
+  Query8 q8;
+  int least, most;  // of the wave's positions
+  u32x4_t raw[4];
+
+  // Columns past the rows repeat the last row.  8-bit operands: a lane has the dims 64 j + 16 G .. +16, j 0 and
+  // 1, of a row (which 32 is free, as long as keys and queries agree).
   __device__ __forceinline__ void load(const AttnSharedParams& p, const Work& w, int col0) {
     const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3, gs = p.group_shift;
-    int lo = INT32_MAX, hi = 0;
+    const int col = col0 + fr;
+    const RowPos x = row_of(p, w, min(col >> gs, w.nr - 1));
+    pos[0] = x.pos;
+    const size_t at = ((size_t)x.row << gs << 3) + ((size_t)w.g << gs) + (col & ((1 << gs) - 1));
+    const u32x4_t* row = reinterpret_cast<const u32x4_t*>(p.q + at * kHeadDim);
 #pragma unroll
-    for (int qi = 0; qi < QI; ++qi) {
-      const int col = col0 + 16 * qi + fr;
-      const RowPos x = row_of(p, w, min(col >> gs, w.nr - 1));
-      pos[qi] = x.pos;
-      const size_t at = ((size_t)x.row << gs << 3) + ((size_t)w.g << gs) + (col & ((1 << gs) - 1));
-      const u32x4_t* row = reinterpret_cast<const u32x4_t*>(p.q + at * kHeadDim);
+    for (int ks = 0; ks < 4; ++ks) raw[ks] = row[F8 ? 8 * (ks >> 1) + 2 * G + (ks & 1) : 4 * ks + G];
+    clear();
+  }
+  __device__ __forceinline__ void set() {
+    if constexpr (F8) {
+      q8.set(raw);
+    } else {
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        q[qi][ks] = __builtin_bit_cast(bf16x8_t, row[PERM ? 8 * (ks >> 1) + 2 * G + (ks & 1) : 4 * ks + G]);
-      lo = min(lo, x.pos), hi = max(hi, x.pos);
+      for (int ks = 0; ks < 4; ++ks) q[0][ks] = __builtin_bit_cast(bf16x8_t, raw[ks]);
     }
+    int lo = pos[0], hi = pos[0];
 #pragma unroll
     for (int s = 1; s < 16; s <<= 1) {
       lo = min(lo, __shfl_xor(lo, s, 64));
@@ -186,12 +242,18 @@ struct Columns : ColumnState<QI> {
     }
     least = __builtin_amdgcn_readfirstlane(lo);
     most = __builtin_amdgcn_readfirstlane(hi);
-    this->clear();
-    // The compiler does not see what the kernels' own waits cover: without one here it would guard the
-    // fragments inside their loops, where that is a wait for the tile in flight.
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   }
 };
+
+// The scores of 16 keys' codes, whose scales are in byte KB of `scales` (a lane's for its row of the operand).
+template <int KB>
+__device__ __forceinline__ f32x4_t scores8(const Query8& q, const u32x4_t& a0, const u32x4_t& a1, uint32_t scales) {
+  const u32x4_t both[2] = {a0, a1};
+  const i32x8_t a = __builtin_bit_cast(i32x8_t, both);
+  f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.c2, s, 0, 0, KB, (int)scales, 0, q.e2);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.c1, s, 0, 0, KB, (int)scales, 0, q.e1);
+}
 
 // Device-scope stores and loads: what one workgroup hands to another within a launch.
 __device__ __forceinline__ void agent_store2(float* p, float a, float b) {
@@ -243,17 +305,15 @@ __device__ __forceinline__ void chunks_of(u32x4_t (&c)[2], const u32x4_t& w, flo
 }
 
 // ---------------------------------------------------------------- narrow form
-// A wave's K tile as operands: lane (fr, G) holds of the rows fr + 16 kb (kb 0 .. 3) the dims
-// 32 ks + 8 G .. +8 (bf16), or the 16 codes from 64 j + 16 G on, j 0 and 1: two operands.
+// A wave's K tile as operands: lane (fr, G) holds of the rows fr + 16 kb (kb 0 .. 3) the dims 32 ks + 8 G .. +8 (bf16),
+// or the codes 64 j + 16 G .. +16, j 0 and 1.
 template <bool F8, int AUX>
 struct NarrowK {
   static constexpr int kLoads = F8 ? 2 : 4;
   u32x4_t w[4][kLoads];
-  uint32_t scales;
-  int rows;
+  uint32_t scales;  // (of a row that is not there anything, its codes are zero: no row sees it)
   __device__ __forceinline__ void issue(const Planes& x, int g) {
     const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3;
-    rows = x.rows;
     const int off = fr * (F8 ? kHeadDim : kRowBytes) + 16 * G;
     if constexpr (F8)
       scales = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * fr, g * kPagePos, AUX);
@@ -264,23 +324,16 @@ struct NarrowK {
         w[kb][j] = __builtin_amdgcn_raw_buffer_load_b128(
             x.k, off + kb * 16 * (F8 ? kHeadDim : kRowBytes) + 64 * j, 0, AUX);
   }
-  __device__ __forceinline__ void scores(f32x4_t (&s)[1][4], const ColumnState<1>& c) const {
-    const int fr = threadIdx.x & 15;
+  __device__ __forceinline__ void scores(f32x4_t (&s)[1][4], const Columns<F8>& c) const {
+    if constexpr (F8) {
+      s[0][0] = scores8<0>(c.q8, w[0][0], w[0][1], scales);
+      s[0][1] = scores8<1>(c.q8, w[1][0], w[1][1], scales);
+      s[0][2] = scores8<2>(c.q8, w[2][0], w[2][1], scales);
+      s[0][3] = scores8<3>(c.q8, w[3][0], w[3][1], scales);
+    } else {
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-      s[0][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      if constexpr (F8) {
-        const float scale = scale_at_byte(scales, kb, 16 * kb + fr < rows);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          u32x4_t a[2];
-          chunks_of(a, w[kb][j], scale);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            s[0][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a[h]), c.q[0][2 * j + h],
-                                                               s[0][kb], 0, 0, 0);
-        }
-      } else {
+      for (int kb = 0; kb < 4; ++kb) {
+        s[0][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
           s[0][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w[kb][ks]), c.q[0][ks],
@@ -363,35 +416,49 @@ struct Joined {
   }
 };
 
-template <bool F8, int AUX>
-__device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Work& w, ColumnState<1>& c, int least,
-                                             int most, int wave, u32x4_t* tile) {
+// `meanwhile` runs while the first tile's loads are on their way.
+template <bool F8, int AUX, typename Do>
+__device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Work& w, Columns<F8>& c, int wave,
+                                             u32x4_t* tile, const Do& meanwhile) {
   NarrowK<F8, AUX> k;
   NarrowV<F8, AUX> v;
   const Frags f;
-  int i = w.i0 + wave;
-  int page = i < w.i1 ? w.table[w.tile(i)] : -1;
+  // The wave's tiles' pages, 64 at a time, a lane each: a load of each by itself would be waited for together with
+  // the tile in flight.
+  const int lane = threadIdx.x & 63;
+  int pages = -1;
+  const auto look_up = [&](int first) {
+    const int i = first + NN * lane;
+    pages = i < w.i1 ? w.table[w.tile(i)] : -1;
+  };
+  int i = w.i0 + wave, n = 0;
+  look_up(i);
+  c.load(p, w, 0);
+  int page = __builtin_amdgcn_readlane(pages, 0);
   {
     const Planes x = planes_of<F8>(p, w.g, page, w.nkeys - w.tile(i) * BKEY);
     k.issue(x, w.g);
     v.issue(x, w.g);
   }
+  c.set();
+  meanwhile();
 #pragma unroll 1
-  for (; i < w.i1; i += NW) {
+  for (; i < w.i1; i += NN) {
     const bool there = page >= 0 && page < p.n_pages;
     const int key0 = w.tile(i) * BKEY;
-    const Sight see = there ? sight(key0, least, most, p.window, p.n_sinks) : kNone;
-    page = i + NW < w.i1 ? w.table[w.tile(i + NW)] : -1;
+    const Sight see = there ? sight(key0, c.least, c.most, p.window, p.n_sinks) : kNone;
+    if ((++n & 63) == 0) look_up(i + NN);
+    page = __builtin_amdgcn_readlane(pages, n & 63);
     // (past the last tile nothing is read)
-    const Planes x = planes_of<F8>(p, w.g, page, w.nkeys - w.tile(i + NW) * BKEY);
+    const Planes x = planes_of<F8>(p, w.g, page, w.nkeys - w.tile(i + NN) * BKEY);
     f32x4_t s[1][4];
     bf16x8_t pb[1][2];
     k.scores(s, c);
     k.issue(x, w.g);
     if (see == kAll)
-      weights<false>(pb, c, s, key0, p.window, p.n_sinks);
+      weights_lazy<false>(pb, c, s, key0, p.window, p.n_sinks);
     else if (see == kSome)
-      weights<true>(pb, c, s, key0, p.window, p.n_sinks);
+      weights_lazy<true>(pb, c, s, key0, p.window, p.n_sinks);
     if (see != kNone) v.stage(tile);
     v.issue(x, w.g);
     // (the wave's own tile: the hardware does its LDS accesses in order; the compiler is held to it)
@@ -404,63 +471,116 @@ __device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Wo
   }
 }
 
+// Adds the partials of `count` splits to j: four values of o and (m, l) of each; AGENT: of workgroups of this launch.
+template <bool AGENT>
+__device__ __forceinline__ void add_splits(Joined& j, const AttnSharedParams& p, size_t slot0, size_t step, int count,
+                                           int d) {
+  for (int s0 = 0; s0 < count; s0 += 8) {
+    f32x4_t po[8];
+    float2 ml[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const size_t slot = slot0 + min(s0 + u, count - 1) * step;
+      const float *o = p.part + slot * kHeadDim + d, *m = p.part_ml + 2 * slot;
+      if constexpr (AGENT) {
+        ml[u] = agent_load2(m);
+        const float2 a = agent_load2(o), b = agent_load2(o + 2);
+        po[u] = f32x4_t{a.x, a.y, b.x, b.y};
+      } else {
+        ml[u] = *reinterpret_cast<const float2*>(m);
+        po[u] = *reinterpret_cast<const f32x4_t*>(o);
+      }
+    }
+    j.add(po, ml, count - s0);
+  }
+}
+
+// The partials of a row's prefix (written by an earlier launch), for row r of sequence b's: part `part` of `parts`.
+__device__ __forceinline__ void add_prefix(Joined& j, const AttnSharedParams& p, int b, int r, int h, int heads, int d,
+                                           int part, int parts) {
+  const int k = p.prefix[b];
+  if (k < 0) return;
+  const int first = p.p_first[k], before = first ? p.member_end[max(first - 1, 0)] : 0;
+  const int all = p.member_end[p.p_end[k] - 1] - before;
+  const int at = (b ? p.member_end[max(b - 1, 0)] : 0) - before + r;
+  const int each = (p.p_splits[k] + parts - 1) / parts, s0 = part * each;
+  const size_t step = (size_t)all * heads;
+  add_splits<false>(j, p, ((size_t)p.p_part0[k] + at) * heads + h + s0 * step, step, min(each, p.p_splits[k] - s0), d);
+}
+
+constexpr int kPrefixParts = 64 * NN / (2 * 32);  // (2 columns at least)
+
 template <bool F8>
 __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w, u32x4_t (*lds)[TC]) {
   __shared__ int s_last;
+  // the waves' sums, and those of the row's prefix in up to kPrefixParts parts
+  __shared__ float2 ml_of[NN + kPrefixParts][kNarrowCols];
+  __shared__ f32x4_t prefix_o[2 * 64 * NN];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tid = threadIdx.x, gs = p.group_shift, heads = kKVHeads << gs;
-  Columns<1> c;
-  c.template load<F8>(p, w, 0);
-  if (p.nt)
-    narrow_tiles<F8, 2>(p, w, c, c.least, c.most, wave, lds[wave]);
+  const int ncols = w.nr << gs;
+  // The first split takes the prefix's partials (of an earlier launch) along: a part of them a thread for each column
+  // and four values, up to two of those a thread.
+  const int parts = !w.with_prefix || w.split ? 0 : max(1, 64 * NN / (ncols * 32));
+  const auto take_prefix = [&] {
+    if (!parts) return;
+    for (int i = tid; i < parts * ncols * 32; i += 64 * NN) {
+      const int part = i / (ncols * 32), col = (i >> 5) - part * ncols, d = 4 * (i & 31);
+      Joined j;
+      add_prefix(j, p, w.seq, w.r0 + (col >> gs), (w.g << gs) + (col & ((1 << gs) - 1)), heads, d, part, parts);
+      prefix_o[i] = j.o;
+      if (d == 0) ml_of[NN + part][col] = make_float2(j.M, j.L);
+    }
+  };
+  Columns<F8> c;
+  if (p.nt && w.nqb == 1)
+    narrow_tiles<F8, 2>(p, w, c, wave, lds[wave], take_prefix);
   else
-    narrow_tiles<F8, 0>(p, w, c, c.least, c.most, wave, lds[wave]);
-  // the waves' sums side by side: [column][128], then (m, l)
+    narrow_tiles<F8, 0>(p, w, c, wave, lds[wave], take_prefix);
+  // the waves' sums side by side: [column][128], and (m, l); the 16-byte pieces of a column in an order of its own (16
+  // columns' meet no bank twice)
   {
     const int fr = tid & 15, G = tid >> 4 & 3;
-    float* mine = reinterpret_cast<float*>(lds[wave]);
+    f32x4_t* mine = reinterpret_cast<f32x4_t*>(lds[wave]) + fr * 32;
 #pragma unroll
-    for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4_t*>(mine + fr * kOutStride + 16 * db + 4 * G) = c.o[0][db];
-    if (G == 0) *reinterpret_cast<float2*>(mine + kNarrowCols * kOutStride + 2 * fr) = make_float2(c.m[0], c.l[0][0]);
+    for (int db = 0; db < 8; ++db) mine[(4 * db + G) ^ fr] = c.o[0][db];
+    if (G == 0) ml_of[wave][fr] = make_float2(c.m[0], c.l[0][0]);
   }
   __syncthreads();
-  const int ncols = w.nr << gs;
-  const bool join = p.join && !w.whole;
-  for (int i = tid; i < ncols * 32; i += 64 * NW) {
+  for (int i = tid; i < ncols * 32; i += 64 * NN) {
     const int col = i >> 5, d = 4 * (i & 31);
-    f32x4_t po[NW];
-    float2 ml[NW];
+    f32x4_t po[NN];
+    float2 ml[NN];
 #pragma unroll
-    for (int u = 0; u < NW; ++u) {
-      const float* from = reinterpret_cast<const float*>(lds[u]);
-      po[u] = *reinterpret_cast<const f32x4_t*>(from + col * kOutStride + d);
-      ml[u] = *reinterpret_cast<const float2*>(from + kNarrowCols * kOutStride + 2 * col);
+    for (int u = 0; u < NN; ++u) {
+      po[u] = reinterpret_cast<const f32x4_t*>(lds[u])[col * 32 + ((i & 31) ^ col)];
+      ml[u] = ml_of[u][col];
     }
-    Joined j;
-    j.add(po, ml, NW);
     const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
-    if (w.whole) {
+    Joined j;
+    j.add(po, ml, NN);
+    for (int k = 0; k < parts; ++k) {
+      const f32x4_t o[1] = {prefix_o[k * ncols * 32 + i]};
+      const float2 m[1] = {ml_of[NN + k][col]};
+      j.add(o, m, 1);
+    }
+    if (w.splits == 1) {
       j.write(p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim + d);
       continue;
     }
     const size_t slot = ((size_t)w.part0 + (size_t)w.split * w.n + w.r0 + r) * heads + h;
-    if (join) {
-      agent_store2(p.part + slot * kHeadDim + d, j.o[0], j.o[1]);
-      agent_store2(p.part + slot * kHeadDim + d + 2, j.o[2], j.o[3]);
-      if (d == 0) agent_store2(p.part_ml + 2 * slot, j.M, j.L);
-    } else {
-      *reinterpret_cast<f32x4_t*>(p.part + slot * kHeadDim + d) = j.o;
-      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(j.M, j.L);
-    }
+    agent_store2(p.part + slot * kHeadDim + d, j.o[0], j.o[1]);
+    agent_store2(p.part + slot * kHeadDim + d + 2, j.o[2], j.o[3]);
+    if (d == 0) agent_store2(p.part_ml + 2 * slot, j.M, j.L);
   }
-  if (!join) return;
-  // The last split of the (sequence, kv head) to arrive joins them, in the splits' order.  The word that
+  if (w.splits == 1) return;
+  // The last split of the block and kv head to arrive joins them, in the splits' order.  The word that
   // counts them is the caller's memory, which may hold anything: a count is one with this call's tag,
   // whatever else is there counts as none.  The last leaves 0.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the partials are there, before the arrival counts
   __syncthreads();
   if (tid == 0) {
-    unsigned long long* word = p.arrived + (size_t)w.seq * kKVHeads + w.g;
+    unsigned long long* word = p.arrived + ((size_t)w.seq * kNarrowBlocks + w.r0 / (kNarrowCols >> gs)) * kKVHeads + w.g;
     unsigned long long cur = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), next;
     do {
       next = cur >> 16 == p.tag ? cur + 1 : p.tag << 16 | 1;
@@ -472,75 +592,84 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
   }
   __syncthreads();
   if (!s_last) return;
-  for (int i = tid; i < ncols * 32; i += 64 * NW) {
+  for (int i = tid; i < ncols * 32; i += 64 * NN) {
     const int col = i >> 5, d = 4 * (i & 31);
     const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
-    const size_t slot0 = ((size_t)w.part0 + w.r0 + r) * heads + h, step = (size_t)w.n * heads;
     Joined j;
-    for (int s0 = 0; s0 < w.splits; s0 += 8) {
-      f32x4_t po[8];
-      float2 ml[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const size_t slot = slot0 + min(s0 + u, w.splits - 1) * step;
-        ml[u] = agent_load2(p.part_ml + 2 * slot);
-        const float2 a = agent_load2(p.part + slot * kHeadDim + d), b = agent_load2(p.part + slot * kHeadDim + d + 2);
-        po[u] = f32x4_t{a.x, a.y, b.x, b.y};
-      }
-      j.add(po, ml, w.splits - s0);
-    }
+    add_splits<true>(j, p, ((size_t)w.part0 + w.r0 + r) * heads + h, (size_t)w.n * heads, w.splits, d);
     j.write(p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim + d);
   }
 }
 
 // ---------------------------------------------------------------- wide form
-// A thread's part of an 8-bit tile: chunk t % 8 (16 codes) of rows t / 8 and t / 8 + 32, of K and V.
-struct Raw8 {
-  u32x4_t k[2], v[2];
-  uint32_t ks, vs;
+// K's codes in LDS: chunk c (16 codes) of row r at slot c ^ (r / 2 % 8) of its 8, so that 16 rows' reads of a chunk
+// column meet no bank twice.
+__device__ __forceinline__ int k8_slot(int r, int c) { return r * 8 + (c ^ ((r >> 1) & 7)); }
+
+// A thread's part of an 8-bit tile: of V chunk t % 8 of row t / 8 (and of the row 32 on, with 4 waves), which becomes
+// bf16 on the way to LDS; K goes there directly, 8 rows a wave's load.
+template <int NW>
+struct Wide8 {
+  static constexpr int kEach = 8 / NW;
+  u32x4_t v[kEach];
+  uint32_t vs;      // the scales of rows t / 8 % 16 + 16 i
+  uint32_t ks[2];   // those of K's rows fr + 16 i, of this tile and the next
   int rows;
   template <int AUX>
-  __device__ __forceinline__ void issue(const Planes& x, int g) {
-    const int t = threadIdx.x;
+  __device__ __forceinline__ void issue(u32x4_t* ktile, const Planes& x, int g, int wave) {
+    const int t = threadIdx.x, r = t >> 3;
     rows = x.rows;
-    // the scales of rows t / 8 % 16 + 16 i
-    ks = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (t >> 3 & 15), g * kPagePos, AUX);
-    vs = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (t >> 3 & 15), (kKVHeads + g) * kPagePos, AUX);
+    ks[0] = ks[1];
+    ks[1] = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (t & 15), g * kPagePos, AUX);
+    vs = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (r & 15), (kKVHeads + g) * kPagePos, AUX);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      k[i] = __builtin_amdgcn_raw_buffer_load_b128(x.k, 16 * t, 4096 * i, AUX);
-      v[i] = __builtin_amdgcn_raw_buffer_load_b128(x.v, 16 * t, 4096 * i, AUX);
+    for (int i = 0; i < kEach; ++i) {  // (the row 32 on has the same swizzle)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(x.k, (lds_void*)(ktile + (wave + NW * i) * 64), 16,
+                                               r * kHeadDim + (((t & 7) ^ ((r >> 1) & 7)) * 16), 32 * i * kHeadDim, 0,
+                                               AUX);
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(x.v, 16 * t, 32 * i * kHeadDim, AUX);
     }
   }
-  __device__ __forceinline__ void stage(u32x4_t* kt, u32x4_t* vt) const {
+  __device__ __forceinline__ void stage(u32x4_t* vt, int wave) const {
     const int t = threadIdx.x, c = 2 * (t & 7);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = (t >> 3) + 32 * i, byte = (t >> 7) + 2 * i;
+    for (int i = 0; i < kEach; ++i) {
+      const int r = (t >> 3) + 32 * i;
       u32x4_t x[2];
-      chunks_of(x, k[i], scale_at_byte(ks, byte, r < rows));
-      kt[kv_slot(r, c)] = x[0];
-      kt[kv_slot(r, c + 1)] = x[1];
-      chunks_of(x, v[i], scale_at_byte(vs, byte, r < rows));
+      chunks_of(x, v[i], scale_at_byte(vs, (wave >> 1) + 2 * i, r < rows));  // (8 rows a wave)
       vt[kv_slot(r, c)] = x[0];
       vt[kv_slot(r, c + 1)] = x[1];
     }
   }
 };
 
-template <bool F8, int QI>
-__device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u32x4_t (*lds)[TC]) {
-  constexpr int CW = 16 * QI;
+template <int KB>
+__device__ __forceinline__ f32x4_t scores8_of(const Query8& q, const u32x4_t* ktile, uint32_t scales) {
+  const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3;
+  const int at = k8_slot(fr, G);  // (16 rows on, the same swizzle)
+  return scores8<KB>(q, ktile[at + KB * 128], ktile[(at ^ 4) + KB * 128], scales);
+}
+
+template <bool F8, int NW>
+__device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u32x4_t* kt, u32x4_t* vt) {
+  constexpr int kStep = F8 ? TC / 2 : TC;  // from the first K tile to the second
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool idle = (wave * CW) >> p.group_shift >= w.nr;  // (no rows)
+  const bool idle = (wave * 16) >> p.group_shift >= w.nr;  // (no rows)
   const bool nt = p.nt && w.nqb == 1;
   const TileLoad<NW> ld(wave);
-  Raw8 raw;
-  auto issue = [&](u32x4_t* ks, u32x4_t* vs, int i, int page) {
-    const Planes x = planes_of<F8>(p, w.g, page, w.nkeys - w.tile(i) * BKEY);
+  Wide8<NW> raw;
+  raw.ks[1] = 0;
+  const auto planes = [&](int i, int page) { return planes_of<F8>(p, w.g, page, w.nkeys - w.tile(i) * BKEY); };
+  // (past the last tile there are no bytes)
+  const auto page_of = [&](int i) { return w.table[w.tile(min(i, w.i1 - 1))]; };
+  const auto checked = [&](int i, int page) { return i < w.i1 ? __builtin_amdgcn_readfirstlane(page) : -1; };
+  // 8 bits: K to LDS, V to registers; bf16: both to LDS.
+  const auto issue = [&](int i, int page) {
+    const Planes x = planes(i, page);
+    u32x4_t *ks = kt + (i & 1) * kStep, *vs = vt + (i & 1) * TC;
     if constexpr (F8) {
-      if (nt) raw.issue<2>(x, w.g);
-      else raw.issue<0>(x, w.g);
+      if (nt) raw.template issue<2>(ks, x, w.g, wave);
+      else raw.template issue<0>(ks, x, w.g, wave);
     } else if (nt) {
       issue_tile<NW, 2>(ks, x.k, ld);
       issue_tile<NW, 2>(vs, x.v, ld);
@@ -552,125 +681,125 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
   // page of the tile in flight, and of the one after it (loaded a step ahead)
   int page = -1, next = -1;
   if (w.i0 < w.i1) {
-    const int here = w.table[w.tile(w.i0)];
-    next = w.table[w.tile(min(w.i0 + 1, w.i1 - 1))];
-    page = __builtin_amdgcn_readfirstlane(here);
-    issue(lds[0], lds[1], w.i0, page);
+    const int here = page_of(w.i0);
+    next = page_of(w.i0 + 1);
+    page = checked(w.i0, here);
+    issue(w.i0, page);
   }
-  Columns<QI> c;
-  c.template load<false>(p, w, wave * CW);
+  Columns<F8> c;
+  c.load(p, w, wave * 16);
+  c.set();
+  // The compiler does not see what the kernel's own waits cover: without one here it would guard the
+  // fragments inside the loops, where that is a wait for the tile in flight.
+  if constexpr (!F8) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   const Frags f;
 
-  auto step = [&](int i, u32x4_t* kc, u32x4_t* vc, u32x4_t* kn, u32x4_t* vn) {
-    // 8 bits: tile i becomes bf16 in the buffers of tile i - 2, which every wave left before the last
-    // barrier.  Then tile i has landed and every wave is done with tile i - 1.
-    if constexpr (F8) {
-      raw.stage(kc, vc);
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    }
-    const bool there = page >= 0 && page < p.n_pages;
-    // tile i + 1 is issued unconditionally: past the last tile it has no bytes
-    page = i + 1 < w.i1 ? __builtin_amdgcn_readfirstlane(next) : -1;
-    issue(kn, vn, i + 1, page);
-    next = w.table[w.tile(min(i + 2, w.i1 - 1))];
-    const int key0 = w.tile(i) * BKEY;
-    const Sight see = there && !idle ? sight(key0, c.least, c.most, p.window, p.n_sinks) : kNone;
-    if (see == kNone) return;  // (wave-uniform)
-    f32x4_t s[QI][4];
-    bf16x8_t pb[QI][2];
-    scores(s, c, f, kc);
-    __builtin_amdgcn_sched_barrier(0);
-    if (see == kAll) {
-      weights<false>(pb, c, s, key0, p.window, p.n_sinks);
-      values<false>(c, pb, f, vc, key0, p.window, p.n_sinks);
-    } else {
-      weights<true>(pb, c, s, key0, p.window, p.n_sinks);
-      __builtin_amdgcn_sched_barrier(0);  // (no fragments held over the softmax: registers)
-      values<true>(c, pb, f, vc, key0, p.window, p.n_sinks);
-    }
+  // Tile i has landed and every wave is done with tile i - 1; tile i + 1 is on its way.  8 bits: tile i's V
+  // becomes bf16 in the buffer of tile i - 2, which every wave left before the last barrier.  (Making tile i + 1's after
+  // the barrier, a step ahead of its use, takes 4% longer: 8192 rows over 4096 keys 565 -> 588 us.)
+  auto arrive = [&](int i) {
+    if constexpr (F8) raw.stage(vt + (i & 1) * TC, wave);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    page = checked(i + 1, next);
+    issue(i + 1, page);
+    next = page_of(i + 2);
   };
-  for (int i = w.i0; i < w.i1; i += 2) {
-    step(i, lds[0], lds[1], lds[2], lds[3]);
-    if (i + 1 < w.i1) step(i + 1, lds[2], lds[3], lds[0], lds[1]);
+  auto tile_scores = [&](f32x4_t (&s)[1][4], int i) {
+    const u32x4_t* kc = kt + (i & 1) * kStep;
+    if constexpr (F8) {
+      s[0][0] = scores8_of<0>(c.q8, kc, raw.ks[0]);
+      s[0][1] = scores8_of<1>(c.q8, kc, raw.ks[0]);
+      s[0][2] = scores8_of<2>(c.q8, kc, raw.ks[0]);
+      s[0][3] = scores8_of<3>(c.q8, kc, raw.ks[0]);
+    } else {
+      scores(s, c, f, kc);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const auto see = [&](int i) {
+    return page >= 0 && page < p.n_pages ? sight(w.tile(i) * BKEY, c.least, c.most, p.window, p.n_sinks) : kNone;
+  };
+  // Tiles that all rows see in full, one after the other, in a loop of their own: with the other kinds in
+  // one body the compiler moves the sums between two sets of registers in each step.
+  if (idle)
+    for (int i = w.i0; i < w.i1; ++i) arrive(i);
+  for (int i = idle ? w.i1 : w.i0; i < w.i1;) {
+#pragma unroll 1
+    for (; i < w.i1 && see(i) == kAll; ++i) {
+      arrive(i);
+      f32x4_t s[1][4];
+      bf16x8_t pb[1][2];
+      tile_scores(s, i);
+      weights_lazy<false>(pb, c, s, 0, p.window, p.n_sinks);
+      values<false>(c, pb, f, vt + (i & 1) * TC, 0, p.window, p.n_sinks);
+    }
+    if (i == w.i1) break;
+    const bool some = see(i) == kSome;
+    arrive(i);
+    if (some) {
+      const int key0 = w.tile(i) * BKEY;
+      f32x4_t s[1][4];
+      bf16x8_t pb[1][2];
+      tile_scores(s, i);
+      weights_lazy<true>(pb, c, s, key0, p.window, p.n_sinks);
+      __builtin_amdgcn_sched_barrier(0);  // (no fragments held over the softmax: registers)
+      values<true>(c, pb, f, vt + (i & 1) * TC, key0, p.window, p.n_sinks);
+    }
+    ++i;
   }
 
   const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3, gs = p.group_shift;
   const int heads = kKVHeads << gs;
+  const int col = wave * 16 + fr, r = col >> gs;
+  if (r >= w.nr) return;
+  const int h = (w.g << gs) + (col & ((1 << gs) - 1));
+  if (!w.whole) {
+    const size_t slot = ((size_t)w.part0 + (size_t)w.split * w.n + w.r0 + r) * heads + h;
+    float* dst = p.part + slot * kHeadDim + 4 * G;
 #pragma unroll
-  for (int qi = 0; qi < QI; ++qi) {
-    const int col = wave * CW + 16 * qi + fr, r = col >> gs;
-    if (r >= w.nr) continue;
-    const int h = (w.g << gs) + (col & ((1 << gs) - 1));
-    if (!w.whole) {
-      const size_t slot = ((size_t)w.part0 + (size_t)w.split * w.n + w.r0 + r) * heads + h;
-      float* dst = p.part + slot * kHeadDim + 4 * G;
+    for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4_t*>(dst + 16 * db) = c.o[0][db];
+    if (G == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(c.m[0], c.l[0][0]);
+  } else {
+    const float inv = c.l[0][0] == 0.f ? 0.f : 1.0f / c.l[0][0];
+    uint16_t* dst = p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim;
 #pragma unroll
-      for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4_t*>(dst + 16 * db) = c.o[qi][db];
-      if (G == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(c.m[qi], c.l[qi][0]);
-    } else {
-      const float inv = c.l[qi][0] == 0.f ? 0.f : 1.0f / c.l[qi][0];
-      uint16_t* dst = p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim;
-#pragma unroll
-      for (int db = 0; db < 8; ++db) {
-        const u32x2_t v = {pack_bf2(c.o[qi][db][0] * inv, c.o[qi][db][1] * inv),
-                           pack_bf2(c.o[qi][db][2] * inv, c.o[qi][db][3] * inv)};
-        *reinterpret_cast<u32x2_t*>(dst + db * 16 + 4 * G) = v;
-      }
+    for (int db = 0; db < 8; ++db) {
+      const u32x2_t v = {pack_bf2(c.o[0][db][0] * inv, c.o[0][db][1] * inv),
+                         pack_bf2(c.o[0][db][2] * inv, c.o[0][db][3] * inv)};
+      *reinterpret_cast<u32x2_t*>(dst + db * 16 + 4 * G) = v;
     }
   }
 }
 
-template <bool F8, int QI>
-__global__ __launch_bounds__(64 * NW, 2) void attn_shared_kernel(AttnSharedParams p) {
-  __shared__ u32x4_t lds[4][TC];
-  const Work w = work_of(p, QI);
-  if ((w.n << p.group_shift) <= kNarrowCols)
-    narrow<F8>(p, w, lds);
-  else
-    wide<F8, QI>(p, w, lds);
+template <bool F8>
+__global__ __launch_bounds__(64 * NN, 2) void attn_shared_narrow_kernel(AttnSharedParams p) {
+  __shared__ u32x4_t lds[NN][TC];
+  narrow<F8>(p, work_of<true>(p, 1), lds);
 }
 
-// Joins the partials of each (row, q head) that has more than one: 32 lanes each, 4 dims a lane, the
-// prefix's splits first, then the row's own.
+// (8-bit pages: 48 KiB of LDS)
+template <bool F8, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : F8 ? 3 : 2) void attn_shared_wide_kernel(AttnSharedParams p) {
+  __shared__ u32x4_t kt[F8 ? TC : 2 * TC], vt[2 * TC];
+  wide<F8, NW>(p, work_of<false>(p, NW), kt, vt);
+}
+
+// Joins the splits of each (row, q head) that the wide form has cut: 32 lanes each, 4 dims a lane.
 __global__ __launch_bounds__(256) void attn_shared_merge_kernel(AttnSharedParams p) {
   const int lane = threadIdx.x & 63;
   const int row_end = p.row_end[lane];
   const int heads = kKVHeads << p.group_shift;
   const int row = blockIdx.x * 8 / heads;  // (8 heads a workgroup: heads is a multiple of 8)
   const int b = __popcll(__ballot(lane < p.n_seqs && row_end <= row));
-  const int k = p.prefix[b], splits = p.splits[b];
-  if (k < 0 && splits < 2) return;
+  const int splits = p.splits[b];
   const int row0 = b ? p.row_end[max(b - 1, 0)] : 0, n = p.row_end[b] - row0;
+  if (splits < 2 || is_narrow(n, p.group_shift, p.prefix[b] >= 0)) return;  // (members are)
   const int h = blockIdx.x * 8 % heads + (threadIdx.x >> 5), d = (threadIdx.x & 31) * 4;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   Joined j;
-  const auto add = [&](size_t slot0, size_t step, int count) {
-    for (int s0 = 0; s0 < count; s0 += 8) {
-      float2 v[8];
-      f32x4_t po[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const size_t slot = slot0 + min(s0 + u, count - 1) * step;
-        v[u] = ml[slot];
-        po[u] = *reinterpret_cast<const f32x4_t*>(p.part + slot * kHeadDim + d);
-      }
-      j.add(po, v, count - s0);
-    }
-  };
-  if (k >= 0) {
-    const int first = p.p_first[k], before = first ? p.member_end[max(first - 1, 0)] : 0;
-    const int all = p.member_end[p.p_end[k] - 1] - before;
-    const int at = (b ? p.member_end[max(b - 1, 0)] : 0) - before + row - row0;
-    add(((size_t)p.p_part0[k] + at) * heads + h, (size_t)all * heads, p.p_splits[k]);
-  }
-  add(((size_t)p.part0[b] + row - row0) * heads + h, (size_t)n * heads, splits);
+  add_splits<false>(j, p, ((size_t)p.part0[b] + row - row0) * heads + h, (size_t)n * heads, splits, d);
   j.write(p.out + ((size_t)row * heads + h) * kHeadDim + d);
 }
 
-// Sequences of up to this many columns share a prefix; others fill a block of the wide form by themselves.
-constexpr int kMemberCols = 64;
 constexpr int kMaxSplits = 64;
 
 // Rows of at most `rows` that share a prefix.
@@ -679,7 +808,8 @@ int members_of(int rows, int heads) { return std::min(rows, kMaxSeqs * std::max(
 // prefix's and an own partial of each row that shares.  It never falls with the rows.
 long long part_rows(int rows, int heads) { return (long long)std::min(rows, 64) * kMaxSplits + 2ll * members_of(rows, heads); }
 
-constexpr size_t kArrivedBytes = (size_t)kMaxSeqs * kKVHeads * sizeof(unsigned long long);
+static_assert(kMemberCols <= kNarrowBlocks * kNarrowCols);
+constexpr size_t kArrivedBytes = (size_t)kMaxSeqs * kNarrowBlocks * kKVHeads * sizeof(unsigned long long);
 
 // A call's tag of the arrival counts, 48 bits.
 unsigned long long next_tag() {
@@ -697,39 +827,34 @@ struct Segment {
   bool narrow;
 };
 
-// Columns a wave of the wide form; tiles a split of either form.
+// Waves of the wide form's workgroups; tiles a split of either form.
 struct Plan {
-  int qi, wide, narrow;
+  int waves, wide, narrow;
   int splits(const Segment& x) const {
     const int t = x.narrow ? narrow : wide;
     return std::clamp((x.tiles + t - 1) / t, 1, kMaxSplits);
   }
-  int blocks(const Segment& x, int gs) const {
-    const int rb = block_rows(x.n, gs, qi);
-    return (x.n + rb - 1) / rb;
-  }
 };
 
-Plan plan_of(const Segment* own, int n_own, const Segment* pre, int n_pre, const int* prefix, int gs, long long room) {
+Plan plan_of(const Segment* own, int n_own, const Segment* pre, int n_pre, int gs, long long room) {
   long long narrow = 0, wide = 0;
-  int longest = 1;
   const auto count = [&](const Segment& x) {
     if (!x.n) return;
-    if (x.narrow) narrow += x.tiles;
-    else wide += (long long)x.tiles * ((x.n << gs) + 63) / 64;
-    longest = std::max(longest, x.tiles);
+    if (x.narrow) narrow += (long long)x.tiles * (((x.n << gs) + kNarrowCols - 1) / kNarrowCols);
+    else wide += (long long)x.tiles * ((x.n << gs) + 127) / 128;
   };
   for (int b = 0; b < n_own; ++b) count(own[b]);
   for (int k = 0; k < n_pre; ++k) count(pre[k]);
-  Plan plan{1, 1, 4};
-  plan.narrow = (int)std::max(4ll, (narrow * kKVHeads + 511) / 512);
+  Plan plan{8, 1, 4};
+  // (cut only where that fills the chip once)
+  plan.narrow = (int)std::max(4ll, (narrow * kKVHeads + 383) / 384);
   plan.wide = (int)std::max(1ll, (wide * kKVHeads + 511) / 512);
   // (at one split a segment the partials fit)
   for (;;) {
     long long part = 0;
     for (int b = 0; b < n_own; ++b) {
       const int k = plan.splits(own[b]);
-      if (k > 1 || prefix[b] >= 0) part += (long long)own[b].n * k;
+      if (k > 1) part += (long long)own[b].n * k;
     }
     for (int k = 0; k < n_pre; ++k) part += (long long)pre[k].n * plan.splits(pre[k]);
     if (part <= room) return plan;
@@ -774,12 +899,11 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
   for (int k = 0; k < p.n_prefixes; ++k) {
     const int n = p.member_end[p.p_end[k] - 1] - (p.p_first[k] ? p.member_end[p.p_first[k] - 1] : 0);
     keys += p.p_blocks[k] * BKEY;
-    pre[k] = {n, run_of(p.p_start[k], p.p_blocks[k] * BKEY - 1, 0, p.p_blocks[k], p.window, p.n_sinks).count,
-              (n << gs) <= kNarrowCols};
+    pre[k] = {n, run_of(p.p_start[k], p.p_blocks[k] * BKEY - 1, 0, p.p_blocks[k], p.window, p.n_sinks).count, false};
   }
   for (int b = 0; b < s.n; ++b) {
-    const int n = s.n_new[b], rb = n ? block_rows(n, gs, 2) : 1, last = n ? (n - 1) / rb * rb : 0;
-    own[b] = {n, 0, (n << gs) <= kNarrowCols};
+    const int n = s.n_new[b], rb = block_rows(gs, 8), last = n ? (n - 1) / rb * rb : 0;
+    own[b] = {n, 0, is_narrow(n, gs, p.prefix[b] >= 0)};
     if (!n) continue;
     const auto tiles = [&](int r0) {
       return run_of(s.start[b] + r0, s.start[b] + std::min(r0 + rb, n) - 1, p.lo[b], kMaxLongCtx / BKEY, p.window,
@@ -787,44 +911,67 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     };
     own[b].tiles = std::max(tiles(0), last ? tiles(last) : 0);
   }
-  const Plan plan = plan_of(own, s.n, pre, p.n_prefixes, p.prefix, gs, part_rows(rows, heads));
+  const Plan plan = plan_of(own, s.n, pre, p.n_prefixes, gs, part_rows(rows, heads));
   // splits, items and partial rows, segment by segment
-  int items = 0, part = 0;
-  bool split_wide = false, split_any = false;
-  const auto place = [&](const Segment& x, bool alone, int& item_end, int& splits, int& part0) {
-    splits = plan.splits(x);
-    if (x.n) items += splits * plan.blocks(x, gs);
-    item_end = items;
-    part0 = part;
-    if (!x.n || (alone && splits == 1)) return;
-    part += x.n * splits;
-    split_any = true;
-    split_wide |= !x.narrow;
+  int wide = 0, narrow = 0, part = 0;
+  bool merge = false, tagged = false;
+  const auto wide_items = [&](int n, int splits) {
+    const int rb = block_rows(gs, plan.waves);
+    wide += splits * ((n + rb - 1) / rb);
   };
-  for (int k = 0; k < p.n_prefixes; ++k) place(pre[k], false, p.p_item_end[k], p.p_splits[k], p.p_part0[k]);
-  p.prefix_items = items;
-  items = 0;
-  for (int b = 0; b < s.n; ++b) place(own[b], p.prefix[b] < 0, p.item_end[b], p.splits[b], p.part0[b]);
-  items += p.prefix_items;
-  p.join = split_any && !split_wide && !p.n_prefixes;
+  for (int k = 0; k < p.n_prefixes; ++k) {
+    p.p_splits[k] = plan.splits(pre[k]);
+    p.p_part0[k] = part;
+    part += pre[k].n * p.p_splits[k];
+    wide_items(pre[k].n, p.p_splits[k]);
+    p.p_item_end[k] = wide;
+  }
+  p.prefix_items = wide;
+  for (int b = 0; b < s.n; ++b) {
+    const Segment& x = own[b];
+    const int splits = p.splits[b] = plan.splits(x);
+    p.part0[b] = part;
+    if (x.n && x.narrow) {
+      narrow += splits * (((x.n << gs) + kNarrowCols - 1) / kNarrowCols);
+      part += splits > 1 ? x.n * splits : 0;
+      tagged |= splits > 1;
+    } else if (x.n) {
+      wide_items(x.n, splits);
+      part += splits > 1 ? x.n * splits : 0;
+      merge |= splits > 1;
+    }
+    p.narrow_end[b] = narrow;
+    p.wide_end[b] = wide - p.prefix_items;
+  }
   // a batch whose keys of all layers exceed the 256 MB cache finds none of them there: such keys, where one
   // workgroup reads them, pass it by
   p.nt = keys > 2048;
   p.arrived = static_cast<unsigned long long*>(workspace);
-  p.tag = p.join ? next_tag() : 0;
+  p.tag = tagged ? next_tag() : 0;
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kArrivedBytes);
   p.part_ml = p.part + (size_t)part * heads * kHeadDim;
-  const dim3 grid(items * kKVHeads), block(64 * NW);
-  if (fp8 && plan.qi == 1)
-    hipLaunchKernelGGL((attn_shared_kernel<true, 1>), grid, block, 0, st, p);
-  else if (fp8)
-    hipLaunchKernelGGL((attn_shared_kernel<true, 2>), grid, block, 0, st, p);
-  else if (plan.qi == 1)
-    hipLaunchKernelGGL((attn_shared_kernel<false, 1>), grid, block, 0, st, p);
-  else
-    hipLaunchKernelGGL((attn_shared_kernel<false, 2>), grid, block, 0, st, p);
-  IE_CHECK_LAUNCH();
-  if (split_any && !p.join) {
+  if (wide) {
+    const dim3 grid(wide * kKVHeads), block(64 * plan.waves);
+    if (fp8 && plan.waves == 8)
+      hipLaunchKernelGGL((attn_shared_wide_kernel<true, 8>), grid, block, 0, st, p);
+    else if (fp8)
+      hipLaunchKernelGGL((attn_shared_wide_kernel<true, 4>), grid, block, 0, st, p);
+    else if (plan.waves == 8)
+      hipLaunchKernelGGL((attn_shared_wide_kernel<false, 8>), grid, block, 0, st, p);
+    else
+      hipLaunchKernelGGL((attn_shared_wide_kernel<false, 4>), grid, block, 0, st, p);
+    IE_CHECK_LAUNCH();
+  }
+  // (after the wide launch: it joins the prefixes' partials to its sequences' own)
+  if (narrow) {
+    const dim3 grid(narrow * kKVHeads), block(64 * NN);
+    if (fp8)
+      hipLaunchKernelGGL((attn_shared_narrow_kernel<true>), grid, block, 0, st, p);
+    else
+      hipLaunchKernelGGL((attn_shared_narrow_kernel<false>), grid, block, 0, st, p);
+    IE_CHECK_LAUNCH();
+  }
+  if (merge) {
     hipLaunchKernelGGL(attn_shared_merge_kernel, dim3(rows << gs), dim3(256), 0, st, p);
     IE_CHECK_LAUNCH();
   }

@@ -24,6 +24,7 @@
 // does it; 8-bit tiles pass through registers, where they become bf16.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <random>
 
 #include "ie_attn_tiles.h"
@@ -112,6 +113,7 @@ __device__ __forceinline__ Work work_of(const AttnSharedParams& p, int waves) {
     pmax = w.nkeys - 1;
   } else {
     item -= NARROW ? 0 : p.prefix_items;
+    if constexpr (NARROW) item -= p.wide_items;
     const int item_end = NARROW ? p.narrow_end[lane] : p.wide_end[lane], row_end = p.row_end[lane],
               starts = p.start[lane], splits = p.splits[lane], part0 = p.part0[lane], los = p.lo[lane],
               prefixes = p.prefix[lane];
@@ -416,10 +418,9 @@ struct Joined {
   }
 };
 
-// `meanwhile` runs while the first tile's loads are on their way.
-template <bool F8, int AUX, typename Do>
+template <bool F8, int AUX>
 __device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Work& w, Columns<F8>& c, int wave,
-                                             u32x4_t* tile, const Do& meanwhile) {
+                                             u32x4_t* tile) {
   NarrowK<F8, AUX> k;
   NarrowV<F8, AUX> v;
   const Frags f;
@@ -441,7 +442,6 @@ __device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Wo
     v.issue(x, w.g);
   }
   c.set();
-  meanwhile();
 #pragma unroll 1
   for (; i < w.i1; i += NN) {
     const bool there = page >= 0 && page < p.n_pages;
@@ -495,48 +495,18 @@ __device__ __forceinline__ void add_splits(Joined& j, const AttnSharedParams& p,
   }
 }
 
-// The partials of a row's prefix (written by an earlier launch), for row r of sequence b's: part `part` of `parts`.
-__device__ __forceinline__ void add_prefix(Joined& j, const AttnSharedParams& p, int b, int r, int h, int heads, int d,
-                                           int part, int parts) {
-  const int k = p.prefix[b];
-  if (k < 0) return;
-  const int first = p.p_first[k], before = first ? p.member_end[max(first - 1, 0)] : 0;
-  const int all = p.member_end[p.p_end[k] - 1] - before;
-  const int at = (b ? p.member_end[max(b - 1, 0)] : 0) - before + r;
-  const int each = (p.p_splits[k] + parts - 1) / parts, s0 = part * each;
-  const size_t step = (size_t)all * heads;
-  add_splits<false>(j, p, ((size_t)p.p_part0[k] + at) * heads + h + s0 * step, step, min(each, p.p_splits[k] - s0), d);
-}
-
-constexpr int kPrefixParts = 64 * NN / (2 * 32);  // (2 columns at least)
-
 template <bool F8>
 __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w, u32x4_t (*lds)[TC]) {
   __shared__ int s_last;
-  // the waves' sums, and those of the row's prefix in up to kPrefixParts parts
-  __shared__ float2 ml_of[NN + kPrefixParts][kNarrowCols];
-  __shared__ f32x4_t prefix_o[2 * 64 * NN];
+  __shared__ float2 ml_of[NN][kNarrowCols];  // (m, l) of the waves' columns, then of parts of the splits
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tid = threadIdx.x, gs = p.group_shift, heads = kKVHeads << gs;
   const int ncols = w.nr << gs;
-  // The first split takes the prefix's partials (of an earlier launch) along: a part of them a thread for each column
-  // and four values, up to two of those a thread.
-  const int parts = !w.with_prefix || w.split ? 0 : max(1, 64 * NN / (ncols * 32));
-  const auto take_prefix = [&] {
-    if (!parts) return;
-    for (int i = tid; i < parts * ncols * 32; i += 64 * NN) {
-      const int part = i / (ncols * 32), col = (i >> 5) - part * ncols, d = 4 * (i & 31);
-      Joined j;
-      add_prefix(j, p, w.seq, w.r0 + (col >> gs), (w.g << gs) + (col & ((1 << gs) - 1)), heads, d, part, parts);
-      prefix_o[i] = j.o;
-      if (d == 0) ml_of[NN + part][col] = make_float2(j.M, j.L);
-    }
-  };
   Columns<F8> c;
   if (p.nt && w.nqb == 1)
-    narrow_tiles<F8, 2>(p, w, c, wave, lds[wave], take_prefix);
+    narrow_tiles<F8, 2>(p, w, c, wave, lds[wave]);
   else
-    narrow_tiles<F8, 0>(p, w, c, wave, lds[wave], take_prefix);
+    narrow_tiles<F8, 0>(p, w, c, wave, lds[wave]);
   // the waves' sums side by side: [column][128], and (m, l); the 16-byte pieces of a column in an order of its own (16
   // columns' meet no bank twice)
   {
@@ -559,21 +529,21 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
     const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
     Joined j;
     j.add(po, ml, NN);
-    for (int k = 0; k < parts; ++k) {
-      const f32x4_t o[1] = {prefix_o[k * ncols * 32 + i]};
-      const float2 m[1] = {ml_of[NN + k][col]};
-      j.add(o, m, 1);
-    }
-    if (w.splits == 1) {
+    if (w.whole) {
       j.write(p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim + d);
       continue;
     }
     const size_t slot = ((size_t)w.part0 + (size_t)w.split * w.n + w.r0 + r) * heads + h;
+    if (w.with_prefix) {  // (joined by a launch of its own)
+      *reinterpret_cast<f32x4_t*>(p.part + slot * kHeadDim + d) = j.o;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(j.M, j.L);
+      continue;
+    }
     agent_store2(p.part + slot * kHeadDim + d, j.o[0], j.o[1]);
     agent_store2(p.part + slot * kHeadDim + d + 2, j.o[2], j.o[3]);
     if (d == 0) agent_store2(p.part_ml + 2 * slot, j.M, j.L);
   }
-  if (w.splits == 1) return;
+  if (w.whole || w.with_prefix) return;
   // The last split of the block and kv head to arrive joins them, in the splits' order.  The word that
   // counts them is the caller's memory, which may hold anything: a count is one with this call's tag,
   // whatever else is there counts as none.  The last leaves 0.
@@ -581,22 +551,46 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
   __syncthreads();
   if (tid == 0) {
     unsigned long long* word = p.arrived + ((size_t)w.seq * kNarrowBlocks + w.r0 / (kNarrowCols >> gs)) * kKVHeads + w.g;
-    unsigned long long cur = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), next;
-    do {
-      next = cur >> 16 == p.tag ? cur + 1 : p.tag << 16 | 1;
-    } while (!__hip_atomic_compare_exchange_strong(word, &cur, next, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                                                   __HIP_MEMORY_SCOPE_AGENT));
+    unsigned long long cur = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), next = 0;
+    // (without this call's tag: the first to put it there counts one; with it, it stays until the last)
+    while (cur >> 16 != p.tag && !next)
+      if (__hip_atomic_compare_exchange_strong(word, &cur, p.tag << 16 | 1, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_AGENT))
+        next = p.tag << 16 | 1;
+    if (!next) next = __hip_atomic_fetch_add(word, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
     const bool last = (int)(next & 0xFFFF) == w.splits;
     if (last) __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s_last = last;
   }
   __syncthreads();
   if (!s_last) return;
-  for (int i = tid; i < ncols * 32; i += 64 * NN) {
+  // few columns: several threads a (column, four values), a part of the splits each, joined through LDS
+  const int pairs = ncols * 32, parts = max(1, 64 * NN / pairs), each = (w.splits + parts - 1) / parts;
+  f32x4_t* part_o = reinterpret_cast<f32x4_t*>(lds[0]);
+  for (int i = tid; i < parts * pairs; i += 64 * NN) {
+    const int part = i / pairs, col = (i - part * pairs) >> 5, d = 4 * (i & 31);
+    const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
+    const size_t step = (size_t)w.n * heads, slot0 = ((size_t)w.part0 + w.r0 + r) * heads + h;
+    Joined j;
+    add_splits<true>(j, p, slot0 + part * each * step, step, min(each, w.splits - part * each), d);
+    if (parts == 1) {
+      j.write(p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim + d);
+    } else {
+      part_o[i] = j.o;
+      if (d == 0) ml_of[0][part * ncols + col] = make_float2(j.M, j.L);
+    }
+  }
+  if (parts == 1) return;
+  __syncthreads();
+  for (int i = tid; i < pairs; i += 64 * NN) {
     const int col = i >> 5, d = 4 * (i & 31);
     const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
     Joined j;
-    add_splits<true>(j, p, ((size_t)w.part0 + w.r0 + r) * heads + h, (size_t)w.n * heads, w.splits, d);
+    for (int k = 0; k < parts; ++k) {
+      const f32x4_t o[1] = {part_o[k * pairs + i]};
+      const float2 ml[1] = {ml_of[0][k * ncols + col]};
+      j.add(o, ml, 1);
+    }
     j.write(p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim + d);
   }
 }
@@ -777,6 +771,15 @@ __global__ __launch_bounds__(64 * NN, 2) void attn_shared_narrow_kernel(AttnShar
   narrow<F8>(p, work_of<true>(p, 1), lds);
 }
 
+template <bool F8>
+__global__ __launch_bounds__(64 * NN, 2) void attn_shared_both_kernel(AttnSharedParams p) {
+  __shared__ u32x4_t lds[NN][TC];
+  if ((int)(blockIdx.x / kKVHeads) < p.wide_items)
+    wide<F8, NN>(p, work_of<false>(p, NN), lds[0], lds[2]);
+  else
+    narrow<F8>(p, work_of<true>(p, 1), lds);
+}
+
 // (8-bit pages: 48 KiB of LDS)
 template <bool F8, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : F8 ? 3 : 2) void attn_shared_wide_kernel(AttnSharedParams p) {
@@ -784,19 +787,30 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : F8 ? 3 : 2) void attn_shared
   wide<F8, NW>(p, work_of<false>(p, NW), kt, vt);
 }
 
-// Joins the splits of each (row, q head) that the wide form has cut: 32 lanes each, 4 dims a lane.
+// Joins the partials of each (row, q head) that has more than one, but for those that the narrow form has joined: 32
+// lanes each, 4 dims a lane, the prefix's splits first, then the row's own.
 __global__ __launch_bounds__(256) void attn_shared_merge_kernel(AttnSharedParams p) {
   const int lane = threadIdx.x & 63;
-  const int row_end = p.row_end[lane];
+  const int row_end = p.row_end[lane], member_end = p.member_end[lane], lane_splits = p.splits[lane],
+            part0 = p.part0[lane], prefix = p.prefix[lane];
   const int heads = kKVHeads << p.group_shift;
   const int row = blockIdx.x * 8 / heads;  // (8 heads a workgroup: heads is a multiple of 8)
-  const int b = __popcll(__ballot(lane < p.n_seqs && row_end <= row));
-  const int splits = p.splits[b];
-  const int row0 = b ? p.row_end[max(b - 1, 0)] : 0, n = p.row_end[b] - row0;
-  if (splits < 2 || is_narrow(n, p.group_shift, p.prefix[b] >= 0)) return;  // (members are)
+  const int b = __popcll(__ballot(lane < p.n_seqs && row_end <= row)), before = max(b - 1, 0);
+  const int k = __builtin_amdgcn_readlane(prefix, b), splits = __builtin_amdgcn_readlane(lane_splits, b);
+  const int row0 = b ? __builtin_amdgcn_readlane(row_end, before) : 0;
+  const int n = __builtin_amdgcn_readlane(row_end, b) - row0;
+  if (k < 0 && (splits < 2 || is_narrow(n, p.group_shift, false))) return;
   const int h = blockIdx.x * 8 % heads + (threadIdx.x >> 5), d = (threadIdx.x & 31) * 4;
   Joined j;
-  add_splits<false>(j, p, ((size_t)p.part0[b] + row - row0) * heads + h, (size_t)n * heads, splits, d);
+  if (k >= 0) {
+    const int first = p.p_first[k], end = p.p_end[k], p_splits = p.p_splits[k], p_part0 = p.p_part0[k];
+    const int base = first ? __builtin_amdgcn_readlane(member_end, max(first - 1, 0)) : 0;
+    const int all = __builtin_amdgcn_readlane(member_end, end - 1) - base;
+    const int at = (b ? __builtin_amdgcn_readlane(member_end, before) : 0) - base + row - row0;
+    add_splits<false>(j, p, ((size_t)p_part0 + at) * heads + h, (size_t)all * heads, p_splits, d);
+  }
+  add_splits<false>(j, p, ((size_t)__builtin_amdgcn_readlane(part0, b) + row - row0) * heads + h, (size_t)n * heads,
+                    splits, d);
   j.write(p.out + ((size_t)row * heads + h) * kHeadDim + d);
 }
 
@@ -824,41 +838,114 @@ unsigned long long next_tag() {
 // A segment as the plan sees it.
 struct Segment {
   int n, tiles;  // rows; tiles of its longest row block
-  bool narrow;
+  bool narrow, parts;  // its form; it leaves partials even where it is not cut
 };
 
-// Waves of the wide form's workgroups; tiles a split of either form.
+int blocks_of(const Segment& x, int gs, int columns) { return ((x.n << gs) + columns - 1) / columns; }
+
+// What is launched: `both` forms in one kernel (the wide one with 4 waves), or each in its own; the tiles a split of
+// either form.
 struct Plan {
+  bool both;
   int waves, wide, narrow;
   int splits(const Segment& x) const {
+    // (16 tiles, four a wave, take as long as the join of two halves does)
+    if (x.narrow && !x.parts && x.tiles <= 16) return 1;
     const int t = x.narrow ? narrow : wide;
     return std::clamp((x.tiles + t - 1) / t, 1, kMaxSplits);
   }
 };
 
-Plan plan_of(const Segment* own, int n_own, const Segment* pre, int n_pre, int gs, long long room) {
-  long long narrow = 0, wide = 0;
-  const auto count = [&](const Segment& x) {
-    if (!x.n) return;
-    if (x.narrow) narrow += (long long)x.tiles * (((x.n << gs) + kNarrowCols - 1) / kNarrowCols);
-    else wide += (long long)x.tiles * ((x.n << gs) + 127) / 128;
-  };
-  for (int b = 0; b < n_own; ++b) count(own[b]);
-  for (int k = 0; k < n_pre; ++k) count(pre[k]);
-  Plan plan{8, 1, 4};
-  // (cut only where that fills the chip once)
-  plan.narrow = (int)std::max(4ll, (narrow * kKVHeads + 383) / 384);
-  plan.wide = (int)std::max(1ll, (wide * kKVHeads + 511) / 512);
+// A form's time for a tile where 1, 2 or 3 workgroups share a CU (0: they do not fit), us.  Measured over 196 tiles
+// of 30 rows, 66 of 8192 rows and 67-126 of four sequences of 742-2500 rows (32 heads).
+struct Rate {
+  int waves;
+  double c[3];
+};
+constexpr Rate kRates[2][3] = {{{8, {1.92, 2.33, 0}}, {4, {1.75, 1.75, 0}}, {4, {1.75, 1.9, 0}}},    // bf16; the last:
+                               {{8, {1.35, 2.1, 0}}, {4, {1.16, 1.35, 1.79}}, {4, {1.2, 1.55, 0}}}};  // both forms
+
+// The time of `items` workgroups of `us` (at one a CU) each, by the rates' growth with their number.
+double turns(const Rate& r, double items, double us) {
+  const int most = r.c[2] > 0 ? 3 : 2;
+  const double rounds = items / (256 * most);
+  // (the longest come first, so that more than a round ends evenly)
+  if (rounds > 1) return us / r.c[0] * r.c[most - 1] * rounds + 0.25 * us;
+  return us / r.c[0] * r.c[items > 512 ? 2 : items > 256 ? 1 : 0];
+}
+
+// The launches with the least modelled time.  A workgroup starts and ends in 4 us and takes its tiles (1.5 more for the
+// masked ones of a run), a narrow one 1.25 for four; a launch more is 3, the join 4.5 and
+// 0.2 a split, its partials written and read at 5 TB/s.  Within 10% of the best of 12 split counts and both workgroup sizes over 13 batches of 1-2500 rows
+// (1 x 200 rows over 16000 keys 345 us uncut, 79-85 in 8; 2500 rows 72 uncut, 104 in two; 2 x 1000 over
+// 4096 keys 148 and 152), and of 8 counts over 10 batches with prefixes.
+Plan plan_of(const Segment* x, int n, bool prefixes, bool fp8, int gs, long long room) {
+  long long narrow = 0;
+  int wide_longest = 0, narrow_longest = 0, narrow_items = 0;
+  bool any_narrow = false;
+  const Segment* wide[kMaxPrefixes + kMaxSeqs];
+  int n_wide = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!x[i].n) continue;
+    if (x[i].narrow) {
+      narrow += (long long)x[i].tiles * blocks_of(x[i], gs, kNarrowCols);
+      narrow_longest = std::max(narrow_longest, x[i].tiles);
+      any_narrow = true;
+    } else {
+      wide_longest = std::max(wide_longest, x[i].tiles);
+      wide[n_wide++] = x + i;
+    }
+  }
+  Plan best{false, 8, 1, 4};
+  // narrow: a workgroup a CU, in whole rounds of its waves, two at least
+  best.narrow = NN * (int)std::max<long long>(2, (narrow * kKVHeads + 256 * NN - 1) / (256 * NN));
+  // (halves of unequal runs are no better than a run)
+  if (2 * narrow_longest <= 3 * best.narrow) best.narrow = std::max(narrow_longest, 1);
+  double narrow_us = 0;
+  if (any_narrow) {
+    for (int i = 0; i < n; ++i)
+      if (x[i].n && x[i].narrow) narrow_items += best.splits(x[i]) * blocks_of(x[i], gs, kNarrowCols) * kKVHeads;
+    narrow_us = 1.25 * ((std::min(best.narrow, narrow_longest) + NN - 1) / NN);
+  }
+  double least = 1e30;
+  for (int form = 0; form < 3 && wide_longest; ++form) {
+    const bool both = form == 2;
+    if (both && !any_narrow) continue;
+    const Rate& r = kRates[fp8][form];
+    int tried = 0;
+    for (const int k : {1, 2, 3, 4, 6, 8, 10, 12, 16, 20, 26, 32, 48, kMaxSplits}) {
+      Plan plan = best;
+      plan.both = both, plan.waves = r.waves, plan.wide = (wide_longest + k - 1) / k;
+      if (k > wide_longest || plan.wide == tried) continue;
+      tried = plan.wide;
+      double items = 0, tiles = 0, parts = 0;
+      int most = 1;  // splits
+      for (int i = 0; i < n_wide; ++i) {
+        const Segment& y = *wide[i];
+        const int s = plan.splits(y), b = blocks_of(y, gs, 16 * r.waves);
+        items += (double)s * b * kKVHeads;
+        tiles += (double)y.tiles * b * kKVHeads;
+        if (s > 1 || y.parts) parts += (double)y.n * s;
+        most = std::max(most, s);
+      }
+      const double each = 4 + (tiles / items + 1.5) * r.c[0];
+      double cost = std::max(both ? turns(r, items + narrow_items, (items * each + narrow_items * (4 + narrow_us)) / (items + narrow_items))
+                                  : turns(r, items, each),
+                             4 + (plan.wide + 1.5) * r.c[0]);
+      if (!both && any_narrow) cost += 3 + turns(kRates[fp8][2], narrow_items, 4 + narrow_us);
+      if (parts || prefixes) cost += 4.5 + 0.2 * most + parts * (kKVHeads << gs) * (kHeadDim + 2) * 4 * 2 / 5e6;
+      if (cost < least) least = cost, best = plan;
+    }
+  }
   // (at one split a segment the partials fit)
   for (;;) {
     long long part = 0;
-    for (int b = 0; b < n_own; ++b) {
-      const int k = plan.splits(own[b]);
-      if (k > 1) part += (long long)own[b].n * k;
+    for (int i = 0; i < n; ++i) {
+      const int k = best.splits(x[i]);
+      if (k > 1 || x[i].parts) part += (long long)x[i].n * k;
     }
-    for (int k = 0; k < n_pre; ++k) part += (long long)pre[k].n * plan.splits(pre[k]);
-    if (part <= room) return plan;
-    plan.wide *= 2, plan.narrow *= 2;
+    if (part <= room) return best;
+    best.wide *= 2, best.narrow *= 2;
   }
 }
 
@@ -887,7 +974,7 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     for (int b = b0; b < b1; ++b)
       if (s.n_new[b] && (s.n_new[b] << gs) <= kMemberCols) p.prefix[b] = k, p.lo[b] = blocks;
   }
-  Segment own[kMaxSeqs], pre[kMaxPrefixes];
+  Segment all[kMaxPrefixes + kMaxSeqs];  // the prefixes, then the sequences
   for (int b = 0; b < s.n; ++b) {
     const int n = s.n_new[b];
     p.start[b] = s.start[b];
@@ -896,14 +983,16 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     keys += std::min(s.start[b] + n - p.lo[b] * BKEY, p.window + p.n_sinks + n);
   }
   if (!rows) return IE_OK;
+  Segment* const pre = all;
+  Segment* const own = all + p.n_prefixes;
   for (int k = 0; k < p.n_prefixes; ++k) {
     const int n = p.member_end[p.p_end[k] - 1] - (p.p_first[k] ? p.member_end[p.p_first[k] - 1] : 0);
     keys += p.p_blocks[k] * BKEY;
-    pre[k] = {n, run_of(p.p_start[k], p.p_blocks[k] * BKEY - 1, 0, p.p_blocks[k], p.window, p.n_sinks).count, false};
+    pre[k] = {n, run_of(p.p_start[k], p.p_blocks[k] * BKEY - 1, 0, p.p_blocks[k], p.window, p.n_sinks).count, false, true};
   }
   for (int b = 0; b < s.n; ++b) {
     const int n = s.n_new[b], rb = block_rows(gs, 8), last = n ? (n - 1) / rb * rb : 0;
-    own[b] = {n, 0, is_narrow(n, gs, p.prefix[b] >= 0)};
+    own[b] = {n, 0, is_narrow(n, gs, p.prefix[b] >= 0), p.prefix[b] >= 0};
     if (!n) continue;
     const auto tiles = [&](int r0) {
       return run_of(s.start[b] + r0, s.start[b] + std::min(r0 + rb, n) - 1, p.lo[b], kMaxLongCtx / BKEY, p.window,
@@ -911,19 +1000,15 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     };
     own[b].tiles = std::max(tiles(0), last ? tiles(last) : 0);
   }
-  const Plan plan = plan_of(own, s.n, pre, p.n_prefixes, gs, part_rows(rows, heads));
+  const Plan plan = plan_of(all, p.n_prefixes + s.n, p.n_prefixes > 0, fp8, gs, part_rows(rows, heads));
   // splits, items and partial rows, segment by segment
   int wide = 0, narrow = 0, part = 0;
   bool merge = false, tagged = false;
-  const auto wide_items = [&](int n, int splits) {
-    const int rb = block_rows(gs, plan.waves);
-    wide += splits * ((n + rb - 1) / rb);
-  };
   for (int k = 0; k < p.n_prefixes; ++k) {
     p.p_splits[k] = plan.splits(pre[k]);
     p.p_part0[k] = part;
     part += pre[k].n * p.p_splits[k];
-    wide_items(pre[k].n, p.p_splits[k]);
+    wide += p.p_splits[k] * blocks_of(pre[k], gs, 16 * plan.waves);
     p.p_item_end[k] = wide;
   }
   p.prefix_items = wide;
@@ -932,11 +1017,12 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     const int splits = p.splits[b] = plan.splits(x);
     p.part0[b] = part;
     if (x.n && x.narrow) {
-      narrow += splits * (((x.n << gs) + kNarrowCols - 1) / kNarrowCols);
-      part += splits > 1 ? x.n * splits : 0;
+      narrow += splits * blocks_of(x, gs, kNarrowCols);
+      part += splits > 1 || x.parts ? x.n * splits : 0;
       tagged |= splits > 1;
+      merge |= x.parts;
     } else if (x.n) {
-      wide_items(x.n, splits);
+      wide += splits * blocks_of(x, gs, 16 * plan.waves);
       part += splits > 1 ? x.n * splits : 0;
       merge |= splits > 1;
     }
@@ -950,6 +1036,16 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
   p.tag = tagged ? next_tag() : 0;
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kArrivedBytes);
   p.part_ml = p.part + (size_t)part * heads * kHeadDim;
+  p.wide_items = plan.both ? wide : 0;
+  if (plan.both) {
+    const dim3 grid((wide + narrow) * kKVHeads), block(64 * NN);
+    if (fp8)
+      hipLaunchKernelGGL((attn_shared_both_kernel<true>), grid, block, 0, st, p);
+    else
+      hipLaunchKernelGGL((attn_shared_both_kernel<false>), grid, block, 0, st, p);
+    IE_CHECK_LAUNCH();
+    wide = narrow = 0;
+  }
   if (wide) {
     const dim3 grid(wide * kKVHeads), block(64 * plan.waves);
     if (fp8 && plan.waves == 8)
@@ -962,7 +1058,6 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
       hipLaunchKernelGGL((attn_shared_wide_kernel<false, 4>), grid, block, 0, st, p);
     IE_CHECK_LAUNCH();
   }
-  // (after the wide launch: it joins the prefixes' partials to its sequences' own)
   if (narrow) {
     const dim3 grid(narrow * kKVHeads), block(64 * NN);
     if (fp8)

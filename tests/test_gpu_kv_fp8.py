@@ -512,6 +512,25 @@ def test_attend_workspace_of_a_larger_batch(hip, ctx):
         check_attend(out, want, tol)
 
 
+@pytest.mark.parametrize("window,evicted", [(ALL, False), (16500, True)])
+def test_attend_long_runs_of_many_sequences(hip, ctx, window, evicted):
+    """More tiles a wave than it looks up at a time (64): 64 sequences of one table, uncut."""
+    say(f"attend, 8 bits: 64 sequences over 20000 keys, window {window}")
+    g = gen(22)
+    start, new = [20000 + 7 * i for i in range(64)], [1 + i % 2 for i in range(64)]
+    n_pages, row = make_tables(g, [max(start) + 2])
+    pool = make_pool8(g, n_pages)
+    if evicted:
+        row[0, 100:330:5] = -1
+    tables = row.repeat(64, 1)
+    q = bf16(g, sum(new), 16, D)
+    out = torch.empty_like(q)
+    attend8(hip, ctx, start, new, window, 70, 16, q, pool, tables, out)
+    torch.cuda.synchronize()
+    want, tol = attend64(start, new, window, 70, 16, q, bf16_pool(pool), tables)
+    check_attend(out, want, tol)
+
+
 @pytest.mark.parametrize("layer", [0, 31])
 def test_layers_and_pages_far_into_the_pool(hip, ctx, layer):
     """Pages past 2^32 bytes from the pool's start, the first and the last layer; other bytes NaN."""

@@ -167,7 +167,9 @@ __device__ __forceinline__ void weights_lazy(bf16x8_t (&pb)[QI][KB / 2], ColumnS
 #pragma unroll
     for (int qi = 0; qi < QI; ++qi) {
       const float nb = -fmaxf(mn[qi], -3.0e38f) * kScoreScale;
-      const float alpha = __builtin_amdgcn_exp2f(fmaf(c.m[qi], kScoreScale, nb));  // m = -inf: 0
+      // (m = -inf: 0; exactly 1 for a column that stays, whatever its neighbours do)
+      const float alpha =
+          mn[qi] != c.m[qi] ? __builtin_amdgcn_exp2f(fmaf(c.m[qi], kScoreScale, nb)) : 1.0f;
       c.m[qi] = mn[qi];
 #pragma unroll
       for (int db = 0; db < 8; ++db) c.o[qi][db] *= alpha;
@@ -195,9 +197,8 @@ __device__ __forceinline__ void weights_lazy(bf16x8_t (&pb)[QI][KB / 2], ColumnS
 
 // o += V^T . P^T and the sums, of 32 KS keys.  MASK: 0 x (an infinity or NaN) of a key that a column does not see must
 // stay 0: such values are kept out of the product and added to the columns that see them.
-// APART: the dims' products in groups of so many, whose fragments are not read before the group (0: as the
-// compiler likes).
-template <bool MASK, int APART = 0, int QI, int KS>
+// AHEAD: the fragments of so many groups of 16 dims are read ahead of their products (0: as the compiler likes).
+template <bool MASK, int AHEAD = 0, int QI, int KS>
 __device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[QI][KS], const Frags& f,
                                        const u32x4_t* vtile, int key0, int window, int n_sinks) {
   const u32x4_t ones_w = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
@@ -212,9 +213,6 @@ __device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[
 #pragma unroll
   for (int db = 0; db < 8; ++db) {
     if constexpr (MASK) __builtin_amdgcn_sched_barrier(0);  // (fewer fragments at once: registers)
-    if constexpr (!MASK && APART) {
-      if (db % APART == 0) __builtin_amdgcn_sched_barrier(0);
-    }
 #pragma unroll
     for (int ks2 = 0; ks2 < KS; ++ks2) {
       const char* va = vb8 + f.v(db) + ks2 * 8192;
@@ -234,6 +232,16 @@ __device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[
 #pragma unroll
       for (int qi = 0; qi < QI; ++qi)
         c.o[qi][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[qi][ks2], c.o[qi][db], 0, 0, 0);
+    }
+  }
+  if constexpr (!MASK && AHEAD > 0) {
+    // (0x100: LDS reads, 0x8: MFMAs; the sums' come first)
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * KS * AHEAD, 0);
+    __builtin_amdgcn_sched_group_barrier(0x8, QI * KS, 0);
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      if (db + AHEAD < 8) __builtin_amdgcn_sched_group_barrier(0x100, 2 * KS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, QI * KS, 0);
     }
   }
   if constexpr (MASK) {

@@ -367,8 +367,8 @@ struct AttnSharedParams {
   int start[kMaxSeqs], row_end[kMaxSeqs], member_end[kMaxSeqs];
   int narrow_end[kMaxSeqs], wide_end[kMaxSeqs], splits[kMaxSeqs], part0[kMaxSeqs];
   int lo[kMaxSeqs], prefix[kMaxSeqs];
-  // by prefix: items up to and with the prefix's; key splits; first partial row; first sequence and
-  // one past the last; shared blocks; the least first position
+  // by prefix: items up to and with the prefix's; key splits; first partial row; its first member and
+  // one past the group's last sequence; shared blocks; the least first position
   int p_item_end[kMaxPrefixes], p_splits[kMaxPrefixes], p_part0[kMaxPrefixes];
   int p_first[kMaxPrefixes], p_end[kMaxPrefixes], p_blocks[kMaxPrefixes], p_start[kMaxPrefixes];
 };

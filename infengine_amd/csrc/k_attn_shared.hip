@@ -24,8 +24,8 @@
 // does it; 8-bit tiles pass through registers, where they become bf16.
 #include <algorithm>
 #include <atomic>
+#include <chrono>
 #include <cmath>
-#include <random>
 
 #include "ie_attn_tiles.h"
 
@@ -77,7 +77,7 @@ constexpr int kMemberCols = 64;
 // A sequence's own keys go to the narrow form: up to 16 columns; and those of members (few beside the prefix's, and
 // joined to it by the narrow form), in blocks of 16.  A prefix never does.
 __host__ __device__ __forceinline__ bool is_narrow(int n, int gs, bool member) {
-  return (n << gs) <= (member ? kMemberCols : kNarrowCols);
+  return n <= (member ? kMemberCols : kNarrowCols) >> gs;
 }
 // Rows of a block of the wide form.
 __host__ __device__ __forceinline__ int block_rows(int gs, int waves) { return (16 * waves) >> gs; }
@@ -647,6 +647,7 @@ __device__ __forceinline__ f32x4_t scores8_of(const Query8& q, const u32x4_t* kt
 template <bool F8, int NW>
 __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u32x4_t* kt, u32x4_t* vt) {
   constexpr int kStep = F8 ? TC / 2 : TC;  // from the first K tile to the second
+  constexpr int kAhead = 2;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool idle = (wave * 16) >> p.group_shift >= w.nr;  // (no rows)
   const bool nt = p.nt && w.nqb == 1;
@@ -725,7 +726,7 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
       bf16x8_t pb[1][2];
       tile_scores(s, i);
       weights_lazy<false>(pb, c, s, 0, p.window, p.n_sinks);
-      values<false>(c, pb, f, vt + (i & 1) * TC, 0, p.window, p.n_sinks);
+      values<false, kAhead>(c, pb, f, vt + (i & 1) * TC, 0, p.window, p.n_sinks);
     }
     if (i == w.i1) break;
     const bool some = see(i) == kSome;
@@ -827,10 +828,10 @@ constexpr size_t kArrivedBytes = (size_t)kMaxSeqs * kNarrowBlocks * kKVHeads * s
 
 // A call's tag of the arrival counts, 48 bits.
 unsigned long long next_tag() {
-  static std::atomic<unsigned long long> n{[] {
-    std::random_device r;
-    return (unsigned long long)r() << 32 | r();
-  }()};
+  // (from a place of its own in each process)
+  static std::atomic<unsigned long long> n{
+      splitmix64((unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() ^
+                 splitmix64(reinterpret_cast<uintptr_t>(&n)))};
   const unsigned long long t = n.fetch_add(1, std::memory_order_relaxed) & ((1ull << 48) - 1);
   return t ? t : next_tag();
 }
@@ -841,7 +842,7 @@ struct Segment {
   bool narrow, parts;  // its form; it leaves partials even where it is not cut
 };
 
-int blocks_of(const Segment& x, int gs, int columns) { return ((x.n << gs) + columns - 1) / columns; }
+int blocks_of(const Segment& x, int gs, int columns) { return (x.n + (columns >> gs) - 1) / (columns >> gs); }
 
 // What is launched: `both` forms in one kernel (the wide one with 4 waves), or each in its own; the tiles a split of
 // either form.
@@ -965,14 +966,19 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
   // the prefixes: groups of two sequences at least that have few rows each
   for (int i = 0, b0 = 0; i < g.n; b0 += g.seqs[i++]) {
     const int b1 = b0 + g.seqs[i], blocks = g.shared[i] / BKEY;
-    int many = 0, least = kMaxLongCtx;
-    for (int b = b0; b < b1; ++b)
-      if (s.n_new[b] && (s.n_new[b] << gs) <= kMemberCols) ++many, least = std::min(least, s.start[b]);
+    const auto member = [&](int b) { return s.n_new[b] && s.n_new[b] <= kMemberCols >> gs; };
+    int many = 0, least = kMaxLongCtx, first = b0;
+    for (int b = b0; b < b1; ++b) {
+      if (!member(b)) continue;
+      if (!many++) first = b;
+      least = std::min(least, s.start[b]);
+    }
     if (!blocks || many < 2) continue;
     const int k = p.n_prefixes++;
-    p.p_first[k] = b0, p.p_end[k] = b1, p.p_blocks[k] = blocks, p.p_start[k] = least;
+    // (the first member's table row is read: one without new rows may be over, its pages gone)
+    p.p_first[k] = first, p.p_end[k] = b1, p.p_blocks[k] = blocks, p.p_start[k] = least;
     for (int b = b0; b < b1; ++b)
-      if (s.n_new[b] && (s.n_new[b] << gs) <= kMemberCols) p.prefix[b] = k, p.lo[b] = blocks;
+      if (member(b)) p.prefix[b] = k, p.lo[b] = blocks;
   }
   Segment all[kMaxPrefixes + kMaxSeqs];  // the prefixes, then the sequences
   for (int b = 0; b < s.n; ++b) {

@@ -451,6 +451,23 @@ def test_attend_nan_row_reaches_only_rows_that_see_it(hip, ctx, rows, at, part):
     assert torch.isnan(out[sees][:, 8:12]).all()
 
 
+@pytest.mark.parametrize("start,new", [([900], [8]), ([900], [100]), ([900], [2500]), ([3000] * 5, [1] * 5)])
+def test_attend_rows_do_not_depend_on_their_neighbours(hip, ctx, start, new):
+    """Other queries in one row, whose scores outgrow their first tiles' by far, leave the others' bits."""
+    say(f"attend, 8 bits: a row among others {start} {new}")
+    g = gen(23)
+    n_pages, tables = make_tables(g, [a + n for a, n in zip(start, new)])
+    pool = make_pool8(g, n_pages)
+    q = bf16(g, sum(new), 32, D)
+    outs = [torch.empty_like(q) for _ in range(2)]
+    for out, factor in zip(outs, (1, 30)):
+        q[1] *= factor
+        attend8(hip, ctx, start, new, ALL, 0, 32, q, pool, tables, out)
+    torch.cuda.synchronize()
+    others = [r for r in range(sum(new)) if r != 1]
+    assert torch.equal(outs[0][others], outs[1][others]) and not torch.equal(outs[0][1], outs[1][1])
+
+
 @pytest.mark.parametrize("start,new,heads", [([6000, 20, 3], [1, 1, 1], 32), ([0, 900], [333, 65], 32),
                                              ([30000], [200], 16), ([40000], [2], 64)])
 def test_attend_in_place(hip, ctx, start, new, heads):
@@ -745,6 +762,23 @@ def test_shared_unseen_values_do_not_matter(hip, ctx, fmt, fill):
     assert torch.isnan(out[sees][:, 8:12]).all()
     other = [h for h in range(32) if h // 4 != 2]
     assert torch.equal(out[:, other], want_bits[:, other])
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_shared_sequences_that_are_over(hip, ctx, fmt):
+    """Sequences of a group without new rows may have no pages at all."""
+    say(f"shared: sequences that are over, format {fmt}")
+    g = gen(63)
+    sizes, lens, start, new = [5], [1280], [1300, 1290, 1280, 1400, 1281], [0, 2, 0, 1, 1]
+    n_pages, tables = shared_tables(g, sizes, lens, start, new)
+    pool, plain = pools(g, fmt, n_pages)
+    tables[0] = tables[2] = -1
+    q = bf16(g, sum(new), 32, D)
+    out = torch.empty_like(q)
+    shared(hip, ctx, fmt, sizes, lens, start, new, ALL, 0, 32, q, pool, tables, out)
+    torch.cuda.synchronize()
+    want, tol = attend64(start, new, ALL, 0, 32, q, plain, tables)
+    check_attend(out, want, tol)
 
 
 def test_no_new_rows_is_no_work(hip, ctx):

@@ -82,15 +82,14 @@ __host__ __device__ __forceinline__ bool is_narrow(int n, int gs, bool member) {
 // Rows of a block of the wide form.
 __host__ __device__ __forceinline__ int block_rows(int gs, int waves) { return (16 * waves) >> gs; }
 
-// Workgroup -> (segment, split, row block, kv head): kv heads go round the XCDs, whose L2 then holds the head's
+// Workgroup and item -> (segment, split, row block, kv head): kv heads go round the XCDs, whose L2 then holds the head's
 // keys for the blocks that share them; prefixes come first, then the sequences, of each the last blocks (the
 // longest runs) first.  (the segments' arguments in one go, a lane each)
 template <bool NARROW>
-__device__ __forceinline__ Work work_of(const AttnSharedParams& p, int waves) {
+__device__ __forceinline__ Work work_of(const AttnSharedParams& p, int waves, int item) {
   const int lane = threadIdx.x & 63, gs = p.group_shift;
   Work w;
   w.g = blockIdx.x % kKVHeads;
-  int item = blockIdx.x / kKVHeads;
   w.prefix = !NARROW && item < p.prefix_items;
   int lo, hi, pmax;
   const int member_end = p.member_end[lane];
@@ -113,7 +112,6 @@ __device__ __forceinline__ Work work_of(const AttnSharedParams& p, int waves) {
     pmax = w.nkeys - 1;
   } else {
     item -= NARROW ? 0 : p.prefix_items;
-    if constexpr (NARROW) item -= p.wide_items;
     const int item_end = NARROW ? p.narrow_end[lane] : p.wide_end[lane], row_end = p.row_end[lane],
               starts = p.start[lane], splits = p.splits[lane], part0 = p.part0[lane], los = p.lo[lane],
               prefixes = p.prefix[lane];
@@ -306,6 +304,31 @@ __device__ __forceinline__ void chunks_of(u32x4_t (&c)[2], const u32x4_t& w, flo
   }
 }
 
+// A wave's columns from col0 on: what they come to, or a partial of it.
+__device__ __forceinline__ void put(const AttnSharedParams& p, const Work& w, const ColumnState<1>& c, int col0) {
+  const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3, gs = p.group_shift;
+  const int heads = kKVHeads << gs;
+  const int col = col0 + fr, r = col >> gs;
+  if (r >= w.nr) return;
+  const int h = (w.g << gs) + (col & ((1 << gs) - 1));
+  if (!w.whole) {
+    const size_t slot = ((size_t)w.part0 + (size_t)w.split * w.n + w.r0 + r) * heads + h;
+    float* dst = p.part + slot * kHeadDim + 4 * G;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4_t*>(dst + 16 * db) = c.o[0][db];
+    if (G == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(c.m[0], c.l[0][0]);
+  } else {
+    const float inv = c.l[0][0] == 0.f ? 0.f : 1.0f / c.l[0][0];
+    uint16_t* dst = p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      const u32x2_t v = {pack_bf2(c.o[0][db][0] * inv, c.o[0][db][1] * inv),
+                         pack_bf2(c.o[0][db][2] * inv, c.o[0][db][3] * inv)};
+      *reinterpret_cast<u32x2_t*>(dst + db * 16 + 4 * G) = v;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- narrow form
 // A wave's K tile as operands: lane (fr, G) holds of the rows fr + 16 kb (kb 0 .. 3) the dims 32 ks + 8 G .. +8 (bf16),
 // or the codes 64 j + 16 G .. +16, j 0 and 1.
@@ -419,8 +442,8 @@ struct Joined {
 };
 
 template <bool F8, int AUX>
-__device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Work& w, Columns<F8>& c, int wave,
-                                             u32x4_t* tile) {
+__device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Work& w, Columns<F8>& c, int from,
+                                             int stride, u32x4_t* tile) {
   NarrowK<F8, AUX> k;
   NarrowV<F8, AUX> v;
   const Frags f;
@@ -429,10 +452,10 @@ __device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Wo
   const int lane = threadIdx.x & 63;
   int pages = -1;
   const auto look_up = [&](int first) {
-    const int i = first + NN * lane;
+    const int i = first + stride * lane;
     pages = i < w.i1 ? w.table[w.tile(i)] : -1;
   };
-  int i = w.i0 + wave, n = 0;
+  int i = w.i0 + from, n = 0;
   look_up(i);
   c.load(p, w, 0);
   int page = __builtin_amdgcn_readlane(pages, 0);
@@ -443,14 +466,14 @@ __device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Wo
   }
   c.set();
 #pragma unroll 1
-  for (; i < w.i1; i += NN) {
+  for (; i < w.i1; i += stride) {
     const bool there = page >= 0 && page < p.n_pages;
     const int key0 = w.tile(i) * BKEY;
     const Sight see = there ? sight(key0, c.least, c.most, p.window, p.n_sinks) : kNone;
-    if ((++n & 63) == 0) look_up(i + NN);
+    if ((++n & 63) == 0) look_up(i + stride);
     page = __builtin_amdgcn_readlane(pages, n & 63);
     // (past the last tile nothing is read)
-    const Planes x = planes_of<F8>(p, w.g, page, w.nkeys - w.tile(i + NN) * BKEY);
+    const Planes x = planes_of<F8>(p, w.g, page, w.nkeys - w.tile(i + stride) * BKEY);
     f32x4_t s[1][4];
     bf16x8_t pb[1][2];
     k.scores(s, c);
@@ -504,9 +527,9 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
   const int ncols = w.nr << gs;
   Columns<F8> c;
   if (p.nt && w.nqb == 1)
-    narrow_tiles<F8, 2>(p, w, c, wave, lds[wave]);
+    narrow_tiles<F8, 2>(p, w, c, wave, NN, lds[wave]);
   else
-    narrow_tiles<F8, 0>(p, w, c, wave, lds[wave]);
+    narrow_tiles<F8, 0>(p, w, c, wave, NN, lds[wave]);
   // the waves' sums side by side: [column][128], and (m, l); the 16-byte pieces of a column in an order of its own (16
   // columns' meet no bank twice)
   {
@@ -593,6 +616,17 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
     }
     j.write(p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim + d);
   }
+}
+
+// An item of a wave's own: no waves to join.
+template <bool F8>
+__device__ __forceinline__ void narrow_alone(const AttnSharedParams& p, const Work& w, u32x4_t* tile) {
+  Columns<F8> c;
+  if (p.nt && w.nqb == 1)
+    narrow_tiles<F8, 2>(p, w, c, 0, 1, tile);
+  else
+    narrow_tiles<F8, 0>(p, w, c, 0, 1, tile);
+  put(p, w, c, 0);
 }
 
 // ---------------------------------------------------------------- wide form
@@ -743,75 +777,82 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
     ++i;
   }
 
-  const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3, gs = p.group_shift;
-  const int heads = kKVHeads << gs;
-  const int col = wave * 16 + fr, r = col >> gs;
-  if (r >= w.nr) return;
-  const int h = (w.g << gs) + (col & ((1 << gs) - 1));
-  if (!w.whole) {
-    const size_t slot = ((size_t)w.part0 + (size_t)w.split * w.n + w.r0 + r) * heads + h;
-    float* dst = p.part + slot * kHeadDim + 4 * G;
-#pragma unroll
-    for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4_t*>(dst + 16 * db) = c.o[0][db];
-    if (G == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(c.m[0], c.l[0][0]);
-  } else {
-    const float inv = c.l[0][0] == 0.f ? 0.f : 1.0f / c.l[0][0];
-    uint16_t* dst = p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim;
-#pragma unroll
-    for (int db = 0; db < 8; ++db) {
-      const u32x2_t v = {pack_bf2(c.o[0][db][0] * inv, c.o[0][db][1] * inv),
-                         pack_bf2(c.o[0][db][2] * inv, c.o[0][db][3] * inv)};
-      *reinterpret_cast<u32x2_t*>(dst + db * 16 + 4 * G) = v;
-    }
-  }
+  put(p, w, c, wave * 16);
 }
 
 template <bool F8>
 __global__ __launch_bounds__(64 * NN, 2) void attn_shared_narrow_kernel(AttnSharedParams p) {
   __shared__ u32x4_t lds[NN][TC];
-  narrow<F8>(p, work_of<true>(p, 1), lds);
+  narrow<F8>(p, work_of<true>(p, 1, blockIdx.x / kKVHeads), lds);
 }
 
-template <bool F8>
+// Both forms; the narrow items a workgroup each, or a wave each where they are short and many.
+template <bool F8, bool ALONE>
 __global__ __launch_bounds__(64 * NN, 2) void attn_shared_both_kernel(AttnSharedParams p) {
   __shared__ u32x4_t lds[NN][TC];
-  if ((int)(blockIdx.x / kKVHeads) < p.wide_items)
-    wide<F8, NN>(p, work_of<false>(p, NN), lds[0], lds[2]);
-  else
-    narrow<F8>(p, work_of<true>(p, 1), lds);
+  const int item = blockIdx.x / kKVHeads - p.wide_items;
+  if (item < 0) {
+    wide<F8, NN>(p, work_of<false>(p, NN, blockIdx.x / kKVHeads), lds[0], lds[2]);
+  } else if constexpr (ALONE) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = item * NN + wave;
+    if (mine < p.narrow_items) narrow_alone<F8>(p, work_of<true>(p, 1, mine), lds[wave]);
+  } else {
+    narrow<F8>(p, work_of<true>(p, 1, item), lds);
+  }
 }
 
 // (8-bit pages: 48 KiB of LDS)
 template <bool F8, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : F8 ? 3 : 2) void attn_shared_wide_kernel(AttnSharedParams p) {
   __shared__ u32x4_t kt[F8 ? TC : 2 * TC], vt[2 * TC];
-  wide<F8, NW>(p, work_of<false>(p, NW), kt, vt);
+  wide<F8, NW>(p, work_of<false>(p, NW, blockIdx.x / kKVHeads), kt, vt);
 }
 
 // Joins the partials of each (row, q head) that has more than one, but for those that the narrow form has joined: 32
-// lanes each, 4 dims a lane, the prefix's splits first, then the row's own.
+// lanes each, 4 dims a lane, the prefix's splits first, then the row's own; PARTS threads share a lane's splits.
+template <int PARTS>
 __global__ __launch_bounds__(256) void attn_shared_merge_kernel(AttnSharedParams p) {
+  constexpr int kEach = 8 / PARTS;  // (row, head) pairs a workgroup
   const int lane = threadIdx.x & 63;
   const int row_end = p.row_end[lane], member_end = p.member_end[lane], lane_splits = p.splits[lane],
             part0 = p.part0[lane], prefix = p.prefix[lane];
   const int heads = kKVHeads << p.group_shift;
-  const int row = blockIdx.x * 8 / heads;  // (8 heads a workgroup: heads is a multiple of 8)
+  const int row = blockIdx.x * kEach / heads;  // (heads is a multiple of 8)
   const int b = __popcll(__ballot(lane < p.n_seqs && row_end <= row)), before = max(b - 1, 0);
   const int k = __builtin_amdgcn_readlane(prefix, b), splits = __builtin_amdgcn_readlane(lane_splits, b);
   const int row0 = b ? __builtin_amdgcn_readlane(row_end, before) : 0;
   const int n = __builtin_amdgcn_readlane(row_end, b) - row0;
-  if (k < 0 && (splits < 2 || is_narrow(n, p.group_shift, false))) return;
-  const int h = blockIdx.x * 8 % heads + (threadIdx.x >> 5), d = (threadIdx.x & 31) * 4;
+  if (k < 0 && (splits < 2 || is_narrow(n, p.group_shift, false))) return;  // (the whole workgroup)
+  const int part = threadIdx.x / (32 * kEach), pair = (threadIdx.x >> 5) % kEach;
+  const int h = blockIdx.x * kEach % heads + pair, d = (threadIdx.x & 31) * 4;
   Joined j;
+  // this part's share of `count` splits
+  const auto add = [&](size_t slot0, size_t step, int count) {
+    const int each = (count + PARTS - 1) / PARTS, from = part * each;
+    add_splits<false>(j, p, slot0 + from * step, step, min(each, count - from), d);
+  };
   if (k >= 0) {
     const int first = p.p_first[k], end = p.p_end[k], p_splits = p.p_splits[k], p_part0 = p.p_part0[k];
     const int base = first ? __builtin_amdgcn_readlane(member_end, max(first - 1, 0)) : 0;
     const int all = __builtin_amdgcn_readlane(member_end, end - 1) - base;
     const int at = (b ? __builtin_amdgcn_readlane(member_end, before) : 0) - base + row - row0;
-    add_splits<false>(j, p, ((size_t)p_part0 + at) * heads + h, (size_t)all * heads, p_splits, d);
+    add(((size_t)p_part0 + at) * heads + h, (size_t)all * heads, p_splits);
   }
-  add_splits<false>(j, p, ((size_t)__builtin_amdgcn_readlane(part0, b) + row - row0) * heads + h, (size_t)n * heads,
-                    splits, d);
+  add(((size_t)__builtin_amdgcn_readlane(part0, b) + row - row0) * heads + h, (size_t)n * heads, splits);
+  if constexpr (PARTS > 1) {
+    __shared__ f32x4_t part_o[PARTS][kEach][32];
+    __shared__ float2 part_ml[PARTS][kEach];
+    part_o[part][pair][threadIdx.x & 31] = j.o;
+    if (d == 0) part_ml[part][pair] = make_float2(j.M, j.L);
+    __syncthreads();
+    if (part) return;
+    f32x4_t o[PARTS];
+    float2 ml[PARTS];
+#pragma unroll
+    for (int u = 0; u < PARTS; ++u) o[u] = part_o[u][pair][threadIdx.x & 31], ml[u] = part_ml[u][pair];
+    j = Joined();
+    j.add(o, ml, PARTS);
+  }
   j.write(p.out + ((size_t)row * heads + h) * kHeadDim + d);
 }
 
@@ -844,10 +885,13 @@ struct Segment {
 
 int blocks_of(const Segment& x, int gs, int columns) { return (x.n + (columns >> gs) - 1) / (columns >> gs); }
 
-// What is launched: `both` forms in one kernel (the wide one with 4 waves), or each in its own; the tiles a split of
-// either form.
+// The join takes a lane's splits by four threads where that fills a launch.
+bool few_pairs(int rows, int gs) { return rows < 512 >> gs; }
+
+// What is launched: `both` forms in one kernel (the wide one with 4 waves, the narrow items a wave each if `alone`), or each
+// in its own; the tiles a split of either form.
 struct Plan {
-  bool both;
+  bool both, alone;
   int waves, wide, narrow;
   int splits(const Segment& x) const {
     // (16 tiles, four a wave, take as long as the join of two halves does)
@@ -877,10 +921,10 @@ double turns(const Rate& r, double items, double us) {
 
 // The launches with the least modelled time.  A workgroup starts and ends in 4 us and takes its tiles (1.5 more for the
 // masked ones of a run), a narrow one 1.25 for four; a launch more is 3, the join 4.5 and
-// 0.2 a split, its partials written and read at 5 TB/s.  Within 10% of the best of 12 split counts and both workgroup sizes over 13 batches of 1-2500 rows
+// 0.2 a split (0.06 by four threads), its partials written and read at 5 TB/s.  Within 10% of the best of 12 split counts and both workgroup sizes over 13 batches of 1-2500 rows
 // (1 x 200 rows over 16000 keys 345 us uncut, 79-85 in 8; 2500 rows 72 uncut, 104 in two; 2 x 1000 over
 // 4096 keys 148 and 152), and of 8 counts over 10 batches with prefixes.
-Plan plan_of(const Segment* x, int n, bool prefixes, bool fp8, int gs, long long room) {
+Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs, long long room) {
   long long narrow = 0;
   int wide_longest = 0, narrow_longest = 0, narrow_items = 0;
   bool any_narrow = false;
@@ -897,7 +941,7 @@ Plan plan_of(const Segment* x, int n, bool prefixes, bool fp8, int gs, long long
       wide[n_wide++] = x + i;
     }
   }
-  Plan best{false, 8, 1, 4};
+  Plan best{false, false, 8, 1, 4};
   // narrow: a workgroup a CU, in whole rounds of its waves, two at least
   best.narrow = NN * (int)std::max<long long>(2, (narrow * kKVHeads + 256 * NN - 1) / (256 * NN));
   // (halves of unequal runs are no better than a run)
@@ -909,14 +953,17 @@ Plan plan_of(const Segment* x, int n, bool prefixes, bool fp8, int gs, long long
     narrow_us = 1.25 * ((std::min(best.narrow, narrow_longest) + NN - 1) / NN);
   }
   double least = 1e30;
-  for (int form = 0; form < 3 && wide_longest; ++form) {
-    const bool both = form == 2;
-    if (both && !any_narrow) continue;
-    const Rate& r = kRates[fp8][form];
+  for (int form = 0; form < 4 && wide_longest; ++form) {
+    const bool both = form >= 2, alone = form == 3;
+    // (a wave each: uncut items that would fill the chip with workgroups)
+    if (both && (!any_narrow || (alone && (narrow_longest > best.narrow || narrow_items < 512)))) continue;
+    const Rate& r = kRates[fp8][std::min(form, 2)];
+    const double small = alone ? (double)narrow_items / NN : narrow_items;  // workgroups
+    const double small_us = 4 + (alone ? 1.25 * narrow_longest : narrow_us);
     int tried = 0;
     for (const int k : {1, 2, 3, 4, 6, 8, 10, 12, 16, 20, 26, 32, 48, kMaxSplits}) {
       Plan plan = best;
-      plan.both = both, plan.waves = r.waves, plan.wide = (wide_longest + k - 1) / k;
+      plan.both = both, plan.alone = alone, plan.waves = r.waves, plan.wide = (wide_longest + k - 1) / k;
       if (k > wide_longest || plan.wide == tried) continue;
       tried = plan.wide;
       double items = 0, tiles = 0, parts = 0;
@@ -930,11 +977,11 @@ Plan plan_of(const Segment* x, int n, bool prefixes, bool fp8, int gs, long long
         most = std::max(most, s);
       }
       const double each = 4 + (tiles / items + 1.5) * r.c[0];
-      double cost = std::max(both ? turns(r, items + narrow_items, (items * each + narrow_items * (4 + narrow_us)) / (items + narrow_items))
+      double cost = std::max(both ? turns(r, items + small, (items * each + small * small_us) / (items + small))
                                   : turns(r, items, each),
                              4 + (plan.wide + 1.5) * r.c[0]);
       if (!both && any_narrow) cost += 3 + turns(kRates[fp8][2], narrow_items, 4 + narrow_us);
-      if (parts || prefixes) cost += 4.5 + 0.2 * most + parts * (kKVHeads << gs) * (kHeadDim + 2) * 4 * 2 / 5e6;
+      if (parts || prefixes) cost += 4.5 + (few_pairs(rows, gs) ? 0.06 : 0.2) * most + parts * (kKVHeads << gs) * (kHeadDim + 2) * 4 * 2 / 5e6;
       if (cost < least) least = cost, best = plan;
     }
   }
@@ -1006,7 +1053,7 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     };
     own[b].tiles = std::max(tiles(0), last ? tiles(last) : 0);
   }
-  const Plan plan = plan_of(all, p.n_prefixes + s.n, p.n_prefixes > 0, fp8, gs, part_rows(rows, heads));
+  const Plan plan = plan_of(all, p.n_prefixes + s.n, rows, p.n_prefixes > 0, fp8, gs, part_rows(rows, heads));
   // splits, items and partial rows, segment by segment
   int wide = 0, narrow = 0, part = 0;
   bool merge = false, tagged = false;
@@ -1043,12 +1090,17 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kArrivedBytes);
   p.part_ml = p.part + (size_t)part * heads * kHeadDim;
   p.wide_items = plan.both ? wide : 0;
+  p.narrow_items = narrow;
   if (plan.both) {
-    const dim3 grid((wide + narrow) * kKVHeads), block(64 * NN);
-    if (fp8)
-      hipLaunchKernelGGL((attn_shared_both_kernel<true>), grid, block, 0, st, p);
+    const dim3 grid((wide + (plan.alone ? (narrow + NN - 1) / NN : narrow)) * kKVHeads), block(64 * NN);
+    if (fp8 && plan.alone)
+      hipLaunchKernelGGL((attn_shared_both_kernel<true, true>), grid, block, 0, st, p);
+    else if (fp8)
+      hipLaunchKernelGGL((attn_shared_both_kernel<true, false>), grid, block, 0, st, p);
+    else if (plan.alone)
+      hipLaunchKernelGGL((attn_shared_both_kernel<false, true>), grid, block, 0, st, p);
     else
-      hipLaunchKernelGGL((attn_shared_both_kernel<false>), grid, block, 0, st, p);
+      hipLaunchKernelGGL((attn_shared_both_kernel<false, false>), grid, block, 0, st, p);
     IE_CHECK_LAUNCH();
     wide = narrow = 0;
   }
@@ -1073,7 +1125,11 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     IE_CHECK_LAUNCH();
   }
   if (merge) {
-    hipLaunchKernelGGL(attn_shared_merge_kernel, dim3(rows << gs), dim3(256), 0, st, p);
+    // (few rows: their partials a few at a time)
+    if (few_pairs(rows, gs))
+      hipLaunchKernelGGL((attn_shared_merge_kernel<4>), dim3(rows << gs << 2), dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((attn_shared_merge_kernel<1>), dim3(rows << gs), dim3(256), 0, st, p);
     IE_CHECK_LAUNCH();
   }
   return IE_OK;

@@ -638,6 +638,7 @@ SHARED = [
     ([2, 2], [131008, 64], [131008, 131071, 64, 64], [1, 1, 40, 2], 3000, 10, 32),        # the last positions
     ([1] * 5, [64, 0, 128, 64, 0], [64, 0, 200, 100, 77], [1, 2, 3, 70, 1], ALL, 0, 32),
     ([3], [640], [640, 700, 1000], [0, 0, 1], ALL, 0, 32),            # the only one with rows is not the first
+    ([1, 1], [64, 128], [3000, 1500], [10, 13], ALL, 0, 32),          # few columns, nothing shared
 ]
 
 
@@ -716,13 +717,16 @@ def test_shared_evicted_pages(hip, ctx, fmt):
 
 
 @pytest.mark.parametrize("fmt,fill", [(0, float("nan")), (0, float("inf")), (1, 0xFF), (1, 0x7E)])
-def test_shared_unseen_values_do_not_matter(hip, ctx, fmt, fill):
+@pytest.mark.parametrize("sizes,lens,start,new", [
+    ([6], [1024], [1024, 1100, 1180, 1250, 1330, 1390], [1, 3, 1, 16, 1, 1]),
+    ([2], [64], [560, 700], [90, 2500]),                              # chunks, each by itself
+])
+def test_shared_unseen_values_do_not_matter(hip, ctx, fmt, fill, sizes, lens, start, new):
     """Windows of different positions cut a prefix at different keys: what a row does not see never reaches it, and
     what lies in no row's sight may be anything."""
-    say(f"shared: unseen values {fill}, format {fmt}")
+    say(f"shared: unseen values {fill}, format {fmt}, rows {new}")
     g = gen(62)
-    sizes, lens, window, sinks = [6], [1024], 400, 5
-    start, new = [1024, 1100, 1180, 1250, 1330, 1390], [1, 3, 1, 16, 1, 1]
+    window, sinks = 400, 5
     n_pages, tables = shared_tables(g, sizes, lens, start, new)
     clean, plain = pools(g, fmt, n_pages)
     pool = pool8(n_pages, fill) if fmt else torch.full_like(clean, fill)
@@ -743,20 +747,22 @@ def test_shared_unseen_values_do_not_matter(hip, ctx, fmt, fill):
     out, want_bits = torch.empty_like(q), torch.empty_like(q)
     shared(hip, ctx, fmt, sizes, lens, start, new, window, sinks, 32, q, clean, tables, want_bits)
     shared(hip, ctx, fmt, sizes, lens, start, new, window, sinks, 32, q, pool, tables, out)
-    # a NaN value at key 700, which the windows of the sequences from 1100 on have passed
     torch.cuda.synchronize()
     want, tol = attend64(start, new, window, sinks, 32, q, plain, tables)
     check_attend(out, want, tol)
     assert torch.equal(out, want_bits)
+    # a NaN value at key 700, which some rows' windows have passed
     at = 700
-    if fmt:
-        codes_of(pool)[tables[0, at // PAGE].long(), LAYER, 1, 2, at % PAGE] = 0x7F
-    else:
-        pool[tables[0, at // PAGE].long(), LAYER, 1, 2, at % PAGE] = float("nan")
+    for b in range(len(start)):
+        page = tables[b, at // PAGE].long()
+        if fmt:
+            codes_of(pool)[page, LAYER, 1, 2, at % PAGE] = 0x7F
+        else:
+            pool[page, LAYER, 1, 2, at % PAGE] = float("nan")
     shared(hip, ctx, fmt, sizes, lens, start, new, window, sinks, 32, q, pool, tables, out)
     torch.cuda.synchronize()
     pos = torch.cat([torch.arange(a, a + n) for a, n in zip(start, new)]).cuda()
-    sees = at > pos - window
+    sees = (at <= pos) & (at > pos - window)
     assert sees.any() and not sees.all()
     assert torch.equal(out[~sees], want_bits[~sees])
     assert torch.isnan(out[sees][:, 8:12]).all()

@@ -479,9 +479,9 @@ __device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Wo
     k.scores(s, c);
     k.issue(x, w.g);
     if (see == kAll)
-      weights_lazy<false>(pb, c, s, key0, p.window, p.n_sinks);
+      weights_grown<false>(pb, c, s, key0, p.window, p.n_sinks);
     else if (see == kSome)
-      weights_lazy<true>(pb, c, s, key0, p.window, p.n_sinks);
+      weights_grown<true>(pb, c, s, key0, p.window, p.n_sinks);
     if (see != kNone) v.stage(tile);
     v.issue(x, w.g);
     // (the wave's own tile: the hardware does its LDS accesses in order; the compiler is held to it)
@@ -759,7 +759,7 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
       f32x4_t s[1][4];
       bf16x8_t pb[1][2];
       tile_scores(s, i);
-      weights_lazy<false>(pb, c, s, 0, p.window, p.n_sinks);
+      weights_grown<false>(pb, c, s, 0, p.window, p.n_sinks);
       values<false, kAhead>(c, pb, f, vt + (i & 1) * TC, 0, p.window, p.n_sinks);
     }
     if (i == w.i1) break;
@@ -770,7 +770,7 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
       f32x4_t s[1][4];
       bf16x8_t pb[1][2];
       tile_scores(s, i);
-      weights_lazy<true>(pb, c, s, key0, p.window, p.n_sinks);
+      weights_grown<true>(pb, c, s, key0, p.window, p.n_sinks);
       __builtin_amdgcn_sched_barrier(0);  // (no fragments held over the softmax: registers)
       values<true>(c, pb, f, vt + (i & 1) * TC, key0, p.window, p.n_sinks);
     }

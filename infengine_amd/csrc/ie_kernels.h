@@ -361,6 +361,7 @@ struct AttnSharedParams {
   unsigned long long* arrived;  // [seqs][4 blocks][8 kv heads]: the last split to arrive joins them
   unsigned long long tag;
   int n_seqs, n_prefixes, prefix_items, wide_items, narrow_items;
+  int merge_row0;           // first row of a launch of the join
   bool nt;                  // nontemporal loads of tiles that one workgroup reads
   // by sequence: first new position; rows up to and with the sequence's, and those of members; items of the narrow
   // and of the wide form; key splits; first partial row; first own block; its prefix or -1

@@ -817,7 +817,7 @@ __global__ __launch_bounds__(256) void attn_shared_merge_kernel(AttnSharedParams
   const int row_end = p.row_end[lane], member_end = p.member_end[lane], lane_splits = p.splits[lane],
             part0 = p.part0[lane], prefix = p.prefix[lane];
   const int heads = kKVHeads << p.group_shift;
-  const int row = blockIdx.x * kEach / heads;  // (heads is a multiple of 8)
+  const int row = p.merge_row0 + blockIdx.x * kEach / heads;  // (heads is a multiple of 8)
   const int b = __popcll(__ballot(lane < p.n_seqs && row_end <= row)), before = max(b - 1, 0);
   const int k = __builtin_amdgcn_readlane(prefix, b), splits = __builtin_amdgcn_readlane(lane_splits, b);
   const int row0 = b ? __builtin_amdgcn_readlane(row_end, before) : 0;
@@ -1125,12 +1125,18 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     IE_CHECK_LAUNCH();
   }
   if (merge) {
-    // (few rows: their partials a few at a time)
-    if (few_pairs(rows, gs))
+    // (few rows: their partials a few at a time; a grid holds 2^32 threads)
+    constexpr int kRows = 1 << 20;
+    if (few_pairs(rows, gs)) {
       hipLaunchKernelGGL((attn_shared_merge_kernel<4>), dim3(rows << gs << 2), dim3(256), 0, st, p);
-    else
-      hipLaunchKernelGGL((attn_shared_merge_kernel<1>), dim3(rows << gs), dim3(256), 0, st, p);
-    IE_CHECK_LAUNCH();
+      IE_CHECK_LAUNCH();
+    } else {
+      for (; p.merge_row0 < rows; p.merge_row0 += kRows) {
+        const int n = std::min(rows - p.merge_row0, kRows);
+        hipLaunchKernelGGL((attn_shared_merge_kernel<1>), dim3(n << gs), dim3(256), 0, st, p);
+        IE_CHECK_LAUNCH();
+      }
+    }
   }
   return IE_OK;
 }

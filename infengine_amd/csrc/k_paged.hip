@@ -144,6 +144,7 @@ __global__ __launch_bounds__(256) void kv_fork_kernel(ForkParams p) {
 // 164 us, 6.15 TB/s read and written (186 with stores that stay in the caches), back 175, 5.8 (two planes a workgroup 174,
 // codes read past the caches 175, but 21.9 in place of 19.3 for 10 pages just written); three pages 7.5.
 constexpr int kPlaneRounds = kPagePos / 16;
+constexpr int kMaxConvert = 1 << 14;  // pages a launch: a grid holds 2^32 threads
 
 __global__ __launch_bounds__(256) void kv_to_fp8_kernel(const int* src, const int* dst, const uint16_t* pages,
                                                         int n_pages, uint8_t* pages8, int n_pages8) {
@@ -365,15 +366,21 @@ int launch_kv_fork(int n_forks, const int* src_rows, const int* dst_rows, const 
 
 int launch_kv_to_fp8(int n, const int* src, const int* dst, const uint16_t* pages, int n_pages, uint8_t* pages8,
                      int n_pages8, hipStream_t st) {
-  hipLaunchKernelGGL(kv_to_fp8_kernel, dim3(n * kPlanes), dim3(256), 0, st, src, dst, pages, n_pages, pages8, n_pages8);
-  IE_CHECK_LAUNCH();
+  for (int i = 0; i < n; i += kMaxConvert) {
+    hipLaunchKernelGGL(kv_to_fp8_kernel, dim3(std::min(n - i, kMaxConvert) * kPlanes), dim3(256), 0, st, src + i, dst + i,
+                       pages, n_pages, pages8, n_pages8);
+    IE_CHECK_LAUNCH();
+  }
   return IE_OK;
 }
 
 int launch_kv_from_fp8(int n, const int* src, const int* dst, const uint8_t* pages8, int n_pages8, uint16_t* pages,
                        int n_pages, hipStream_t st) {
-  hipLaunchKernelGGL(kv_from_fp8_kernel, dim3(n * kPlanes), dim3(256), 0, st, src, dst, pages8, n_pages8, pages, n_pages);
-  IE_CHECK_LAUNCH();
+  for (int i = 0; i < n; i += kMaxConvert) {
+    hipLaunchKernelGGL(kv_from_fp8_kernel, dim3(std::min(n - i, kMaxConvert) * kPlanes), dim3(256), 0, st, src + i,
+                       dst + i, pages8, n_pages8, pages, n_pages);
+    IE_CHECK_LAUNCH();
+  }
   return IE_OK;
 }
 

@@ -225,6 +225,29 @@ def test_pages_outside_the_pools_are_left_out(hip, ctx):
     assert torch.equal(a, kept)
 
 
+def test_pages_of_long_lists(hip, ctx):
+    """The longest lists, nearly all of whose pairs are left out."""
+    say("pages: lists of 65536")
+    g = gen(5)
+    a, b = bf16(g, 2, LAYERS, 2, KVH, PAGE, D), pool8(3, 0x33)
+    src, dst = torch.full((65536,), -1, dtype=torch.int32, device="cuda"), torch.zeros(65536, dtype=torch.int32,
+                                                                                      device="cuda")
+    src[16383], src[16384], src[65535] = 0, 1, 0
+    dst[16383], dst[16384], dst[65535] = 2, 1, 0
+    to_fp8(hip, ctx, src, dst, a, b)
+    torch.cuda.synchronize()
+    for page, of in ((2, 0), (1, 1), (0, 0)):
+        check_page(a[of], b, page)
+    back, want = torch.full_like(a, 7.0), torch.full_like(a[:1], 7.0)
+    from_fp8(hip, ctx, ids(1), ids(0), b, want)
+    dst.fill_(-1)
+    src.zero_()
+    src[65535], dst[65535] = 1, 1
+    from_fp8(hip, ctx, src, dst, b, back)
+    torch.cuda.synchronize()
+    assert torch.equal(back[1], want[0]) and (back[0] == 7.0).all()
+
+
 # ------------------------------------------------------------------------------- append
 def append8(hip, ctx, start, new, heads, qkv, wq, wk, cos, sin, q, pool, tables, layer=LAYER):
     hip.check(hip.lib.ie_qk_norm_rope_paged_fp8(
@@ -785,6 +808,27 @@ def test_shared_sequences_that_are_over(hip, ctx, fmt):
     torch.cuda.synchronize()
     want, tol = attend64(start, new, ALL, 0, 32, q, plain, tables)
     check_attend(out, want, tol)
+
+
+def test_shared_after_very_many_rows(hip, ctx):
+    """Two sequences that share a prefix, behind 2^21 rows: more than one launch of the join."""
+    start, new, heads = [0] * 16 + [200, 300], [131072] * 16 + [1, 1], 64
+    say(f"shared, {sum(new)} rows of {heads} heads")
+    g = gen(330)
+    pool = make_pool8(g, 40)
+    plain = bf16_pool(pool)
+    tables = torch.randint(0, 40, (18, 2048), dtype=torch.int32, device="cuda", generator=g)
+    tables[17, :2] = tables[16, :2]
+    rows = sum(new)
+    q = torch.empty(rows, heads, D, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    out = torch.full_like(q, 7.0)
+    shared(hip, ctx, 1, [16, 2], [0, 128], start, new, 64, 0, heads, q, pool, tables, out)
+    torch.cuda.synchronize()
+    for first, n, seqs, at in ((rows - 2, 2, slice(16, 18), [200, 300]), (rows - 9, 7, slice(15, 16), [131065]),
+                               (131072 * 7 + 1000, 5, slice(7, 8), [1000]), (0, 3, slice(0, 1), [0])):
+        count = [1, 1] if len(at) == 2 else [n]
+        want, tol = attend64(at, count, 64, 0, heads, q[first:first + n], plain, tables[seqs])
+        check_attend(out[first:first + n], want, tol, first)
 
 
 def test_no_new_rows_is_no_work(hip, ctx):

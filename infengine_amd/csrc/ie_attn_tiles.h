@@ -88,6 +88,23 @@ __device__ __forceinline__ void scores(f32x4_t (&s)[QI][4], const ColumnState<QI
   }
 }
 
+// Scores of keys that a column does not see to -inf.
+template <int QI, int KB>
+__device__ __forceinline__ void mask(f32x4_t (&s)[QI][KB], const ColumnState<QI>& c, int key0, int window, int n_sinks) {
+  int first = 4 * (threadIdx.x >> 4 & 3);  // the lane's first key in each 16
+  asm volatile("" : "+v"(first));  // (opaque: nothing made of it is kept over the tiles)
+#pragma unroll
+  for (int qi = 0; qi < QI; ++qi)
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = key0 + first + 16 * kb + r;
+        const bool seen = (key <= c.pos[qi]) & ((key > c.pos[qi] - window) | (key < n_sinks));
+        s[qi][kb][r] = seen ? s[qi][kb][r] : -INFINITY;
+      }
+}
+
 // The scores to weights (bf16, as P^T operands), the outputs and sums so far rescaled.  MASK applies the
 // window, the sinks and the diagonal.  A column may have seen no key so far: its max stays -inf and its
 // weights are 0 (the exponent's offset is then taken from a finite stand-in).
@@ -134,14 +151,13 @@ __device__ __forceinline__ void weights(bf16x8_t (&pb)[QI][2], ColumnState<QI>& 
   }
 }
 
-// The same, rescaling only where a column's maximum has grown: in most tiles of a long run none has.  (A reference that
+// The same as weights, rescaling only where a column's maximum has grown: in most tiles of a long run none has.  (A reference that
 // stays until the scores outgrow it by 2^8 saves 3% more of 8192 rows' time, but the largest weight is then rounded as
 // all others are, where it is an exact 1 here: 0.0023 of error in place of 0.0020.)
 template <bool MASK, int QI, int KB>
 __device__ __forceinline__ void weights_grown(bf16x8_t (&pb)[QI][KB / 2], ColumnState<QI>& c,
                                              f32x4_t (&s)[QI][KB], int key0, int window, int n_sinks) {
-  int first = 4 * (threadIdx.x >> 4 & 3);  // the lane's first key in each 16
-  if constexpr (MASK) asm volatile("" : "+v"(first));  // (opaque: nothing made of it is kept over the tiles)
+  if constexpr (MASK) mask(s, c, key0, window, n_sinks);
   float mn[QI];
   bool moved = false;
 #pragma unroll
@@ -151,11 +167,6 @@ __device__ __forceinline__ void weights_grown(bf16x8_t (&pb)[QI][KB / 2], Column
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if constexpr (MASK) {
-          const int key = key0 + first + 16 * kb + r;
-          const bool seen = (key <= c.pos[qi]) & ((key > c.pos[qi] - window) | (key < n_sinks));
-          s[qi][kb][r] = seen ? s[qi][kb][r] : -INFINITY;
-        }
         mt = fmaxf(mt, s[qi][kb][r]);
       }
     mt = xor32_max(xor16_max(mt));

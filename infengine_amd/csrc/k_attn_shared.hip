@@ -936,10 +936,13 @@ constexpr Rate kRates[2][3] = {{{8, {1.92, 2.33, 0}}, {4, {1.75, 1.75, 0}}, {4, 
 // The time of `items` workgroups of `us` (at one a CU) each, by the rates' growth with their number.
 double turns(const Rate& r, double items, double us) {
   const int most = r.c[2] > 0 ? 3 : 2;
-  const double rounds = items / (256 * most);
-  // (the longest come first, so that more than a round ends evenly)
-  if (rounds > 1) return us / r.c[0] * r.c[most - 1] * rounds + 0.25 * us;
-  return us / r.c[0] * r.c[items > 512 ? 2 : items > 256 ? 1 : 0];
+  const double round = 256 * most, each = us / r.c[0];
+  const auto part = [&](double n) { return each * r.c[n > 512 ? 2 : n > 256 ? 1 : 0]; };
+  if (items <= round) return part(items);
+  // a second round takes what its workgroups take by themselves (2048 rows 88 us, 2100 and 3000 rows 130 with 8 waves, 122
+  // and 143 with 4); the ends of more come more evenly
+  if (items <= 2 * round) return each * r.c[most - 1] + part(items - round);
+  return each * r.c[most - 1] * items / round + 0.25 * us;
 }
 
 // The launches with the least modelled time.  A workgroup starts and ends in 4 us and takes its tiles (1.5 more for the

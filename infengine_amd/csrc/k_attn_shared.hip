@@ -657,35 +657,41 @@ __device__ __forceinline__ void narrow_alone(const AttnSharedParams& p, const Wo
 // column meet no bank twice.
 __device__ __forceinline__ int k8_slot(int r, int c) { return r * 8 + (c ^ ((r >> 1) & 7)); }
 
-// A thread's part of an 8-bit tile: of V chunk t % 8 of row t / 8 (and of the row 32 on, with 4 waves), which becomes
-// bf16 on the way to LDS; K goes there directly, 8 rows a wave's load.
+// A thread's part of an 8-bit tile: of V chunk vchunk() of row vrow() (and of the row 32 on, with 4 waves), which becomes
+// bf16 on the way to LDS; K goes there directly, 8 rows a wave's load.  V's rows and chunks go over the lanes so that
+// eight lanes' stores are half a row and half of the row 4 on, whose swizzle differs: they meet no bank twice.
 template <int NW>
 struct Wide8 {
   static constexpr int kEach = 8 / NW;
   u32x4_t v[kEach];
-  uint32_t vs;      // the scales of rows t / 8 % 16 + 16 i
+  uint32_t vs;      // the scales of rows vrow() % 16 + 16 i
   uint32_t ks[2];   // those of K's rows fr + 16 i, of this tile and the next
   int rows;
+  static __device__ __forceinline__ int vrow() {
+    const int t = threadIdx.x;
+    return (t >> 6) * 8 + (t >> 2 & 1) * 4 + (t >> 3 & 3);
+  }
+  static __device__ __forceinline__ int vchunk() { return (threadIdx.x >> 5 & 1) * 4 + (threadIdx.x & 3); }
   template <int AUX>
   __device__ __forceinline__ void issue(u32x4_t* ktile, const Planes& x, int g, int wave) {
     const int t = threadIdx.x, r = t >> 3;
     rows = x.rows;
     ks[0] = ks[1];
     ks[1] = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (t & 15), g * kPagePos, AUX);
-    vs = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (r & 15), (kKVHeads + g) * kPagePos, AUX);
+    vs = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (vrow() & 15), (kKVHeads + g) * kPagePos, AUX);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {  // (the row 32 on has the same swizzle)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(x.k, (lds_void*)(ktile + (wave + NW * i) * 64), 16,
                                                r * kHeadDim + (((t & 7) ^ ((r >> 1) & 7)) * 16), 32 * i * kHeadDim, 0,
                                                AUX);
-      v[i] = __builtin_amdgcn_raw_buffer_load_b128(x.v, 16 * t, 32 * i * kHeadDim, AUX);
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(x.v, vrow() * kHeadDim + vchunk() * 16, 32 * i * kHeadDim, AUX);
     }
   }
   __device__ __forceinline__ void stage(u32x4_t* vt, int wave) const {
-    const int t = threadIdx.x, c = 2 * (t & 7);
+    const int c = 2 * vchunk();
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int r = (t >> 3) + 32 * i;
+      const int r = vrow() + 32 * i;
       u32x4_t x[2];
       chunks_of(x, v[i], scale_at_byte(vs, (wave >> 1) + 2 * i, r < rows));  // (8 rows a wave)
       vt[kv_slot(r, c)] = x[0];
@@ -903,6 +909,7 @@ unsigned long long next_tag() {
 // A segment as the plan sees it.
 struct Segment {
   int n, tiles;  // rows; tiles of its longest row block
+  double mean;   // and of a row block in the mean
   bool narrow, parts;  // its form; it leaves partials even where it is not cut
 };
 
@@ -933,16 +940,19 @@ struct Rate {
 constexpr Rate kRates[2][3] = {{{8, {1.92, 2.33, 0}}, {4, {1.75, 1.75, 0}}, {4, {1.75, 1.9, 0}}},    // bf16; the last:
                                {{8, {1.35, 2.1, 0}}, {4, {1.16, 1.35, 1.79}}, {4, {1.2, 1.55, 0}}}};  // both forms
 
-// The time of `items` workgroups of `us` (at one a CU) each, by the rates' growth with their number.
-double turns(const Rate& r, double items, double us) {
+// The time of `items` workgroups of `us` (at one a CU) each, by the rates' growth with their number; even: 1 where they are
+// all as long as the longest, 0 where half as long in the mean.
+double turns(const Rate& r, double items, double us, double even) {
   const int most = r.c[2] > 0 ? 3 : 2;
   const double round = 256 * most, each = us / r.c[0];
   const auto part = [&](double n) { return each * r.c[n > 512 ? 2 : n > 256 ? 1 : 0]; };
   if (items <= round) return part(items);
-  // a second round takes what its workgroups take by themselves (2048 rows 88 us, 2100 and 3000 rows 130 with 8 waves, 122
-  // and 143 with 4); the ends of more come more evenly
-  if (items <= 2 * round) return each * r.c[most - 1] + part(items - round);
-  return each * r.c[most - 1] * items / round + 0.25 * us;
+  // (the longest come first, so that more than a round ends evenly)
+  const double mixed = each * r.c[most - 1] * items / round + 0.25 * us;
+  if (items > 2 * round) return mixed;
+  // equal ones: the second round takes what its workgroups take by themselves (2048 rows over 2048 keys each 88 us, 2100 and
+  // 3000 rows 130 with 8 waves, 122 and 143 with 4)
+  return mixed + even * (each * r.c[most - 1] + part(items - round) - mixed);
 }
 
 // The launches with the least modelled time.  A workgroup starts and ends in 4 us and takes its tiles (1.5 more for the
@@ -998,15 +1008,16 @@ Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs,
         const Segment& y = *wide[i];
         const int s = plan.splits(y), b = blocks_of(y, gs, 16 * r.waves);
         items += (double)s * b * kKVHeads;
-        tiles += (double)y.tiles * b * kKVHeads;
+        tiles += y.mean * b * kKVHeads;
         if (s > 1 || y.parts) parts += (double)y.n * s;
         most = std::max(most, s);
       }
       const double each = 4 + (tiles / items + 1.5) * r.c[0];
-      double cost = std::max(both ? turns(r, items + small, (items * each + small * small_us) / (items + small))
-                                  : turns(r, items, each),
+      const double even = std::clamp(2 * tiles / (items * plan.wide) - 1, 0.0, 1.0);
+      double cost = std::max(both ? turns(r, items + small, (items * each + small * small_us) / (items + small), even)
+                                  : turns(r, items, each, even),
                              4 + (plan.wide + 1.5) * r.c[0]);
-      if (!both && any_narrow) cost += 3 + turns(kRates[fp8][2], narrow_items, 4 + narrow_us);
+      if (!both && any_narrow) cost += 3 + turns(kRates[fp8][2], narrow_items, 4 + narrow_us, 0);
       if (parts || prefixes) cost += 4.5 + (few_pairs(rows, gs) ? 0.06 : 0.2) * most + parts * (kKVHeads << gs) * (kHeadDim + 2) * 4 * 2 / 5e6;
       if (cost < least) least = cost, best = plan;
     }
@@ -1067,17 +1078,23 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
   for (int k = 0; k < p.n_prefixes; ++k) {
     const int n = p.member_end[p.p_end[k] - 1] - (p.p_first[k] ? p.member_end[p.p_first[k] - 1] : 0);
     keys += p.p_blocks[k] * BKEY;
-    pre[k] = {n, run_of(p.p_start[k], p.p_blocks[k] * BKEY - 1, 0, p.p_blocks[k], p.window, p.n_sinks).count, false, true};
+    const int tiles = run_of(p.p_start[k], p.p_blocks[k] * BKEY - 1, 0, p.p_blocks[k], p.window, p.n_sinks).count;
+    pre[k] = {n, tiles, (double)tiles, false, true};
   }
   for (int b = 0; b < s.n; ++b) {
-    const int n = s.n_new[b], rb = block_rows(gs, 8), last = n ? (n - 1) / rb * rb : 0;
-    own[b] = {n, 0, is_narrow(n, gs, p.prefix[b] >= 0), p.prefix[b] >= 0};
+    const int n = s.n_new[b], rb = block_rows(gs, 8), last = n ? (n - 1) / rb : 0;
+    own[b] = {n, 0, 0, is_narrow(n, gs, p.prefix[b] >= 0), p.prefix[b] >= 0};
     if (!n) continue;
-    const auto tiles = [&](int r0) {
+    const auto tiles = [&](int block) {
+      const int r0 = block * rb;
       return run_of(s.start[b] + r0, s.start[b] + std::min(r0 + rb, n) - 1, p.lo[b], kMaxLongCtx / BKEY, p.window,
                     p.n_sinks).count;
     };
-    own[b].tiles = std::max(tiles(0), last ? tiles(last) : 0);
+    for (int i = 0; i < 8; ++i) {
+      const int x = tiles((int)((long long)last * i / 7));
+      own[b].tiles = std::max(own[b].tiles, x);
+      own[b].mean += x / 8.0;
+    }
   }
   const Plan plan = plan_of(all, p.n_prefixes + s.n, rows, p.n_prefixes > 0, fp8, gs, part_rows(rows, heads));
   // splits, items and partial rows, segment by segment

@@ -4,24 +4,37 @@
 //
 // The row at position p sees the keys j <= p with j > p - window or j < n_sinks whose page is there:
 //   o = sum_j softmax_j(q . k_j / sqrt(128)) v_j,  zeros where it sees none.
-// An 8-bit row is read as its codes times its scale 2^e, which bf16 holds exactly, so that both kinds of pages
-// run the same products (k_attn_window.hip: S^T = K . Q^T, online softmax, O^T = V^T . P^T in bf16 with fp32
-// sums, weights rounded to bf16).
+// An 8-bit row stands for its codes times its scale 2^e.  Scores of 8-bit keys: one 16x16x128 scaled product takes the
+// codes as they lie, with the keys' scales in its own scale operand (a lane's dword is the scales of its four
+// rows), and the queries as two e4m3 operands (Query8), which lose nothing against bf16.  Two such products cost as
+// much as the bf16 ones of the same keys, without a conversion or a second byte.  Values become bf16, exactly, on their way
+// to LDS: their scales go with the summed index, where the scaled product has none.  The rest is k_attn_window.hip's:
+// S^T = K . Q^T, online softmax, O^T = V^T . P^T in bf16 with fp32 sums, weights rounded to bf16 (2^-8 of a weight, the
+// sum is of the rounded ones).
 //
 // Softmax over a union of key sets is joined from (o, m, l) of each.  So the keys that a group of sequences
 // shares are attended once, by the rows of all of them (a prefix segment: rows of different sequences
 // are columns of one block, each with its own position), and each sequence's other keys by its rows (an own
-// segment).  Sequences that fill the columns of a block by themselves gain nothing from that and attend all
-// their keys in their own segment.
+// segment).  Sequences that fill the columns of a block by themselves (kMemberCols) gain nothing from that and attend
+// all their keys in their own segment.
 //
-// A workgroup of 4 waves takes one kv head of a segment in one of two forms.
-// Narrow (up to 16 columns, a column being a (row, q head of the kv head's group)): the key tiles go round
+// A workgroup takes one kv head of a block of a segment, in one of two forms.
+// Narrow (4 waves, up to 16 columns, a column being a (row, q head of the kv head's group)): the key tiles go round
 // the waves, each of which holds all the columns: nothing is shared until the waves' (o, m, l) are
 // joined at the end.  K comes from memory in the layout of the product's operand (the order of the 128 dims
 // within the sum is free, and Q's fragments are taken in the same order), V through registers into a tile of the
-// wave's own in LDS, from which it is read transposed.  No barrier, a tile of loads in flight a wave.
-// Wide: 16 or 32 columns a wave, the tiles staged in LDS for all four, double-buffered, as k_attn_window.hip
-// does it; 8-bit tiles pass through registers, where they become bf16.
+// wave's own in LDS, from which it is read transposed.  No barrier, a tile of loads in flight a wave (256 registers: in
+// 128, half a tile at a time, 16 tokens over 4096 keys take 92 us, not 30).  Bound by latency for few keys (one token
+// over 600 keys 9.0 us, of which the launch is 3; over 60000 33), by HBM past that (16 tokens over 4096
+// keys each 29.9, 4.5 TB/s; 5.7 but for the 9 of a run of one tile).  Splits are joined by the last to arrive.
+// Wide (4 or 8 waves of 16 columns): the tiles are staged in LDS for all waves, double-buffered; 8-bit
+// values pass through registers.  Bound by the vector units (busy 61% of the cycles) beside the matrix units (45%) and
+// LDS (43%): 8192 rows over 4096 keys 571-595 us, 0.94-0.98 PFLOP/s.  32 columns a wave, as the bf16
+// kernel has them, do not fit the registers beside the raw codes (680-690 us).
+// A batch with wide and few narrow items runs both in one launch; short narrow items that would fill the chip by themselves
+// take a wave each there (64 sequences behind one prefix 50 -> 45 us).  Rows with a prefix, or cut wide items, are
+// joined by a launch of their own (4.8 us for 16 tokens, 6.8 for 64; joining the prefix's partials in the narrow
+// kernel, behind a count, took longer than that launch).
 #include <algorithm>
 #include <atomic>
 #include <chrono>
@@ -402,7 +415,8 @@ struct NarrowV {
           x.v, off + (F8 ? (16 * (i >> 1) + (i & 1)) * kHeadDim : 4 * i * kRowBytes), 0, AUX);
   }
   // CHECK: whether the tile has an infinity or a NaN (8 bits: or may have).  Masked tiles need it: those without run the
-  // product of the others (a third of the instructions; 32 tokens over windows of 512 14.5 -> 12.2 us, one at 600 9.6 -> 9.0).
+  // product of the others (a third of the instructions; 32 tokens over windows of 512 14.5 -> 12.2 us, one at 600
+  // 9.6 -> 9.0).
   template <bool CHECK>
   __device__ __forceinline__ bool stage(u32x4_t* tile) const {
     const int lane = threadIdx.x & 63;
@@ -891,7 +905,9 @@ constexpr int kMaxSplits = 64;
 int members_of(int rows, int heads) { return std::min(rows, kMaxSeqs * std::max(1, kMemberCols / (heads / kKVHeads))); }
 // Partial rows (a row and split) that a workspace for `rows` rows holds: 64 splits of up to 64 rows, and a
 // prefix's and an own partial of each row that shares.  It never falls with the rows.
-long long part_rows(int rows, int heads) { return (long long)std::min(rows, 64) * kMaxSplits + 2ll * members_of(rows, heads); }
+long long part_rows(int rows, int heads) {
+  return (long long)std::min(rows, 64) * kMaxSplits + 2ll * members_of(rows, heads);
+}
 
 static_assert(kMemberCols <= kNarrowBlocks * kNarrowCols);
 constexpr size_t kArrivedBytes = (size_t)kMaxSeqs * kNarrowBlocks * kKVHeads * sizeof(unsigned long long);
@@ -957,9 +973,10 @@ double turns(const Rate& r, double items, double us, double even) {
 
 // The launches with the least modelled time.  A workgroup starts and ends in 4 us and takes its tiles (1.5 more for the
 // masked ones of a run), a narrow one 1.25 for four; a launch more is 3, the join 4.5 and
-// 0.2 a split (0.06 by four threads), its partials written and read at 5 TB/s.  Within 10% of the best of 12 split counts and both workgroup sizes over 13 batches of 1-2500 rows
-// (1 x 200 rows over 16000 keys 345 us uncut, 79-85 in 8; 2500 rows 72 uncut, 104 in two; 2 x 1000 over
-// 4096 keys 148 and 152), and of 8 counts over 10 batches with prefixes.
+// 0.2 a split (0.06 by four threads), its partials written and read at 5 TB/s.  Within 10% of the best of 12 split counts
+// and both workgroup sizes over 13 batches of 1-2500 rows (1 x 200 rows over 16000 keys 345 us uncut, 79-85 in 8;
+// 2500 rows 72 uncut, 104 in two; 2 x 1000 over 4096 keys 148 and 152), and of 8 counts over 10 batches with
+// prefixes; within 12% over 8 of 1100-3500 rows, which fill one round and part of another.
 Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs, long long room) {
   long long narrow = 0;
   int wide_longest = 0, narrow_longest = 0, narrow_items = 0;
@@ -1018,7 +1035,8 @@ Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs,
                                   : turns(r, items, each, even),
                              4 + (plan.wide + 1.5) * r.c[0]);
       if (!both && any_narrow) cost += 3 + turns(kRates[fp8][2], narrow_items, 4 + narrow_us, 0);
-      if (parts || prefixes) cost += 4.5 + (few_pairs(rows, gs) ? 0.06 : 0.2) * most + parts * (kKVHeads << gs) * (kHeadDim + 2) * 4 * 2 / 5e6;
+      if (parts || prefixes)
+        cost += 4.5 + (few_pairs(rows, gs) ? 0.06 : 0.2) * most + parts * (kKVHeads << gs) * (kHeadDim + 2) * 4 * 2 / 5e6;
       if (cost < least) least = cost, best = plan;
     }
   }
@@ -1125,8 +1143,8 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     p.narrow_end[b] = narrow;
     p.wide_end[b] = wide - p.prefix_items;
   }
-  // a batch whose keys of all layers exceed the 256 MB cache finds none of them there: such keys, where one
-  // workgroup reads them, pass it by
+  // a batch whose keys of all layers are about the 256 MB cache and more (2048 are 268 MB in bf16, 135 in 8 bits) finds
+  // few of them there: such keys, where one workgroup reads them, pass it by
   p.nt = keys > 2048;
   p.arrived = static_cast<unsigned long long*>(workspace);
   p.tag = tagged ? next_tag() : 0;

@@ -19,13 +19,13 @@
 // all their keys in their own segment.
 //
 // A workgroup takes one kv head of a block of a segment, in one of two forms.
-// Narrow (4 waves, up to 16 columns, a column being a (row, q head of the kv head's group)): the key tiles go round
+// Narrow (4 or 8 waves, up to 16 columns, a column being a (row, q head of the kv head's group)): the key tiles go round
 // the waves, each of which holds all the columns: nothing is shared until the waves' (o, m, l) are
 // joined at the end.  K comes from memory in the layout of the product's operand (the order of the 128 dims
 // within the sum is free, and Q's fragments are taken in the same order), V through registers into a tile of the
 // wave's own in LDS, from which it is read transposed.  No barrier, a tile of loads in flight a wave (256 registers: in
 // 128, half a tile at a time, 16 tokens over 4096 keys take 92 us, not 30).  Bound by latency for few keys (one token
-// over 600 keys 9.0 us, of which the launch is 3; over 60000 33), by HBM past that (16 tokens over 4096
+// over 600 keys 8.7 us, of which the launch is 3; over 60000 33), by HBM past that (16 tokens over 4096
 // keys each 29.9, 4.5 TB/s; 5.7 but for the 9 of a run of one tile).  Splits are joined by the last to arrive.
 // Wide (4 or 8 waves of 16 columns): the tiles are staged in LDS for all waves, double-buffered; 8-bit
 // values pass through registers.  Bound by the vector units (busy 61% of the cycles) beside the matrix units (45%) and
@@ -46,7 +46,7 @@ namespace ie {
 
 namespace {
 
-constexpr int NN = 4;  // waves of the narrow form's workgroups
+constexpr int NN = 4;  // waves of the narrow form's workgroups (8 where the plan says so)
 constexpr int kNarrowCols = 16;
 constexpr int kNarrowBlocks = 4;  // of a sequence, at most
 
@@ -415,8 +415,7 @@ struct NarrowV {
           x.v, off + (F8 ? (16 * (i >> 1) + (i & 1)) * kHeadDim : 4 * i * kRowBytes), 0, AUX);
   }
   // CHECK: whether the tile has an infinity or a NaN (8 bits: or may have).  Masked tiles need it: those without run the
-  // product of the others (a third of the instructions; 32 tokens over windows of 512 14.5 -> 12.2 us, one at 600
-  // 9.6 -> 9.0).
+  // product of the others (a third of the instructions; 32 tokens over windows of 512 14.5 -> 12.2 us).
   template <bool CHECK>
   __device__ __forceinline__ bool stage(u32x4_t* tile) const {
     const int lane = threadIdx.x & 63;
@@ -555,18 +554,18 @@ __device__ __forceinline__ void add_splits(Joined& j, const AttnSharedParams& p,
   }
 }
 
-template <bool F8>
+template <bool F8, int NW>
 __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w, u32x4_t (*lds)[TC]) {
   __shared__ int s_last;
-  __shared__ float2 ml_of[NN][kNarrowCols];  // (m, l) of the waves' columns, then of parts of the splits
+  __shared__ float2 ml_of[NW][kNarrowCols];  // (m, l) of the waves' columns, then of parts of the splits
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tid = threadIdx.x, gs = p.group_shift, heads = kKVHeads << gs;
   const int ncols = w.nr << gs;
   Columns<F8> c;
   if (p.nt && w.nqb == 1)
-    narrow_tiles<F8, 2>(p, w, c, wave, NN, lds[wave]);
+    narrow_tiles<F8, 2>(p, w, c, wave, NW, lds[wave]);
   else
-    narrow_tiles<F8, 0>(p, w, c, wave, NN, lds[wave]);
+    narrow_tiles<F8, 0>(p, w, c, wave, NW, lds[wave]);
   // the waves' sums side by side: [column][128], and (m, l); the 16-byte pieces of a column in an order of its own (16
   // columns' meet no bank twice)
   {
@@ -577,18 +576,18 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
     if (G == 0) ml_of[wave][fr] = make_float2(c.m[0], c.l[0][0]);
   }
   __syncthreads();
-  for (int i = tid; i < ncols * 32; i += 64 * NN) {
+  for (int i = tid; i < ncols * 32; i += 64 * NW) {
     const int col = i >> 5, d = 4 * (i & 31);
-    f32x4_t po[NN];
-    float2 ml[NN];
+    f32x4_t po[NW];
+    float2 ml[NW];
 #pragma unroll
-    for (int u = 0; u < NN; ++u) {
+    for (int u = 0; u < NW; ++u) {
       po[u] = reinterpret_cast<const f32x4_t*>(lds[u])[col * 32 + ((i & 31) ^ col)];
       ml[u] = ml_of[u][col];
     }
     const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
     Joined j;
-    j.add(po, ml, NN);
+    j.add(po, ml, NW);
     if (w.whole) {
       j.write(p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim + d);
       continue;
@@ -625,9 +624,9 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
   __syncthreads();
   if (!s_last) return;
   // few columns: several threads a (column, four values), a part of the splits each, joined through LDS
-  const int pairs = ncols * 32, parts = max(1, 64 * NN / pairs), each = (w.splits + parts - 1) / parts;
+  const int pairs = ncols * 32, parts = max(1, 64 * NW / pairs), each = (w.splits + parts - 1) / parts;
   f32x4_t* part_o = reinterpret_cast<f32x4_t*>(lds[0]);
-  for (int i = tid; i < parts * pairs; i += 64 * NN) {
+  for (int i = tid; i < parts * pairs; i += 64 * NW) {
     const int part = i / pairs, col = (i - part * pairs) >> 5, d = 4 * (i & 31);
     const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
     const size_t step = (size_t)w.n * heads, slot0 = ((size_t)w.part0 + w.r0 + r) * heads + h;
@@ -642,7 +641,7 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
   }
   if (parts == 1) return;
   __syncthreads();
-  for (int i = tid; i < pairs; i += 64 * NN) {
+  for (int i = tid; i < pairs; i += 64 * NW) {
     const int col = i >> 5, d = 4 * (i & 31);
     const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
     Joined j;
@@ -823,10 +822,10 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
   put(p, w, c, wave * 16);
 }
 
-template <bool F8>
-__global__ __launch_bounds__(64 * NN, 2) void attn_shared_narrow_kernel(AttnSharedParams p) {
-  __shared__ u32x4_t lds[NN][TC];
-  narrow<F8>(p, work_of<true>(p, 1, blockIdx.x / kKVHeads), lds);
+template <bool F8, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_shared_narrow_kernel(AttnSharedParams p) {
+  __shared__ u32x4_t lds[NW][TC];
+  narrow<F8, NW>(p, work_of<true>(p, 1, blockIdx.x / kKVHeads), lds);
 }
 
 // Both forms; the narrow items a workgroup each, or a wave each where they are short and many.
@@ -840,7 +839,7 @@ __global__ __launch_bounds__(64 * NN, 2) void attn_shared_both_kernel(AttnShared
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = item * NN + wave;
     if (mine < p.narrow_items) narrow_alone<F8>(p, work_of<true>(p, 1, mine), lds[wave]);
   } else {
-    narrow<F8>(p, work_of<true>(p, 1, item), lds);
+    narrow<F8, NN>(p, work_of<true>(p, 1, item), lds);
   }
 }
 
@@ -939,6 +938,7 @@ bool few_pairs(int rows, int gs) { return rows < 512 >> gs; }
 struct Plan {
   bool both, alone;
   int waves, wide, narrow;
+  int nwaves = NN;  // of the narrow kernel
   int splits(const Segment& x) const {
     // (16 tiles, four a wave, take as long as the join of two halves does)
     if (x.narrow && !x.parts && x.tiles <= 16) return 1;
@@ -994,7 +994,7 @@ Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs,
       wide[n_wide++] = x + i;
     }
   }
-  Plan best{false, false, 8, 1, 4};
+  Plan best{false, false, 8, 1, 4, NN};
   // narrow: a workgroup a CU, in whole rounds of its waves, two at least
   best.narrow = NN * (int)std::max<long long>(2, (narrow * kKVHeads + 256 * NN - 1) / (256 * NN));
   // (halves of unequal runs are no better than a run)
@@ -1003,6 +1003,10 @@ Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs,
   if (any_narrow) {
     for (int i = 0; i < n; ++i)
       if (x[i].n && x[i].narrow) narrow_items += best.splits(x[i]) * blocks_of(x[i], gs, kNarrowCols) * kKVHeads;
+    // A run of few tiles, where a workgroup has a CU for itself: by eight waves in two steps, not three (8 bits: 5 tiles 7.6 ->
+    // 7.2 us, 10 tiles 9.1 -> 8.7; of 16 tiles on, and with twice the bytes, a CU's loads take the time: 2-5% slower, and
+    // with more workgroups than CUs 18-49%).
+    if (fp8 && narrow_longest > NN && narrow_longest <= 3 * NN && narrow_items <= 256) best.nwaves = 8;
     narrow_us = 1.25 * ((std::min(best.narrow, narrow_longest) + NN - 1) / NN);
   }
   double least = 1e30;
@@ -1178,11 +1182,13 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
     IE_CHECK_LAUNCH();
   }
   if (narrow) {
-    const dim3 grid(narrow * kKVHeads), block(64 * NN);
-    if (fp8)
-      hipLaunchKernelGGL((attn_shared_narrow_kernel<true>), grid, block, 0, st, p);
+    const dim3 grid(narrow * kKVHeads), block(64 * plan.nwaves);
+    if (fp8 && plan.nwaves == 8)
+      hipLaunchKernelGGL((attn_shared_narrow_kernel<true, 8>), grid, block, 0, st, p);
+    else if (fp8)
+      hipLaunchKernelGGL((attn_shared_narrow_kernel<true, 4>), grid, block, 0, st, p);
     else
-      hipLaunchKernelGGL((attn_shared_narrow_kernel<false>), grid, block, 0, st, p);
+      hipLaunchKernelGGL((attn_shared_narrow_kernel<false, 4>), grid, block, 0, st, p);
     IE_CHECK_LAUNCH();
   }
   if (merge) {

@@ -530,16 +530,17 @@ __device__ __forceinline__ void narrow_tiles(const AttnSharedParams& p, const Wo
   }
 }
 
-// Adds the partials of `count` splits to j: four values of o and (m, l) of each; AGENT: of workgroups of this launch.
-template <bool AGENT>
-__device__ __forceinline__ void add_splits(Joined& j, const AttnSharedParams& p, size_t slot0, size_t step, int count,
-                                           int d) {
-  for (int s0 = 0; s0 < count; s0 += 8) {
+// Adds the partials from..end - 1 of a row and head to j, four values of o and (m, l) of each: slot_of(i) is the i-th's
+// slot.  AGENT: of workgroups of this launch.
+template <bool AGENT, typename Slot>
+__device__ __forceinline__ void add_splits(Joined& j, const AttnSharedParams& p, int from, int end, int d,
+                                           const Slot& slot_of) {
+  for (int s0 = from; s0 < end; s0 += 8) {
     f32x4_t po[8];
     float2 ml[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const size_t slot = slot0 + min(s0 + u, count - 1) * step;
+      const size_t slot = slot_of(min(s0 + u, end - 1));
       const float *o = p.part + slot * kHeadDim + d, *m = p.part_ml + 2 * slot;
       if constexpr (AGENT) {
         ml[u] = agent_load2(m);
@@ -550,7 +551,7 @@ __device__ __forceinline__ void add_splits(Joined& j, const AttnSharedParams& p,
         po[u] = *reinterpret_cast<const f32x4_t*>(o);
       }
     }
-    j.add(po, ml, count - s0);
+    j.add(po, ml, end - s0);
   }
 }
 
@@ -631,7 +632,8 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
     const int h = (w.g << gs) + (col & ((1 << gs) - 1)), r = col >> gs;
     const size_t step = (size_t)w.n * heads, slot0 = ((size_t)w.part0 + w.r0 + r) * heads + h;
     Joined j;
-    add_splits<true>(j, p, slot0 + part * each * step, step, min(each, w.splits - part * each), d);
+    add_splits<true>(j, p, part * each, min(part * each + each, w.splits), d,
+                     [&](int s) { return slot0 + s * step; });
     if (parts == 1) {
       j.write(p.out + ((size_t)(w.row0 + r) * heads + h) * kHeadDim + d);
     } else {
@@ -867,20 +869,22 @@ __global__ __launch_bounds__(256) void attn_shared_merge_kernel(AttnSharedParams
   if (k < 0 && (splits < 2 || is_narrow(n, p.group_shift, false))) return;  // (the whole workgroup)
   const int part = threadIdx.x / (32 * kEach), pair = (threadIdx.x >> 5) % kEach;
   const int h = blockIdx.x * kEach % heads + pair, d = (threadIdx.x & 31) * 4;
-  Joined j;
-  // this part's share of `count` splits
-  const auto add = [&](size_t slot0, size_t step, int count) {
-    const int each = (count + PARTS - 1) / PARTS, from = part * each;
-    add_splits<false>(j, p, slot0 + from * step, step, min(each, count - from), d);
-  };
+  size_t pre = 0, pre_step = 0;
+  int n_pre = 0;
   if (k >= 0) {
-    const int first = p.p_first[k], end = p.p_end[k], p_splits = p.p_splits[k], p_part0 = p.p_part0[k];
+    const int first = p.p_first[k], end = p.p_end[k], p_part0 = p.p_part0[k];
+    n_pre = p.p_splits[k];
     const int base = first ? __builtin_amdgcn_readlane(member_end, max(first - 1, 0)) : 0;
     const int all = __builtin_amdgcn_readlane(member_end, end - 1) - base;
     const int at = (b ? __builtin_amdgcn_readlane(member_end, before) : 0) - base + row - row0;
-    add(((size_t)p_part0 + at) * heads + h, (size_t)all * heads, p_splits);
+    pre = ((size_t)p_part0 + at) * heads + h, pre_step = (size_t)all * heads;
   }
-  add(((size_t)__builtin_amdgcn_readlane(part0, b) + row - row0) * heads + h, (size_t)n * heads, splits);
+  const size_t own = ((size_t)__builtin_amdgcn_readlane(part0, b) + row - row0) * heads + h, own_step = (size_t)n * heads;
+  // this part's share of the two lists, one behind the other
+  const int count = n_pre + splits, each = (count + PARTS - 1) / PARTS;
+  Joined j;
+  add_splits<false>(j, p, part * each, min(part * each + each, count), d,
+                    [&](int s) { return s < n_pre ? pre + s * pre_step : own + (s - n_pre) * own_step; });
   if constexpr (PARTS > 1) {
     __shared__ f32x4_t part_o[PARTS][kEach][32];
     __shared__ float2 part_ml[PARTS][kEach];

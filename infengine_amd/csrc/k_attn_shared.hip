@@ -33,8 +33,10 @@
 // kernel has them, do not fit the registers beside the raw codes (680-690 us).
 // A batch with wide and few narrow items runs both in one launch; short narrow items that would fill the chip by themselves
 // take a wave each there (64 sequences behind one prefix 50 -> 45 us).  Rows with a prefix, or cut wide items, are
-// joined by a launch of their own (4.8 us for 16 tokens, 6.8 for 64; joining the prefix's partials in the narrow
-// kernel, behind a count, took longer than that launch).
+// joined by a launch of their own (4.0 us for 16 tokens, 5.5 for 64; joining the prefix's partials in the narrow
+// kernel, behind a count, took longer than that launch).  Few prefix tiles a workgroup are bound by latency: 16 tokens
+// behind 4992 bf16 positions take 19.1 us, of the first launch's 11 us 1 the arguments, 1.6 the first loads' addresses
+// and the queries, 1.5 the first tile, 1.8 a tile, 1 the end.
 #include <algorithm>
 #include <atomic>
 #include <chrono>

@@ -978,13 +978,14 @@ double turns(const Rate& r, double items, double us, double even) {
 }
 
 // The launches with the least modelled time.  A workgroup starts and ends in 4 us and takes its tiles (1.5 more for the
-// masked ones of a run), a narrow one 1.25 for four; a launch more is 3, the join 4.5 and
+// masked ones of a run), a narrow one 1.25 for four, all narrow ones
+// what HBM takes for their keys; a launch more is 3, the join 4.5 and
 // 0.2 a split (0.06 by four threads), its partials written and read at 5 TB/s.  Within 10% of the best of 12 split counts
 // and both workgroup sizes over 13 batches of 1-2500 rows (1 x 200 rows over 16000 keys 345 us uncut, 79-85 in 8;
 // 2500 rows 72 uncut, 104 in two; 2 x 1000 over 4096 keys 148 and 152), and of 8 counts over 10 batches with
 // prefixes; within 12% over 8 of 1100-3500 rows, which fill one round and part of another.
 Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs, long long room) {
-  long long narrow = 0;
+  long long narrow = 0, narrow_runs = 0;
   int wide_longest = 0, narrow_longest = 0, narrow_items = 0;
   bool any_narrow = false;
   const Segment* wide[kMaxPrefixes + kMaxSeqs];
@@ -993,6 +994,7 @@ Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs,
     if (!x[i].n) continue;
     if (x[i].narrow) {
       narrow += (long long)x[i].tiles * blocks_of(x[i], gs, kNarrowCols);
+      narrow_runs += x[i].tiles;
       narrow_longest = std::max(narrow_longest, x[i].tiles);
       any_narrow = true;
     } else {
@@ -1015,6 +1017,8 @@ Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs,
     if (fp8 && narrow_longest > NN && narrow_longest <= 3 * NN && narrow_items <= 256) best.nwaves = 8;
     narrow_us = 1.25 * ((std::min(best.narrow, narrow_longest) + NN - 1) / NN);
   }
+  // what the narrow segments' keys take at 5.5 TB/s
+  const double narrow_hbm = 4 + narrow_runs * (double)(kKVHeads * BKEY) * (fp8 ? 2 * kHeadDim + 2 : 4 * kHeadDim) / 5.5e6;
   double least = 1e30;
   for (int form = 0; form < 4 && wide_longest; ++form) {
     const bool both = form >= 2, alone = form == 3;
@@ -1044,7 +1048,8 @@ Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs,
       double cost = std::max(both ? turns(r, items + small, (items * each + small * small_us) / (items + small), even)
                                   : turns(r, items, each, even),
                              4 + (plan.wide + 1.5) * r.c[0]);
-      if (!both && any_narrow) cost += 3 + turns(kRates[fp8][2], narrow_items, 4 + narrow_us, 0);
+      if (!both && any_narrow) cost += 3 + std::max(turns(kRates[fp8][2], narrow_items, 4 + narrow_us, 0), narrow_hbm);
+      if (both) cost = std::max(cost, narrow_hbm);
       if (parts || prefixes)
         cost += 4.5 + (few_pairs(rows, gs) ? 0.06 : 0.2) * most + parts * (kKVHeads << gs) * (kHeadDim + 2) * 4 * 2 / 5e6;
       if (cost < least) least = cost, best = plan;

@@ -978,11 +978,10 @@ double turns(const Rate& r, double items, double us, double even) {
 }
 
 // The launches with the least modelled time.  A workgroup starts and ends in 4 us and takes its tiles (1.5 more for the
-// masked ones of a run), a narrow one 1.25 for four, all narrow ones
-// what HBM takes for their keys; a launch more is 3, the join 4.5 and
-// 0.2 a split (0.06 by four threads), its partials written and read at 5 TB/s.  Within 10% of the best of 12 split counts
-// and both workgroup sizes over 13 batches of 1-2500 rows (1 x 200 rows over 16000 keys 345 us uncut, 79-85 in 8;
-// 2500 rows 72 uncut, 104 in two; 2 x 1000 over 4096 keys 148 and 152), and of 8 counts over 10 batches with
+// masked ones of a run), a narrow one 1.25 for four, and all narrow ones what HBM takes for their keys; a launch more is
+// 3, the join 4.5 and 0.2 a split (0.06 by four threads), its partials written and read at 5 TB/s.  Within 10% of the best
+// of 12 split counts and both workgroup sizes over 13 batches of 1-2500 rows (1 x 200 rows over 16000 keys 345 us uncut,
+// 79-85 in 8; 2500 rows 72 uncut, 104 in two; 2 x 1000 over 4096 keys 148 and 152), and of 8 counts over 10 batches with
 // prefixes; within 12% over 8 of 1100-3500 rows, which fill one round and part of another.
 Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs, long long room) {
   long long narrow = 0, narrow_runs = 0;

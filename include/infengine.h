@@ -525,8 +525,9 @@ IE_API int ie_attn_window_paged_fp8(ie_context* ctx, int n_seqs, const int* star
  * multiple of 64, at most the start_pos of each that has new rows) in common, the next group_seqs[1] those of
  * shared_len[1], and so on (HOST arrays; the n_groups groups hold all n_seqs sequences; a group may be one sequence
  * or share 0 positions).  Those keys are read once for the group's sequences of few rows, not once for each.  The
- * table rows of sequences with new rows name the shared pages each, as ie_kv_fork_paged leaves them; which of them is
- * read is not specified.  Otherwise ie_attn_window_paged's contract: every row sees what it sees there. */
+ * table rows of sequences with new rows name the shared pages each, as ie_kv_fork_paged leaves them; all may lack the
+ * same ones, and each those that none of its new rows sees (as ie_kv_compact_paged leaves them, with this window and
+ * sinks or larger ones).  Otherwise ie_attn_window_paged's contract: every row sees what it sees there. */
 IE_API int ie_attn_shared_paged(ie_context* ctx, int kv_format, int n_groups, const int* group_seqs,
                                 const int* shared_len, int n_seqs, const int* start_pos,
                                 const int* n_new, int window, int n_sinks, int n_q_heads,

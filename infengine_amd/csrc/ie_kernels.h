@@ -369,9 +369,9 @@ struct AttnSharedParams {
   int narrow_end[kMaxSeqs], wide_end[kMaxSeqs], splits[kMaxSeqs], part0[kMaxSeqs];
   int lo[kMaxSeqs], prefix[kMaxSeqs];
   // by prefix: items up to and with the prefix's; key splits; first partial row; its first member and
-  // one past the group's last sequence; shared blocks; the least first position
+  // one past the group's last sequence; shared blocks; the member with the least first position
   int p_item_end[kMaxPrefixes], p_splits[kMaxPrefixes], p_part0[kMaxPrefixes];
-  int p_first[kMaxPrefixes], p_end[kMaxPrefixes], p_blocks[kMaxPrefixes], p_start[kMaxPrefixes];
+  int p_first[kMaxPrefixes], p_end[kMaxPrefixes], p_blocks[kMaxPrefixes], p_seq[kMaxPrefixes];
 };
 static_assert(sizeof(AttnSharedParams) <= 4096, "kernel arguments");
 struct SharedGroups {

@@ -60,7 +60,7 @@ struct Work {
   int p0, row0;     // own: position and batch row of the block's first row
   int first, end;   // prefix: its sequences
   int nkeys;        // keys of the segment: positions below
-  int seq;          // own: the sequence, whose table is read (prefix: the first's)
+  int seq;          // own: the sequence; prefix: the one furthest back, whose table is read
   bool prefix;
   bool whole;       // its rows have no other partials
   bool with_prefix; // they have a prefix's
@@ -111,7 +111,7 @@ __device__ __forceinline__ Work work_of(const AttnSharedParams& p, int waves, in
   if (w.prefix) {
     const int l = lane & 31;
     const int item_end = p.p_item_end[l], firsts = p.p_first[l], ends = p.p_end[l], splits = p.p_splits[l],
-              part0 = p.p_part0[l], starts = p.p_start[l], blocks = p.p_blocks[l];
+              part0 = p.p_part0[l], seqs = p.p_seq[l], blocks = p.p_blocks[l], starts = p.start[lane];
     const int k = __popcll(__ballot(lane < p.n_prefixes && item_end <= item));
     w.first = __builtin_amdgcn_readlane(firsts, k), w.end = __builtin_amdgcn_readlane(ends, k);
     w.splits = __builtin_amdgcn_readlane(splits, k), w.part0 = __builtin_amdgcn_readlane(part0, k);
@@ -119,10 +119,10 @@ __device__ __forceinline__ Work work_of(const AttnSharedParams& p, int waves, in
     w.row0 = w.first ? __builtin_amdgcn_readlane(member_end, max(w.first - 1, 0)) : 0;
     w.n = __builtin_amdgcn_readlane(member_end, w.end - 1) - w.row0;
     item -= k ? __builtin_amdgcn_readlane(item_end, max(k - 1, 0)) : 0;
-    w.p0 = __builtin_amdgcn_readlane(starts, k);
+    w.seq = __builtin_amdgcn_readlane(seqs, k);
+    w.p0 = __builtin_amdgcn_readlane(starts, w.seq);
     lo = 0, hi = __builtin_amdgcn_readlane(blocks, k);
     w.nkeys = hi * BKEY;
-    w.seq = w.first;
     w.whole = w.with_prefix = false;
     pmax = w.nkeys - 1;
   } else {
@@ -1083,16 +1083,17 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
   for (int i = 0, b0 = 0; i < g.n; b0 += g.seqs[i++]) {
     const int b1 = b0 + g.seqs[i], blocks = g.shared[i] / BKEY;
     const auto member = [&](int b) { return s.n_new[b] && s.n_new[b] <= kMemberCols >> gs; };
-    int many = 0, least = kMaxLongCtx, first = b0;
+    int many = 0, back = b0, first = b0;
     for (int b = b0; b < b1; ++b) {
       if (!member(b)) continue;
-      if (!many++) first = b;
-      least = std::min(least, s.start[b]);
+      if (!many++) first = back = b;
+      if (s.start[b] < s.start[back]) back = b;
     }
     if (!blocks || many < 2) continue;
     const int k = p.n_prefixes++;
-    // (the first member's table row is read: one without new rows may be over, its pages gone)
-    p.p_first[k] = first, p.p_end[k] = b1, p.p_blocks[k] = blocks, p.p_start[k] = least;
+    // The table row of the member furthest back is read: behind a window the others' may have lost pages that it
+    // still sees, while what it has lost none of them sees.  (One without new rows may be over, its pages gone.)
+    p.p_first[k] = first, p.p_end[k] = b1, p.p_blocks[k] = blocks, p.p_seq[k] = back;
     for (int b = b0; b < b1; ++b)
       if (member(b)) p.prefix[b] = k, p.lo[b] = blocks;
   }
@@ -1110,7 +1111,7 @@ int launch_attn_shared(AttnSharedParams p, const SeqBatch& s, const SharedGroups
   for (int k = 0; k < p.n_prefixes; ++k) {
     const int n = p.member_end[p.p_end[k] - 1] - (p.p_first[k] ? p.member_end[p.p_first[k] - 1] : 0);
     keys += p.p_blocks[k] * BKEY;
-    const int tiles = run_of(p.p_start[k], p.p_blocks[k] * BKEY - 1, 0, p.p_blocks[k], p.window, p.n_sinks).count;
+    const int tiles = run_of(s.start[p.p_seq[k]], p.p_blocks[k] * BKEY - 1, 0, p.p_blocks[k], p.window, p.n_sinks).count;
     pre[k] = {n, tiles, (double)tiles, false, true};
   }
   for (int b = 0; b < s.n; ++b) {

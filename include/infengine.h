@@ -445,7 +445,9 @@ IE_API int ie_attn_window_paged(ie_context* ctx, int n_seqs, const int* start_po
  * n_pos[i] % 64 positions are copied, all layers, to page new_pages[i] (ignored where n_pos[i] is a multiple of
  * 64), later entries become -1.  block_tables: device [n_rows][table_stride], updated; the four
  * lists are HOST arrays.  A row may be forked several times, but not in the call that writes it; the
- * new pages must be no table's, each taken once.  A source page outside [0, n_pages) is not copied. */
+ * new pages must be no table's, each taken once.  A source page outside [0, n_pages) is not copied.
+ * kv_pages: a bf16 pool, or NULL where every n_pos[i] is a multiple of 64 and nothing is copied (other pools:
+ * with NULL a fork within a page is refused). */
 IE_API int ie_kv_fork_paged(ie_context* ctx, int n_forks, const int* src_rows,
                             const int* dst_rows, const int* n_pos, const int* new_pages,
                             void* kv_pages, int n_pages, int* block_tables, int n_rows,
@@ -458,7 +460,7 @@ IE_API int ie_kv_fork_paged(ie_context* ctx, int n_forks, const int* src_rows,
  * fewest moves: live ids >= the live count go to the free ids below it, both in ascending order, all layers.
  * Outputs (device): new_tables (may be block_tables), entries that went and ids outside
  * [0, n_pages) as -1; d_remap [n_pages], a page's new id or -1; d_counts: live pages, moved pages.
- * A page that several rows share is moved once.  n_pages up to 65536 (512 GiB).  workspace:
+ * A page that several rows share is moved once.  kv_pages: a bf16 pool of up to 65536 pages (512 GiB).  workspace:
  * ie_kv_compact_workspace_size(n_pages) bytes. */
 IE_API size_t ie_kv_compact_workspace_size(int n_pages);
 IE_API int ie_kv_compact_paged(ie_context* ctx, int n_rows, const int* seq_lens, int window,
@@ -491,8 +493,9 @@ IE_API int ie_sample_filtered(ie_context* ctx, int rows, int vocab, const float*
  *   x ~ c * 2^e,  e the least integer >= -110 with max |x| <= 448 * 2^e,  c the code nearest to x * 2^-e, ties to even,
  * so a value is off by at most 2^-4 of itself, or 2^-10 * 2^e if that is more; all NaN if the row holds an infinity
  * or a NaN.  Layer by layer, [32]: the codes [K|V][8][64][128], then the bytes e + 127 [K|V][8][64], position r's (of
- * the page's 64) at index 4 * (r % 16) + r / 16.  Pools move by whole pages (ie_kv_fork_paged shares full pages
- * of any pool; its copy of a partly filled one, and ie_kv_compact_paged, are for bf16 pools). */
+ * the page's 64) at index 4 * (r % 16) + r / 16.  Pools move by whole pages: ie_kv_fork_paged shares full pages
+ * of any pool (given NULL for an 8-bit one, it refuses to copy a partly filled page, which it does, as
+ * ie_kv_compact_paged moves pages, by a bf16 pool's strides). */
 #define IE_KV_BF16 0
 #define IE_KV_FP8 1
 IE_API size_t ie_kv_page_size_fp8(void);

@@ -1792,8 +1792,7 @@ int ie_kv_fork_paged(ie_context* c, int n_forks, const int* src_rows, const int*
                      const int* n_pos, const int* new_pages, void* kv_pages, int n_pages,
                      int* block_tables, int n_rows, int table_stride) {
   IE_REQUIRE(c != nullptr, "kv_fork_paged: null context");
-  IE_REQUIRE(src_rows && dst_rows && n_pos && new_pages && kv_pages && block_tables,
-             "kv_fork_paged: null pointer");
+  IE_REQUIRE(src_rows && dst_rows && n_pos && new_pages && block_tables, "kv_fork_paged: null pointer");
   IE_REQUIRE(n_forks >= 0 && n_forks <= IE_MAX_SEQS, "kv_fork_paged: %d forks out of [0, %d]",
              n_forks, IE_MAX_SEQS);
   IE_REQUIRE(n_pages >= 1 && n_rows >= 1, "kv_fork_paged: n_pages %d, n_rows %d", n_pages, n_rows);
@@ -1807,6 +1806,7 @@ int ie_kv_fork_paged(ie_context* c, int n_forks, const int* src_rows, const int*
                "kv_fork_paged: fork %d has %d positions, a row holds %d", i, n_pos[i],
                table_stride * kPagePos);
     const bool copies = n_pos[i] % kPagePos != 0;
+    IE_REQUIRE(!copies || kv_pages, "kv_fork_paged: fork %d ends within a page, and there is no pool to copy in", i);
     IE_REQUIRE(!copies || (new_pages[i] >= 0 && new_pages[i] < n_pages),
                "kv_fork_paged: fork %d takes page %d of %d", i, new_pages[i], n_pages);
     for (int j = 0; j < n_forks; ++j) {

@@ -72,3 +72,16 @@ def test_shared_after_compaction(hip, ctx):
     torch.cuda.synchronize()
     want, tol = attend64(start, new, window, sinks, 32, q, pool, tables)
     check_attend(out, want, tol)
+
+
+def test_fork_without_a_pool(hip, ctx):
+    """Forks at full pages copy ids only: the pool, which may have any format, need not be given."""
+    say("fork without a pool")
+    tables = torch.arange(40, dtype=torch.int32, device="cuda").view(4, 10)
+    want = tables.clone()
+    want[1, 3:], want[3, :] = -1, -1
+    want[1, :3] = tables[0, :3]
+    hip.check(hip.lib.ie_kv_fork_paged(ctx.handle, 2, ints([0, 2]), ints([1, 3]), ints([192, 0]), ints([-1, -1]), None,
+                                       5, ptr(tables), 4, 10))
+    torch.cuda.synchronize()
+    assert torch.equal(tables, want)

@@ -59,9 +59,8 @@ struct ColumnState {
 // keys, + 4096 for keys + 16).  ks and db are XORs of the swizzled chunk.
 struct Frags {
   uint32_t k0, v0;
-  __device__ __forceinline__ Frags() : Frags(threadIdx.x) {}
-  __device__ __forceinline__ explicit Frags(int tid) {
-    const int fr = tid & 15, G = tid >> 4 & 3;
+  __device__ __forceinline__ Frags() {
+    const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3;
     k0 = (uint32_t)kv_slot(fr, G) * 16;
     v0 = (uint32_t)kv_slot(4 * G + (fr >> 2), (fr & 3) >> 1) * 16 + (fr & 1) * 8;
   }
@@ -89,14 +88,14 @@ __device__ __forceinline__ void scores(f32x4_t (&s)[QI][4], const ColumnState<QI
 }
 
 // Scores of keys that a column does not see to -inf.
-template <int QI, int KB>
-__device__ __forceinline__ void mask(f32x4_t (&s)[QI][KB], const ColumnState<QI>& c, int key0, int window, int n_sinks) {
+template <int QI>
+__device__ __forceinline__ void mask(f32x4_t (&s)[QI][4], const ColumnState<QI>& c, int key0, int window, int n_sinks) {
   int first = 4 * (threadIdx.x >> 4 & 3);  // the lane's first key in each 16
   asm volatile("" : "+v"(first));  // (opaque: nothing made of it is kept over the tiles)
 #pragma unroll
   for (int qi = 0; qi < QI; ++qi)
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int key = key0 + first + 16 * kb + r;
@@ -154,9 +153,9 @@ __device__ __forceinline__ void weights(bf16x8_t (&pb)[QI][2], ColumnState<QI>& 
 // The same as weights, rescaling only where a column's maximum has grown: in most tiles of a long run none has (8192 rows
 // over 4096 8-bit keys 607 -> 587 us).  (A reference that stays until the scores outgrow it by 2^8 saves 3% more, but the largest
 // weight is then rounded as all others are, where it is an exact 1 here: 0.0023 of error in place of 0.0020.)
-template <bool MASK, int QI, int KB>
-__device__ __forceinline__ void weights_grown(bf16x8_t (&pb)[QI][KB / 2], ColumnState<QI>& c,
-                                             f32x4_t (&s)[QI][KB], int key0, int window, int n_sinks) {
+template <bool MASK, int QI>
+__device__ __forceinline__ void weights_grown(bf16x8_t (&pb)[QI][2], ColumnState<QI>& c,
+                                             f32x4_t (&s)[QI][4], int key0, int window, int n_sinks) {
   if constexpr (MASK) mask(s, c, key0, window, n_sinks);
   float mn[QI];
   bool moved = false;
@@ -164,7 +163,7 @@ __device__ __forceinline__ void weights_grown(bf16x8_t (&pb)[QI][KB / 2], Column
   for (int qi = 0; qi < QI; ++qi) {
     float mt = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         mt = fmaxf(mt, s[qi][kb][r]);
@@ -190,12 +189,12 @@ __device__ __forceinline__ void weights_grown(bf16x8_t (&pb)[QI][KB / 2], Column
   for (int qi = 0; qi < QI; ++qi) {
     const float nb = -fmaxf(mn[qi], -3.0e38f) * kScoreScale;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         s[qi][kb][r] = __builtin_amdgcn_exp2f(fmaf(s[qi][kb][r], kScoreScale, nb));
 #pragma unroll
-    for (int ks2 = 0; ks2 < KB / 2; ++ks2) {
+    for (int ks2 = 0; ks2 < 2; ++ks2) {
       const u32x4_t w = {pack_bf2(s[qi][2 * ks2][0], s[qi][2 * ks2][1]),
                          pack_bf2(s[qi][2 * ks2][2], s[qi][2 * ks2][3]),
                          pack_bf2(s[qi][2 * ks2 + 1][0], s[qi][2 * ks2 + 1][1]),
@@ -205,11 +204,11 @@ __device__ __forceinline__ void weights_grown(bf16x8_t (&pb)[QI][KB / 2], Column
   }
 }
 
-// o += V^T . P^T and the sums, of 32 KS keys.  MASK: 0 x (an infinity or NaN) of a key that a column does not see must
+// o += V^T . P^T and the sums, of a tile.  MASK: 0 x (an infinity or NaN) of a key that a column does not see must
 // stay 0: such values are kept out of the product and added to the columns that see them.
 // AHEAD: the fragments of so many groups of 16 dims are read ahead of their products (0: as the compiler likes).
-template <bool MASK, int AHEAD = 0, int QI, int KS>
-__device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[QI][KS], const Frags& f,
+template <bool MASK, int AHEAD = 0, int QI>
+__device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[QI][2], const Frags& f,
                                        const u32x4_t* vtile, int key0, int window, int n_sinks) {
   const u32x4_t ones_w = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
   const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, ones_w);
@@ -217,14 +216,14 @@ __device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[
 #pragma unroll
   for (int qi = 0; qi < QI; ++qi)
 #pragma unroll
-    for (int ks2 = 0; ks2 < KS; ++ks2)
+    for (int ks2 = 0; ks2 < 2; ++ks2)
       c.l[qi] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[qi][ks2], c.l[qi], 0, 0, 0);
   uint32_t bad = 0;
 #pragma unroll
   for (int db = 0; db < 8; ++db) {
     if constexpr (MASK) __builtin_amdgcn_sched_barrier(0);  // (fewer fragments at once: registers)
 #pragma unroll
-    for (int ks2 = 0; ks2 < KS; ++ks2) {
+    for (int ks2 = 0; ks2 < 2; ++ks2) {
       const char* va = vb8 + f.v(db) + ks2 * 8192;
       const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)va);
       const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(va + 4096));
@@ -246,12 +245,12 @@ __device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[
   }
   if constexpr (!MASK && AHEAD > 0) {
     // (0x100: LDS reads, 0x8: MFMAs; the sums' come first)
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * KS * AHEAD, 0);
-    __builtin_amdgcn_sched_group_barrier(0x8, QI * KS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4 * AHEAD, 0);
+    __builtin_amdgcn_sched_group_barrier(0x8, 2 * QI, 0);
 #pragma unroll
     for (int db = 0; db < 8; ++db) {
-      if (db + AHEAD < 8) __builtin_amdgcn_sched_group_barrier(0x100, 2 * KS, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, QI * KS, 0);
+      if (db + AHEAD < 8) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 2 * QI, 0);
     }
   }
   if constexpr (MASK) {
@@ -261,7 +260,7 @@ __device__ __forceinline__ void values(ColumnState<QI>& c, const bf16x8_t (&pb)[
 #pragma unroll
       for (int qi = 0; qi < QI; ++qi) {
 #pragma unroll 1
-        for (int key = 0; key < 32 * KS; ++key) {
+        for (int key = 0; key < BKEY; ++key) {
           const int k = key0 + key;
           const bool seen = k <= c.pos[qi] && (k > c.pos[qi] - window || k < n_sinks);
 #pragma unroll
@@ -302,11 +301,10 @@ __device__ __forceinline__ void issue_tile(u32x4_t* stage, __amdgpu_buffer_rsrc_
   for (int j = 0; j < 16 / NW; ++j)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(stage + (ld.wave + NW * j) * 64), 16, ld.voff[j], 0, 0, AUX);
 }
-// How the rows at positions wp0 .. wp1 see the keys from key0 on.
+// How the rows at positions wp0 .. wp1 see the tile of keys from key0 on.
 enum Sight { kNone, kSome, kAll };
-template <int KEYS = BKEY>
 __device__ __forceinline__ Sight sight(int key0, int wp0, int wp1, int window, int n_sinks) {
-  const int last = key0 + KEYS - 1;
+  const int last = key0 + BKEY - 1;
   if (wp1 < wp0 || key0 > wp1 || (last <= wp0 - window && key0 >= n_sinks)) return kNone;
   return last <= wp0 && (key0 > wp1 - window || last < n_sinks) ? kAll : kSome;
 }

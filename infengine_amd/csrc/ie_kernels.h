@@ -358,7 +358,7 @@ struct AttnSharedParams {
   // set by the launcher
   float* part;              // partials [slots][heads][128], then (m, l)
   float* part_ml;
-  unsigned long long* arrived;  // [seqs][4 blocks][8 kv heads]: the last split to arrive joins them
+  unsigned long long* arrived;  // [seqs][8 kv heads]: the last split to arrive joins them
   unsigned long long tag;
   int n_seqs, n_prefixes, prefix_items, wide_items, narrow_items;
   int merge_row0;           // first row of a launch of the join

@@ -50,7 +50,6 @@ namespace {
 
 constexpr int NN = 4;  // waves of the narrow form's workgroups (8 where the plan says so)
 constexpr int kNarrowCols = 16;
-constexpr int kNarrowBlocks = 4;  // of a sequence, at most
 
 // A workgroup's work: rows r0 .. r0 + nr - 1 of a segment of n rows, one kv head, the tiles i0 .. i1 - 1
 // of the segment's run: na blocks from a0 on (sinks), then those from b0 on.
@@ -89,8 +88,9 @@ __host__ __device__ __forceinline__ Run run_of(int p0, int p1, int lo, int hi, i
 
 // Sequences of up to so many columns share a prefix; others fill blocks of the wide form by themselves.
 constexpr int kMemberCols = 64;
-// A sequence's own keys go to the narrow form: up to 16 columns; and those of members (few beside the prefix's, and
-// joined to it by the narrow form), in blocks of 16.  A prefix never does.
+// A sequence's own keys go to the narrow form: up to 16 columns, one block; and those of members, in blocks of 16.  (A member's
+// long own keys are then read by each of its blocks: 4 x 16 rows of 32 heads over 20000 own keys of 8 bits take 70 us
+// behind 64 shared positions, 49 without the group.)  A prefix never does.
 __host__ __device__ __forceinline__ bool is_narrow(int n, int gs, bool member) {
   return n <= (member ? kMemberCols : kNarrowCols) >> gs;
 }
@@ -606,13 +606,13 @@ __device__ __forceinline__ void narrow(const AttnSharedParams& p, const Work& w,
     if (d == 0) agent_store2(p.part_ml + 2 * slot, j.M, j.L);
   }
   if (w.whole || w.with_prefix) return;
-  // The last split of the block and kv head to arrive joins them, in the splits' order.  The word that
-  // counts them is the caller's memory, which may hold anything: a count is one with this call's tag,
-  // whatever else is there counts as none.  The last leaves 0.
+  // The last split of the sequence (one block: up to 16 columns) and kv head to arrive joins them, in the splits'
+  // order.  The word that counts them is the caller's memory, which may hold anything: a count is one with this
+  // call's tag, whatever else is there counts as none.  The last leaves 0.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the partials are there, before the arrival counts
   __syncthreads();
   if (tid == 0) {
-    unsigned long long* word = p.arrived + ((size_t)w.seq * kNarrowBlocks + w.r0 / (kNarrowCols >> gs)) * kKVHeads + w.g;
+    unsigned long long* word = p.arrived + w.seq * kKVHeads + w.g;
     unsigned long long cur = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), next = 0;
     // (without this call's tag: the first to put it there counts one; with it, it stays until the last)
     while (cur >> 16 != p.tag && !next)
@@ -914,8 +914,7 @@ long long part_rows(int rows, int heads) {
   return (long long)std::min(rows, 64) * kMaxSplits + 2ll * members_of(rows, heads);
 }
 
-static_assert(kMemberCols <= kNarrowBlocks * kNarrowCols);
-constexpr size_t kArrivedBytes = (size_t)kMaxSeqs * kNarrowBlocks * kKVHeads * sizeof(unsigned long long);
+constexpr size_t kArrivedBytes = (size_t)kMaxSeqs * kKVHeads * sizeof(unsigned long long);
 
 // A call's tag of the arrival counts, 48 bits.
 unsigned long long next_tag() {

@@ -4,13 +4,13 @@
 //
 // The row at position p sees the keys j <= p with j > p - window or j < n_sinks whose page is there:
 //   o = sum_j softmax_j(q . k_j / sqrt(128)) v_j,  zeros where it sees none.
-// An 8-bit row stands for its codes times its scale 2^e.  Scores of 8-bit keys: one 16x16x128 scaled product takes the
-// codes as they lie, with the keys' scales in its own scale operand (a lane's dword is the scales of its four
-// rows), and the queries as two e4m3 operands (Query8), which lose nothing against bf16.  Two such products cost as
-// much as the bf16 ones of the same keys, without a conversion or a second byte.  Values become bf16, exactly, on their way
-// to LDS: their scales go with the summed index, where the scaled product has none.  The rest is k_attn_window.hip's:
-// S^T = K . Q^T, online softmax, O^T = V^T . P^T in bf16 with fp32 sums, weights rounded to bf16 (2^-8 of a weight, the
-// sum is of the rounded ones).
+// An 8-bit row stands for its codes times its scale 2^e, exact in bf16 (past its largest, an infinity); keys and values
+// become that on their way to the products, which are k_attn_window.hip's: S^T = K . Q^T, online softmax, O^T = V^T . P^T in bf16 with fp32 sums, weights
+// rounded to bf16 (2^-8 of a weight, the sum is of the rounded ones).  The matrix unit would take the codes as they lie,
+// with the scales in an operand of their own and the queries in two e4m3 parts, at twice the rate; but its 8-bit products
+// are summed eight at a time to 13 bits below the largest of the eight (measured, with and without scales: a product of less
+// than 2^-13 of its neighbour adds nothing), so that a channel in which keys and queries are large takes the
+// others' bits: scores of products of up to 53 came out 5 times further off than the bf16 roundings allow.
 //
 // Softmax over a union of key sets is joined from (o, m, l) of each.  So the keys that a group of sequences
 // shares are attended once, by the rows of all of them (a prefix segment: rows of different sequences
@@ -27,10 +27,8 @@
 // 128, half a tile at a time, 16 tokens over 4096 keys take 92 us, not 30).  Bound by latency for few keys (one token
 // over 600 keys 8.7 us, of which the launch is 3; over 60000 33), by HBM past that (16 tokens over 4096
 // keys each 29.9, 4.5 TB/s; 5.7 but for the 9 of a run of one tile).  Splits are joined by the last to arrive.
-// Wide (4 or 8 waves of 16 columns): the tiles are staged in LDS for all waves, double-buffered; 8-bit
-// values pass through registers.  Bound by the vector units (busy 61% of the cycles) beside the matrix units (45%) and
-// LDS (43%): 8192 rows over 4096 keys 571-595 us, 0.94-0.98 PFLOP/s.  32 columns a wave, as the bf16
-// kernel has them, do not fit the registers beside the raw codes (680-690 us).
+// Wide (4 or 8 waves of 16 columns): the tiles are staged in LDS for all waves, bf16 ones directly and
+// double-buffered, 8-bit ones through registers: 8192 rows over 4096 keys 611-622 us, 0.90-0.92 PFLOP/s.
 // A batch with wide and few narrow items runs both in one launch; short narrow items that would fill the chip by themselves
 // take a wave each there (64 sequences behind one prefix 50 -> 45 us).  Rows with a prefix, or cut wide items, are
 // joined by a launch of their own (4.0 us for 16 tokens, 5.5 for 64; joining the prefix's partials in the narrow
@@ -182,73 +180,25 @@ __device__ __forceinline__ RowPos row_of(const AttnSharedParams& p, const Work& 
   return RowPos{rows + at - before, __shfl(start, b, 64) + at - before};
 }
 
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
-
-// 32 values q as two e4m3 operands: q 2^-e = c1 + 2^-4 c2 with c1 the nearest codes (4 bits of the 8 that a bf16
-// has) and c2 those of what is left (the others).  Values of at least 2^-15 of the column's largest are exact, smaller
-// ones off by at most 2^-22 of it: as much as the fp32 sums of their products.
-struct Query8 {
-  i32x8_t c1, c2;
-  int e1, e2;  // the exponents' bytes
-  // w: the lane's 32 values; a column's 128 are in lanes 16 apart
-  __device__ __forceinline__ void set(const u32x4_t (&w)[4]) {
-    float v[32];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t x = w[i >> 2][i & 3];
-      v[2 * i] = bf_lo(x), v[2 * i + 1] = bf_hi(x);
-      top = max(top, max(__float_as_uint(v[2 * i]) & 0x7FFFFFFFu, __float_as_uint(v[2 * i + 1]) & 0x7FFFFFFFu));
-    }
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-    const bool bad = top >= 0x7F800000u;  // an infinity or a NaN: the column's scores become NaN
-    e1 = bad ? 127 : scale_byte(top);
-    e2 = e1 - 4;
-    const float inv = __uint_as_float((uint32_t)(254 - e1) << 23);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float r[4];
-      int a = 0, b = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = v[4 * i + j] * inv;
-      a = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], a, false);
-      a = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], a, true);
-      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
-      b = __builtin_amdgcn_cvt_pk_fp8_f32((r[0] - lo[0]) * 16.f, (r[1] - lo[1]) * 16.f, b, false);
-      b = __builtin_amdgcn_cvt_pk_fp8_f32((r[2] - hi[0]) * 16.f, (r[3] - hi[1]) * 16.f, b, true);
-      c1[i] = bad ? 0x7F7F7F7F : a;
-      c2[i] = bad ? 0x7F7F7F7F : b;
-    }
-  }
-};
-
-template <bool F8>
+// CODES: of the keys' operands made of 16 codes a lane (NarrowK): the dims 64 j + 16 G .. +16, j 0 and 1, of a row, in
+// two operands each (which dims an operand holds is free, as long as keys and queries agree).
+template <bool CODES>
 struct Columns : ColumnState<1> {
-  Query8 q8;
   int least, most;  // of the wave's positions
-  u32x4_t raw[4];
 
-  // Columns past the rows repeat the last row.  8-bit operands: a lane has the dims 64 j + 16 G .. +16, j 0 and
-  // 1, of a row (which 32 is free, as long as keys and queries agree).
+  // Columns past the rows repeat the last row.
   __device__ __forceinline__ void load(const AttnSharedParams& p, const Work& w, int col0) {
     const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3, gs = p.group_shift;
     const int col = col0 + fr;
     const RowPos x = row_of(p, w, min(col >> gs, w.nr - 1));
     pos[0] = x.pos;
     const size_t at = ((size_t)x.row << gs << 3) + ((size_t)w.g << gs) + (col & ((1 << gs) - 1));
-    const u32x4_t* row = reinterpret_cast<const u32x4_t*>(p.q + at * kHeadDim);
+    const bf16x8_t* row = reinterpret_cast<const bf16x8_t*>(p.q + at * kHeadDim);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) raw[ks] = row[F8 ? 8 * (ks >> 1) + 2 * G + (ks & 1) : 4 * ks + G];
+    for (int ks = 0; ks < 4; ++ks) q[0][ks] = row[CODES ? 8 * (ks >> 1) + 2 * G + (ks & 1) : 4 * ks + G];
     clear();
   }
   __device__ __forceinline__ void set() {
-    if constexpr (F8) {
-      q8.set(raw);
-    } else {
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) q[0][ks] = __builtin_bit_cast(bf16x8_t, raw[ks]);
-    }
     int lo = pos[0], hi = pos[0];
 #pragma unroll
     for (int s = 1; s < 16; s <<= 1) {
@@ -259,16 +209,6 @@ struct Columns : ColumnState<1> {
     most = __builtin_amdgcn_readfirstlane(hi);
   }
 };
-
-// The scores of 16 keys' codes, whose scales are in byte KB of `scales` (a lane's for its row of the operand).
-template <int KB>
-__device__ __forceinline__ f32x4_t scores8(const Query8& q, const u32x4_t& a0, const u32x4_t& a1, uint32_t scales) {
-  const u32x4_t both[2] = {a0, a1};
-  const i32x8_t a = __builtin_bit_cast(i32x8_t, both);
-  f32x4_t s = {0.f, 0.f, 0.f, 0.f};
-  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.c2, s, 0, 0, KB, (int)scales, 0, q.e2);
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.c1, s, 0, 0, KB, (int)scales, 0, q.e1);
-}
 
 // Device-scope stores and loads: what one workgroup hands to another within a launch.
 __device__ __forceinline__ void agent_store2(float* p, float a, float b) {
@@ -355,12 +295,12 @@ __device__ __forceinline__ void put(const AttnSharedParams& p, const Work& w, co
 
 // ---------------------------------------------------------------- narrow form
 // A wave's K tile as operands: lane (fr, G) holds of the rows fr + 16 kb (kb 0 .. 3) the dims 32 ks + 8 G .. +8 (bf16),
-// or the codes 64 j + 16 G .. +16, j 0 and 1.
+// or the codes 64 j + 16 G .. +16, j 0 and 1, two operands each.
 template <bool F8, int AUX>
 struct NarrowK {
   static constexpr int kLoads = F8 ? 2 : 4;
   u32x4_t w[4][kLoads];
-  uint32_t scales;  // (of a row that is not there anything, its codes are zero: no row sees it)
+  uint32_t scales;  // (of a row that is not there anything: no row sees it)
   __device__ __forceinline__ void issue(const Planes& x, int g) {
     const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3;
     const int off = fr * (F8 ? kHeadDim : kRowBytes) + 16 * G;
@@ -374,20 +314,25 @@ struct NarrowK {
             x.k, off + kb * 16 * (F8 ? kHeadDim : kRowBytes) + 64 * j, 0, AUX);
   }
   __device__ __forceinline__ void scores(f32x4_t (&s)[1][4], const Columns<F8>& c) const {
-    if constexpr (F8) {
-      s[0][0] = scores8<0>(c.q8, w[0][0], w[0][1], scales);
-      s[0][1] = scores8<1>(c.q8, w[1][0], w[1][1], scales);
-      s[0][2] = scores8<2>(c.q8, w[2][0], w[2][1], scales);
-      s[0][3] = scores8<3>(c.q8, w[3][0], w[3][1], scales);
-    } else {
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
-        s[0][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int kb = 0; kb < 4; ++kb) {
+      u32x4_t a[4];
+      if constexpr (F8) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          s[0][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w[kb][ks]), c.q[0][ks],
-                                                             s[0][kb], 0, 0, 0);
+        for (int j = 0; j < 2; ++j) {
+          u32x4_t two[2];
+          chunks_of(two, w[kb][j], scale_of(scales >> (8 * kb) & 0xFF));
+          a[2 * j] = two[0], a[2 * j + 1] = two[1];
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) a[ks] = w[kb][ks];
       }
+      s[0][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        s[0][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a[ks]), c.q[0][ks], s[0][kb],
+                                                           0, 0, 0);
     }
   }
 };
@@ -670,81 +615,65 @@ __device__ __forceinline__ void narrow_alone(const AttnSharedParams& p, const Wo
 }
 
 // ---------------------------------------------------------------- wide form
-// K's codes in LDS: chunk c (16 codes) of row r at slot c ^ (r / 2 % 8) of its 8, so that 16 rows' reads of a chunk
-// column meet no bank twice.
-__device__ __forceinline__ int k8_slot(int r, int c) { return r * 8 + (c ^ ((r >> 1) & 7)); }
-
-// A thread's part of an 8-bit tile: of V chunk vchunk() of row vrow() (and of the row 32 on, with 4 waves), which becomes
-// bf16 on the way to LDS; K goes there directly, 8 rows a wave's load.  V's rows and chunks go over the lanes so that
-// eight lanes' stores are half a row and half of the row 4 on, whose swizzle differs: they meet no bank twice.
+// A thread's part of an 8-bit tile: chunk at() of row row() (and of the row 32 on, with 4 waves) of K and V, which become
+// bf16 on the way to LDS.  Rows and chunks go over the lanes so that eight lanes' stores are half a row and half of
+// the row 4 on, whose swizzle differs: they meet no bank twice.
 template <int NW>
 struct Wide8 {
   static constexpr int kEach = 8 / NW;
-  u32x4_t v[kEach];
-  uint32_t vs;      // the scales of rows vrow() % 16 + 16 i
-  uint32_t ks[2];   // those of K's rows fr + 16 i, of this tile and the next
+  u32x4_t k[kEach], v[kEach];
+  uint32_t ks, vs;  // the scales of rows row() % 16 + 16 i
   int rows;
-  static __device__ __forceinline__ int vrow() {
+  static __device__ __forceinline__ int row() {
     const int t = threadIdx.x;
     return (t >> 6) * 8 + (t >> 2 & 1) * 4 + (t >> 3 & 3);
   }
-  static __device__ __forceinline__ int vchunk() { return (threadIdx.x >> 5 & 1) * 4 + (threadIdx.x & 3); }
+  static __device__ __forceinline__ int at() { return (threadIdx.x >> 5 & 1) * 4 + (threadIdx.x & 3); }
   template <int AUX>
-  __device__ __forceinline__ void issue(u32x4_t* ktile, const Planes& x, int g, int wave) {
-    const int t = threadIdx.x, r = t >> 3;
+  __device__ __forceinline__ void issue(const Planes& x, int g) {
     rows = x.rows;
-    ks[0] = ks[1];
-    ks[1] = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (t & 15), g * kPagePos, AUX);
-    vs = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (vrow() & 15), (kKVHeads + g) * kPagePos, AUX);
+    ks = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (row() & 15), g * kPagePos, AUX);
+    vs = __builtin_amdgcn_raw_buffer_load_b32(x.scales, 4 * (row() & 15), (kKVHeads + g) * kPagePos, AUX);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {  // (the row 32 on has the same swizzle)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(x.k, (lds_void*)(ktile + (wave + NW * i) * 64), 16,
-                                               r * kHeadDim + (((t & 7) ^ ((r >> 1) & 7)) * 16), 32 * i * kHeadDim, 0,
-                                               AUX);
-      v[i] = __builtin_amdgcn_raw_buffer_load_b128(x.v, vrow() * kHeadDim + vchunk() * 16, 32 * i * kHeadDim, AUX);
+      k[i] = __builtin_amdgcn_raw_buffer_load_b128(x.k, row() * kHeadDim + at() * 16, 32 * i * kHeadDim, AUX);
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(x.v, row() * kHeadDim + at() * 16, 32 * i * kHeadDim, AUX);
     }
   }
-  __device__ __forceinline__ void stage(u32x4_t* vt, int wave) const {
-    const int c = 2 * vchunk();
+  __device__ __forceinline__ void stage(u32x4_t* kt, u32x4_t* vt, int wave) const {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int r = vrow() + 32 * i;
+      const int r = row() + 32 * i, byte = (wave >> 1) + 2 * i;  // (8 rows a wave)
+      const int first = kv_slot(r, 2 * at()), second = kv_slot(r, 2 * at() + 1);
       u32x4_t x[2];
-      chunks_of(x, v[i], scale_at_byte(vs, (wave >> 1) + 2 * i, r < rows));  // (8 rows a wave)
-      vt[kv_slot(r, c)] = x[0];
-      vt[kv_slot(r, c + 1)] = x[1];
+      chunks_of(x, k[i], scale_at_byte(ks, byte, r < rows));
+      kt[first] = x[0], kt[second] = x[1];
+      chunks_of(x, v[i], scale_at_byte(vs, byte, r < rows));
+      vt[first] = x[0], vt[second] = x[1];
     }
   }
 };
 
-template <int KB>
-__device__ __forceinline__ f32x4_t scores8_of(const Query8& q, const u32x4_t* ktile, uint32_t scales) {
-  const int fr = threadIdx.x & 15, G = threadIdx.x >> 4 & 3;
-  const int at = k8_slot(fr, G);  // (16 rows on, the same swizzle)
-  return scores8<KB>(q, ktile[at + KB * 128], ktile[(at ^ 4) + KB * 128], scales);
-}
-
 template <bool F8, int NW>
 __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u32x4_t* kt, u32x4_t* vt) {
-  constexpr int kStep = F8 ? TC / 2 : TC;  // from the first K tile to the second
   constexpr int kAhead = 2;
+  constexpr int kBuffer = F8 ? 0 : 1;  // (of two, or one)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool idle = (wave * 16) >> p.group_shift >= w.nr;  // (no rows)
   const bool nt = p.nt && w.nqb == 1;
   const TileLoad<NW> ld(wave);
   Wide8<NW> raw;
-  raw.ks[1] = 0;
   const auto planes = [&](int i, int page) { return planes_of<F8>(p, w.g, page, w.nkeys - w.tile(i) * BKEY); };
   // (past the last tile there are no bytes)
   const auto page_of = [&](int i) { return w.table[w.tile(min(i, w.i1 - 1))]; };
   const auto checked = [&](int i, int page) { return i < w.i1 ? __builtin_amdgcn_readfirstlane(page) : -1; };
-  // 8 bits: K to LDS, V to registers; bf16: both to LDS.
+  // 8 bits: to registers; bf16: to LDS.
   const auto issue = [&](int i, int page) {
     const Planes x = planes(i, page);
-    u32x4_t *ks = kt + (i & 1) * kStep, *vs = vt + (i & 1) * TC;
+    u32x4_t *ks = kt + (i & kBuffer) * TC, *vs = vt + (i & kBuffer) * TC;
     if constexpr (F8) {
-      if (nt) raw.template issue<2>(ks, x, w.g, wave);
-      else raw.template issue<0>(ks, x, w.g, wave);
+      if (nt) raw.template issue<2>(x, w.g);
+      else raw.template issue<0>(x, w.g);
     } else if (nt) {
       issue_tile<NW, 2>(ks, x.k, ld);
       issue_tile<NW, 2>(vs, x.v, ld);
@@ -761,34 +690,30 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
     page = checked(w.i0, here);
     issue(w.i0, page);
   }
-  Columns<F8> c;
+  Columns<false> c;
   c.load(p, w, wave * 16);
   c.set();
   // The compiler does not see what the kernel's own waits cover: without one here it would guard the
   // fragments inside the loops, where that is a wait for the tile in flight.
-  if constexpr (!F8) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   const Frags f;
 
-  // Tile i has landed and every wave is done with tile i - 1; tile i + 1 is on its way.  8 bits: tile i's V
-  // becomes bf16 in the buffer of tile i - 2, which every wave left before the last barrier.  (Making tile i + 1's after
-  // the barrier, a step ahead of its use, takes 4% longer: 8192 rows over 4096 keys 565 -> 588 us.)
+  // Tile i is there, for all waves; tile i + 1 is on its way.  bf16: it has landed in LDS, and every wave is done with tile
+  // i - 1, whose buffer tile i + 1 takes.  8 bits: it becomes bf16 in the one buffer, once every wave has left that; with
+  // two buffers, and no barrier before, a CU holds two workgroups of four waves, not three (6 x 333 rows 88 -> 68
+  // us, 8192 rows 626 -> 615).
   auto arrive = [&](int i) {
-    if constexpr (F8) raw.stage(vt + (i & 1) * TC, wave);
+    if constexpr (F8) {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      raw.stage(kt, vt, wave);
+    }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     page = checked(i + 1, next);
     issue(i + 1, page);
     next = page_of(i + 2);
   };
   auto tile_scores = [&](f32x4_t (&s)[1][4], int i) {
-    const u32x4_t* kc = kt + (i & 1) * kStep;
-    if constexpr (F8) {
-      s[0][0] = scores8_of<0>(c.q8, kc, raw.ks[0]);
-      s[0][1] = scores8_of<1>(c.q8, kc, raw.ks[0]);
-      s[0][2] = scores8_of<2>(c.q8, kc, raw.ks[0]);
-      s[0][3] = scores8_of<3>(c.q8, kc, raw.ks[0]);
-    } else {
-      scores(s, c, f, kc);
-    }
+    scores(s, c, f, kt + (i & kBuffer) * TC);
     __builtin_amdgcn_sched_barrier(0);
   };
   const auto see = [&](int i) {
@@ -806,7 +731,7 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
       bf16x8_t pb[1][2];
       tile_scores(s, i);
       weights_grown<false>(pb, c, s, 0, p.window, p.n_sinks);
-      values<false, kAhead>(c, pb, f, vt + (i & 1) * TC, 0, p.window, p.n_sinks);
+      values<false, kAhead>(c, pb, f, vt + (i & kBuffer) * TC, 0, p.window, p.n_sinks);
     }
     if (i == w.i1) break;
     const bool some = see(i) == kSome;
@@ -818,7 +743,7 @@ __device__ __forceinline__ void wide(const AttnSharedParams& p, const Work& w, u
       tile_scores(s, i);
       weights_grown<true>(pb, c, s, key0, p.window, p.n_sinks);
       __builtin_amdgcn_sched_barrier(0);  // (no fragments held over the softmax: registers)
-      values<true>(c, pb, f, vt + (i & 1) * TC, key0, p.window, p.n_sinks);
+      values<true>(c, pb, f, vt + (i & kBuffer) * TC, key0, p.window, p.n_sinks);
     }
     ++i;
   }
@@ -847,10 +772,10 @@ __global__ __launch_bounds__(64 * NN, 2) void attn_shared_both_kernel(AttnShared
   }
 }
 
-// (8-bit pages: 48 KiB of LDS)
 template <bool F8, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : F8 ? 3 : 2) void attn_shared_wide_kernel(AttnSharedParams p) {
-  __shared__ u32x4_t kt[F8 ? TC : 2 * TC], vt[2 * TC];
+  constexpr int kTiles = F8 ? 1 : 2;
+  __shared__ u32x4_t kt[kTiles * TC], vt[kTiles * TC];
   wide<F8, NW>(p, work_of<false>(p, NW, blockIdx.x / kKVHeads), kt, vt);
 }
 
@@ -959,7 +884,7 @@ struct Rate {
   double c[3];
 };
 constexpr Rate kRates[2][3] = {{{8, {1.92, 2.33, 0}}, {4, {1.75, 1.75, 0}}, {4, {1.75, 1.9, 0}}},    // bf16; the last:
-                               {{8, {1.35, 2.1, 0}}, {4, {1.16, 1.35, 1.79}}, {4, {1.2, 1.55, 0}}}};  // both forms
+                               {{8, {1.83, 2.1, 0}}, {4, {1.18, 1.5, 2.0}}, {4, {1.15, 1.6, 0}}}};  // both forms
 
 // The time of `items` workgroups of `us` (at one a CU) each, by the rates' growth with their number; even: 1 where they are
 // all as long as the longest, 0 where half as long in the mean.

@@ -151,7 +151,7 @@ __device__ __forceinline__ void weights(bf16x8_t (&pb)[QI][2], ColumnState<QI>& 
 }
 
 // The same as weights, rescaling only where a column's maximum has grown: in most tiles of a long run none has (8192 rows
-// over 4096 8-bit keys 607 -> 587 us).  (A reference that stays until the scores outgrow it by 2^8 saves 3% more, but the largest
+// over 4096 8-bit keys 673 -> 621 us).  (A reference that stays until the scores outgrow it by 2^8 saves 3% more, but the largest
 // weight is then rounded as all others are, where it is an exact 1 here: 0.0023 of error in place of 0.0020.)
 template <bool MASK, int QI>
 __device__ __forceinline__ void weights_grown(bf16x8_t (&pb)[QI][2], ColumnState<QI>& c,

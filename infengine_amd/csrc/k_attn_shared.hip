@@ -7,10 +7,11 @@
 // An 8-bit row stands for its codes times its scale 2^e, exact in bf16 (past its largest, an infinity); keys and values
 // become that on their way to the products, which are k_attn_window.hip's: S^T = K . Q^T, online softmax, O^T = V^T . P^T in bf16 with fp32 sums, weights
 // rounded to bf16 (2^-8 of a weight, the sum is of the rounded ones).  The matrix unit would take the codes as they lie,
-// with the scales in an operand of their own and the queries in two e4m3 parts, at twice the rate; but its 8-bit products
-// are summed eight at a time to 13 bits below the largest of the eight (measured, with and without scales: a product of less
-// than 2^-13 of its neighbour adds nothing), so that a channel in which keys and queries are large takes the
-// others' bits: scores of products of up to 53 came out 5 times further off than the bf16 roundings allow.
+// with the scales in an operand of their own and the queries in two e4m3 parts, in as many cycles (8192 rows over 4096 keys
+// 572 us, not 615); but it sums 8-bit products eight at a time to 13 bits below the largest of the eight (measured, with
+// and without scales: a product of less than 2^-13 of its neighbour adds nothing), so that a channel in which keys and
+// queries are large takes the others' bits: with products of up to 53 in the scores, outputs were 5 times further
+// off than the bf16 roundings allow.
 //
 // Softmax over a union of key sets is joined from (o, m, l) of each.  So the keys that a group of sequences
 // shares are attended once, by the rows of all of them (a prefix segment: rows of different sequences
@@ -25,12 +26,13 @@
 // within the sum is free, and Q's fragments are taken in the same order), V through registers into a tile of the
 // wave's own in LDS, from which it is read transposed.  No barrier, a tile of loads in flight a wave (256 registers: in
 // 128, half a tile at a time, 16 tokens over 4096 keys take 92 us, not 30).  Bound by latency for few keys (one token
-// over 600 keys 8.7 us, of which the launch is 3; over 60000 33), by HBM past that (16 tokens over 4096
-// keys each 29.9, 4.5 TB/s; 5.7 but for the 9 of a run of one tile).  Splits are joined by the last to arrive.
+// over 600 keys 8.6 us, of which the launch is 3; over 60000 33), by HBM past that (16 tokens over 4096
+// keys each 29.9, 4.5 TB/s; 6.5 but for the 9 of a run of one tile).  Splits are joined by the last to arrive.
 // Wide (4 or 8 waves of 16 columns): the tiles are staged in LDS for all waves, bf16 ones directly and
-// double-buffered, 8-bit ones through registers: 8192 rows over 4096 keys 611-622 us, 0.90-0.92 PFLOP/s.
+// double-buffered, 8-bit ones through registers.  Bound by the vector units (busy 54% of the cycles), LDS (48%) and
+// the matrix units (41%), partly one after the other: 8192 rows over 4096 keys 611-622 us, 0.90-0.92 PFLOP/s.
 // A batch with wide and few narrow items runs both in one launch; short narrow items that would fill the chip by themselves
-// take a wave each there (64 sequences behind one prefix 50 -> 45 us).  Rows with a prefix, or cut wide items, are
+// take a wave each there (64 sequences behind 1024 8-bit positions 19.5 -> 17.3 us, behind 16384 54 -> 51).  Rows with a prefix, or cut wide items, are
 // joined by a launch of their own (4.0 us for 16 tokens, 5.5 for 64; joining the prefix's partials in the narrow
 // kernel, behind a count, took longer than that launch).  Few prefix tiles a workgroup are bound by latency: 16 tokens
 // behind 4992 bf16 positions take 19.1 us, of the first launch's 11 us 1 the arguments, 1.6 the first loads' addresses
@@ -87,8 +89,8 @@ __host__ __device__ __forceinline__ Run run_of(int p0, int p1, int lo, int hi, i
 // Sequences of up to so many columns share a prefix; others fill blocks of the wide form by themselves.
 constexpr int kMemberCols = 64;
 // A sequence's own keys go to the narrow form: up to 16 columns, one block; and those of members, in blocks of 16.  (A member's
-// long own keys are then read by each of its blocks: 4 x 16 rows of 32 heads over 20000 own keys of 8 bits take 70 us
-// behind 64 shared positions, 49 without the group.)  A prefix never does.
+// long own keys are then read by each of its blocks: 4 x 16 rows of 32 heads over 20000 own keys of 8 bits take 77 us
+// behind 64 shared positions, 52 without the group.)  A prefix never does.
 __host__ __device__ __forceinline__ bool is_narrow(int n, int gs, bool member) {
   return n <= (member ? kMemberCols : kNarrowCols) >> gs;
 }
@@ -878,7 +880,8 @@ struct Plan {
 };
 
 // A form's time for a tile where 1, 2 or 3 workgroups share a CU (0: they do not fit), us.  Measured over 196 tiles
-// of 30 rows, 66 of 8192 rows and 67-126 of four sequences of 742-2500 rows (32 heads).
+// of 30 rows, 66 of 8192 rows and 67-126 of four sequences of 742-2500 rows (32 heads); 8 bits: by these and 25 more
+// batches, all counts of splits of each form.
 struct Rate {
   int waves;
   double c[3];
@@ -896,17 +899,18 @@ double turns(const Rate& r, double items, double us, double even) {
   // (the longest come first, so that more than a round ends evenly)
   const double mixed = each * r.c[most - 1] * items / round + 0.25 * us;
   if (items > 2 * round) return mixed;
-  // equal ones: the second round takes what its workgroups take by themselves (2048 rows over 2048 keys each 88 us, 2100 and
-  // 3000 rows 130 with 8 waves, 122 and 143 with 4)
+  // equal ones: the second round takes what its workgroups take by themselves (2048 rows over 2048 8-bit keys each 89 us, 2100
+  // and 3000 rows 134 with 8 waves, 128 and 150 with 4)
   return mixed + even * (each * r.c[most - 1] + part(items - round) - mixed);
 }
 
 // The launches with the least modelled time.  A workgroup starts and ends in 4 us and takes its tiles (1.5 more for the
 // masked ones of a run), a narrow one 1.25 for four, and all narrow ones what HBM takes for their keys; a launch more is
-// 3, the join 4.5 and 0.2 a split (0.06 by four threads), its partials written and read at 5 TB/s.  Within 10% of the best
-// of 12 split counts and both workgroup sizes over 13 batches of 1-2500 rows (1 x 200 rows over 16000 keys 345 us uncut,
-// 79-85 in 8; 2500 rows 72 uncut, 104 in two; 2 x 1000 over 4096 keys 148 and 152), and of 8 counts over 10 batches with
-// prefixes; within 12% over 8 of 1100-3500 rows, which fill one round and part of another.
+// 3, the join 4.5 and 0.2 a split (0.06 by four threads), its partials written and read at 5 TB/s.  8 bits: within 6% of the
+// best of 14 split counts and all forms over 29 batches of 1-8192 rows, with prefixes and without (1 x 200 rows over
+// 16000 keys 371 us uncut, 89 in 8; 2500 rows 79 uncut, 111 in two; 2 x 1000 over 4096 keys 165 and 177), within 12% over
+// six of 64 sequences behind a prefix.  bf16: within 12% over 13 batches, and over five of 64 sequences behind a prefix; a sixth, 64
+// rows behind 1024 positions with 200 of their own, takes 24 us, not 19.
 Plan plan_of(const Segment* x, int n, int rows, bool prefixes, bool fp8, int gs, long long room) {
   long long narrow = 0, narrow_runs = 0;
   int wide_longest = 0, narrow_longest = 0, narrow_items = 0;

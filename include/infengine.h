@@ -515,9 +515,9 @@ IE_API int ie_qk_norm_rope_paged_fp8(ie_context* ctx, int n_seqs, const int* sta
                                      const float* d_rope_cos, const float* d_rope_sin, int rope_rows,
                                      ie_bf16* d_q_out, void* fp8_pages, int n_pages,
                                      const int* block_tables, int table_stride, int layer);
-/* ie_attn_window_paged over an 8-bit pool, to its contract, with a workspace of
- * ie_attn_shared_workspace_size(rows, n_q_heads) bytes for at least the batch's rows, contents of no account (the
- * size never falls as rows grow). */
+/* ie_attn_window_paged over an 8-bit pool, to its contract: the keys and values are the bf16 ones that
+ * ie_kv_pages_from_fp8 gives.  workspace: ie_attn_shared_workspace_size(rows, n_q_heads) bytes for at least the
+ * batch's rows, contents of no account (the size never falls as rows grow). */
 IE_API size_t ie_attn_shared_workspace_size(int rows, int n_q_heads);
 IE_API int ie_attn_window_paged_fp8(ie_context* ctx, int n_seqs, const int* start_pos, const int* n_new,
                                     int window, int n_sinks, int n_q_heads, const ie_bf16* d_q,

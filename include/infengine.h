@@ -429,8 +429,9 @@ IE_API int ie_qk_norm_rope_paged(ie_context* ctx, int n_seqs, const int* start_p
  * (evicted pages; unlike ie_attn_prefill_core_paged, which reads them as zeros); a row that sees none
  * gets zeros, and so does one whose scores are all -inf.  Values at keys that a row does not see
  * never reach it, infinities and NaN included.
- * d_q, d_out: [rows][n_q_heads][128] (bf16).  Softmax and sums in fp32; the weights are rounded to bf16
- * for their product with V.  Few rows over many keys are split over the keys by a rule on all the
+ * d_q, d_out: [rows][n_q_heads][128] (bf16).  Softmax and sums in fp32, for sums q . k of up to 2^33 in size (the
+ * exponents' rounding, 2^-24 of the scaled score, goes past fp32's range from about there on); the weights are rounded
+ * to bf16 for their product with V.  Few rows over many keys are split over the keys by a rule on all the
  * lengths, on which the rounding depends.  d_out may be d_q.  workspace:
  * ie_attn_window_workspace_size(rows, n_q_heads) bytes for at least the batch's rows, contents of no account
  * (the size never falls as rows grow). */

@@ -113,3 +113,35 @@ def test_queries_of_any_magnitude(hip, ctx, power):
         torch.cuda.synchronize()
         outs.append((a, b))
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("sizes,lens,start,new", [
+    ([1], [0], [300], [2]), ([1], [0], [20000], [1]), ([1], [0], [300], [200]), ([3], [256], [300, 256, 310], [1, 2, 1]),
+])
+def test_scores_of_the_largest_size(hip, ctx, sizes, lens, start, new, sign, fmt):
+    """Sums q . k of nearly 2^33, all of one sign: a row's weight is all on the key of its largest, whose value it gets."""
+    say(f"shared, {8 if fmt else 16} bits: scores of 2^33, sign {sign}, {start} {new}")
+    g = gen(5 + sum(new))
+    n_pages, tables = shared_tables(g, sizes, lens, start, new)
+    kv = bf16(g, n_pages, 2, KVH, PAGE, D)
+    steps = torch.randint(1, 7, (n_pages, KVH, PAGE, 1), generator=g, device="cuda")
+    kv[:, 0] = (2.0**11 * (1 + steps / 8)).bfloat16()
+    # position 37 of every sequence has the largest score: 1.875 x 2^11 or, of negative scores, 2^11
+    kv[tables[:, 0].long(), 0, :, 37] = 2.0**11 * (1.875 if sign > 0 else 1.0)
+    kv[:, 1] = torch.randint(-15, 16, kv[:, 1].shape, generator=g, device="cuda").bfloat16() * 28    # (codes of scale 1)
+    pool = pool8(n_pages) if fmt else torch.zeros(n_pages, LAYERS, 2, KVH, PAGE, D, dtype=torch.bfloat16, device="cuda")
+    if fmt:
+        put8(pool, LAYER, kv)
+        assert torch.equal(bf16_pool(pool)[:, LAYER, 0], kv[:, 0])
+        kv = bf16_pool(pool)[:, LAYER]
+    else:
+        pool[:, LAYER] = kv
+    q = torch.full((sum(new), 32, D), sign * 2.0**14, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty_like(q)
+    shared(hip, ctx, fmt, sizes, lens, start, new, ALL, 0, 32, q, pool, tables, out)
+    torch.cuda.synchronize()
+    seq = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new)).cuda()
+    want = kv[tables[seq, 0].long(), 1, :, 37].repeat_interleave(4, 1)
+    assert torch.equal(out, want)
